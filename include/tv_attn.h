@@ -228,6 +228,68 @@ int tv_read_kv_blocks(void* k_out, void* v_out, const void* k_cache, const void*
                       int num_kv_heads, int head_dim, int block_size, int num_blocks,
                       int dtype, void* stream);
 
+/* ---- 8-bit K/V cache --------------------------------------------------------
+ * No counterpart in the reference, whose caches hold the model dtype.
+ * k_cache / v_cache hold e4m3 numbers [num_blocks, num_kv_heads, block_size,
+ * head_dim] (the rows of a block and head contiguous), k_scale / v_scale float
+ * [num_blocks, num_kv_heads] powers of two; an element stands for number *
+ * scale.  A scale below 2^-100 (a zeroed one) counts as 2^-100, and of any other
+ * positive number only the power of two counts.  dtype is that of the rows
+ * written, of the queries and of the values read back.  head_dim 64, 128 or 256,
+ * block_size at most 1024 (TV_EUNSUPPORTED otherwise).
+ */
+
+/*
+ * tv_reshape_and_cache for the 8-bit cache.  For a block and KV head the scale is
+ * the least 2^e, e >= -100, with amax <= 448 * 2^e over the rows that the call
+ * writes there.  A call that writes row 0 of a block starts it: the scale is the
+ * call's, and rows that the call does not write become zero.  Any other call
+ * keeps the larger of the block's scale and its own, and where that grew, the
+ * rows held are rounded again.  Numbers are x / 2^e rounded to nearest, ties to
+ * even; NaN and infinite elements are stored as NaN and count for no scale.  Of
+ * tokens with the same slot the last one is written.  Strides, negative slots and
+ * err_count are tv_reshape_and_cache's.  Two calls may overlap (streams) if they
+ * write different blocks.
+ */
+int tv_reshape_and_cache_fp8(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const void* k,
+                             const void* v, const int32_t* slot_mapping, int num_tokens, int num_kv_heads,
+                             int head_dim, int block_size, int num_blocks, int64_t k_stride, int64_t v_stride,
+                             int dtype, uint32_t* err_count, void* stream);
+
+/* tv_write_kv for the 8-bit cache: rows start_offset .. of one block, by the rule above. */
+int tv_write_kv_fp8(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const void* k, const void* v,
+                    int block_id, int start_offset, int num_tokens, int num_kv_heads, int head_dim, int block_size,
+                    int num_blocks, int64_t k_stride, int64_t v_stride, int dtype, void* stream);
+
+/*
+ * tv_read_kv_blocks for the 8-bit cache: the first context_len rows of the listed
+ * blocks as values, k_out / v_out [context_len, num_kv_heads, head_dim] of dtype
+ * (16-byte aligned; TV_F16 limits values to +-65504).
+ */
+int tv_read_kv_blocks_fp8(void* k_out, void* v_out, const void* k_cache, const void* v_cache, const float* k_scale,
+                          const float* v_scale, const int32_t* block_ids, int num_block_ids, int context_len,
+                          int num_kv_heads, int head_dim, int block_size, int num_blocks, int dtype, void* stream);
+
+/*
+ * tv_paged_decode over the 8-bit cache; arguments as there.  Differences: a
+ * context_lens[b] <= 0 gives zeros (there is no reference behaviour to keep), any
+ * number of query heads per KV head, partition_size a multiple of 32.  Rows past
+ * a context are not read.  A block id outside [0, num_blocks) among a sequence's
+ * attended ones gives NaN for that sequence.  The workspace is required for split
+ * contexts and optional otherwise (a longest-first schedule for 32 to 1024
+ * sequences); two launches that may overlap need one each.
+ */
+size_t tv_paged_decode_fp8_workspace_bytes(int num_seqs, int num_heads, int head_dim, int max_blocks, int block_size,
+                                           int partition_size);
+int tv_paged_decode_fp8_partition_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int max_blocks,
+                                       int block_size, int dtype);
+int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, const void* v_cache,
+                        const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                        const int32_t* context_lens, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                        int block_size, int num_blocks, int block_table_stride, int max_blocks, float scale,
+                        int dtype, int out_dtype, int partition_size, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,13 @@ SIGNATURES = {
     "tv_reshape_and_cache": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _L, _L, _I, _P, _P]),
     "tv_write_kv": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _L, _L, _I, _P]),
     "tv_read_kv_blocks": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "tv_reshape_and_cache_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _L, _L, _I, _P, _P]),
+    "tv_write_kv_fp8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _L, _L, _I, _P]),
+    "tv_read_kv_blocks_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "tv_paged_decode_fp8_workspace_bytes": (_S, [_I, _I, _I, _I, _I, _I]),
+    "tv_paged_decode_fp8_partition_size": (_I, [_I, _I, _I, _I, _I, _I, _I]),
+    "tv_paged_decode_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I,
+                                 _P, _S, _P]),
     # include/tv_llama.h
     "tv_linear_k_split": (_I, [_I, _I, _I]),
     "tv_linear_kernel": (_I, [_I, _I, _I, _I, _I, _I]),
@@ -55,7 +62,7 @@ SIGNATURES = {
     # include/tv_bench.h
     "tv_stream_read": (_I, [_P, _L, _I, _I, _I, _I, _P, _P]),
 }
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _lib = None
 

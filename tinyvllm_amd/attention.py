@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .kv_cache import check_fp8_cache
 
 _lib.load()
 
@@ -276,6 +277,71 @@ class PagedDecodePlan:
     def run(self):
         _lib.check(self.lib.tv_paged_decode(*self.args, _lib.stream_ptr(self.dev)), "PagedDecodePlan.run")
         return self.out
+
+
+class PagedDecodeFP8Plan:
+    """``PagedDecodePlan`` over an 8-bit cache: one layer's tensors of ``kv_cache.FP8KVCache``.
+
+    queries [B, 1, Hq, D]; k_cache / v_cache [NB, Hkv, bs, D] float8_e4m3fn; k_scale / v_scale
+    [NB, Hkv] float32.  The tensors are read on every ``run()`` and must keep their storage.
+    """
+
+    def __init__(self, queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
+                 n_heads, n_kv_heads, head_dim, block_size, max_context_len=None,
+                 *, partition_size=None, out_dtype=None):
+        self.lib = _lib.load()
+        self.dev = _on_gpu(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
+        nb, hkv, bs, d = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+        _require(queries.dim() == 4 and queries.shape[1] == 1,
+                 f"queries must be [B,1,Hq,D], got {tuple(queries.shape)}")
+        b = queries.shape[0]
+        _require(tuple(queries.shape) == (b, 1, n_heads, head_dim), "queries shape does not match n_heads/head_dim")
+        _require((hkv, bs, d) == (n_kv_heads, block_size, head_dim),
+                 f"cache shape {tuple(k_cache.shape)} does not match n_kv_heads/block_size/head_dim")
+        _require(n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
+        _require(block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32,
+                 "block_tables and context_lens must be int32")
+        _require(block_tables.dim() == 2 and block_tables.shape[0] == b, "block_tables must be [B, max_blocks]")
+        _require(context_lens.numel() == b, "context_lens must have B entries")
+        for t in (queries, block_tables, context_lens):
+            _require(t.is_contiguous(), "all inputs must be contiguous")
+        mb = block_tables.shape[1]
+        used = mb if max_context_len is None else min((int(max_context_len) + block_size - 1) // block_size, mb)
+        _require(used > 0, "no block table columns to attend over")
+        code = _lib.dtype_code(queries.dtype)
+        if partition_size is None:
+            partition_size = self.lib.tv_paged_decode_fp8_partition_size(b, n_heads, n_kv_heads, head_dim, used,
+                                                                         block_size, code)
+            _lib.check(0 if partition_size > 0 else _lib.TV_EINVAL, "paged_decode_attention_fp8")
+        self.partition_size = int(partition_size)
+        out_dtype = queries.dtype if out_dtype is None else out_dtype
+        self.out = torch.empty((b, 1, n_heads, head_dim), dtype=out_dtype, device=self.dev)
+        self.ws_bytes = self.lib.tv_paged_decode_fp8_workspace_bytes(b, n_heads, head_dim, used, block_size,
+                                                                     self.partition_size)
+        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.dev) if self.ws_bytes else None
+        self._inputs = (queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
+        self.args = (self.out.data_ptr(), queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                     k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(),
+                     b, n_heads, n_kv_heads, head_dim, block_size, nb, mb, used, 1.0 / math.sqrt(head_dim), code,
+                     _lib.dtype_code(out_dtype), self.partition_size,
+                     self.ws.data_ptr() if self.ws is not None else None, self.ws_bytes)
+
+    def run(self):
+        _lib.check(self.lib.tv_paged_decode_fp8(*self.args, _lib.stream_ptr(self.dev)), "PagedDecodeFP8Plan.run")
+        return self.out
+
+
+def paged_decode_attention_fp8(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
+                               n_heads, n_kv_heads, head_dim, block_size, max_context_len=None,
+                               *, partition_size=None, out_dtype=None):
+    """``paged_decode_attention`` over an 8-bit cache (one layer's tensors of ``kv_cache.FP8KVCache``; no
+    reference counterpart).  queries may be float32, float16 or bfloat16 whatever dtype the cache was
+    written from; head_dim 64, 128 or 256, any number of query heads per KV head.  A context of no tokens
+    gives zeros.  ``partition_size`` is a multiple of 32."""
+    plan = PagedDecodeFP8Plan(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, n_heads,
+                              n_kv_heads, head_dim, block_size, max_context_len, partition_size=partition_size,
+                              out_dtype=out_dtype)
+    return plan.run()
 
 
 class PrefillPlan:

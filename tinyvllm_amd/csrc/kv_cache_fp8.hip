@@ -1,0 +1,248 @@
+// Writing and reading the 8-bit paged cache (format, scales and layout: tv_fp8.h).
+//
+// kv_write_fp8_kernel.  Token t's K and V rows go to slot s_t, block s_t /
+// block_size, row s_t % block_size.  Per block touched, KV head and cache:
+//   amax   the largest finite magnitude among the rows that the call writes there
+//   e      the least exponent with amax <= 448 * 2^e; not below the block's
+//          present one, unless the call writes row 0: that starts the block anew
+//   rows   x * 2^-e rounded to e4m3; held rows are rounded again by 2^(old - e)
+//          where the exponent grew, and become zero where the block starts anew
+// A block's scale depends on all of the call's rows for it, so one work-group
+// owns a block (for heads_per_group of its heads) and no atomics are needed: the
+// work-group of the first token whose slot lies in the block.  It finds the
+// others by reading the slot list, which also settles a slot that is named twice
+// (the last token wins).  Only tokens whose predecessor lies in another block
+// read the list, one per 16 tokens of a prompt: 8192 tokens read it 512 times,
+// 32 KiB from L2 each, under the rows' own 25 MB.
+// Wave w takes (head, cache) pairs w, w + 4, ...: D / 8 lanes cover a row with
+// eight elements each, and up to kWriteHold rows a lane stay in registers from
+// the maximum to the rounding.
+#include "tv_fp8.h"
+
+namespace tv {
+
+constexpr int kWriteThreads = 256;
+constexpr int kWriteHold = 4;
+
+struct Row8 {
+  f32x4 a, b;
+};
+
+// Eight elements; `aligned` (uniform over the launch): their addresses are multiples of 16 bytes.
+template <typename T> __device__ __forceinline__ Row8 load_row8(const T* p, bool aligned) {
+  if (!aligned) {
+    Row8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.a[i] = to_float<T>(p[i]);
+      r.b[i] = to_float<T>(p[4 + i]);
+    }
+    return r;
+  }
+  if constexpr (sizeof(T) == 4) {
+    return Row8{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+  } else {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+    Row8 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x, y;
+      unpack2<T>(w[i], x, y);
+      r.a[2 * i] = x; r.a[2 * i + 1] = y;
+      unpack2<T>(w[2 + i], x, y);
+      r.b[2 * i] = x; r.b[2 * i + 1] = y;
+    }
+    return r;
+  }
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < __builtin_inff() ? a : 0.0f;
+}
+__device__ __forceinline__ float amax8(const Row8& r, float m) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(finite_abs(r.a[i]), finite_abs(r.b[i])));
+  return m;
+}
+__device__ __forceinline__ u32x2 round_row8(const Row8& r, float inv) {
+  return u32x2{f32x4_to_fp8(r.a * inv), f32x4_to_fp8(r.b * inv)};
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWriteThreads) kv_write_fp8_kernel(const KVWriteFp8Params p) {
+  constexpr int LPR = D / 8;        // lanes of a row
+  constexpr int RPI = 64 / LPR;     // rows a wave covers at once
+  __shared__ int winner[kFp8MaxBlock];   // token that writes row r of the block, or -1
+  const int t = blockIdx.x;
+  const int bs = p.block_size;
+  const long long num_slots = (long long)p.num_blocks * bs;
+  auto slot_of = [&](int i) { return p.slots ? (long long)p.slots[i] : (long long)p.base_slot + i; };
+
+  const long long slot = slot_of(t);
+  if (slot < 0) return;
+  if (slot >= num_slots) {
+    if (threadIdx.x == 0 && blockIdx.y == 0 && p.err_count) atomicAdd(p.err_count, 1u);
+    return;
+  }
+  const int blk = (int)(slot / bs);
+  const long long first = (long long)blk * bs;      // slots [first, first + bs) are the block's
+  if (t > 0) {
+    const long long before = slot_of(t - 1) - first;
+    if (before >= 0 && before < bs) return;         // an earlier token's work-group owns the block
+  }
+  for (int r = threadIdx.x; r < bs; r += kWriteThreads) winner[r] = -1;
+  __syncthreads();
+  bool earlier = false;
+  for (int i = threadIdx.x; i < p.num_tokens; i += kWriteThreads) {
+    const long long r = slot_of(i) - first;
+    if (r >= 0 && r < bs) {
+      earlier |= i < t;
+      atomicMax(&winner[(int)r], i);
+    }
+  }
+  if (__syncthreads_or(earlier ? 1 : 0)) return;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int lr = lane / LPR;
+  const int lc = (lane % LPR) * 8;
+  const int h0 = blockIdx.y * p.heads_per_group;
+  const int units = 2 * min(p.heads_per_group, p.num_kv_heads - h0);
+  const bool restart = winner[0] >= 0;
+  for (int u = wave; u < units; u += kWriteThreads / 64) {
+    const int h = h0 + (u >> 1);
+    const bool is_v = u & 1;
+    const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (size_t)h * D + lc;
+    const long long stride = is_v ? p.v_stride : p.k_stride;
+    uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + ((size_t)blk * p.num_kv_heads + h) * bs * D + lc;
+    float* scale = (is_v ? p.v_scale : p.k_scale) + (size_t)blk * p.num_kv_heads + h;
+    const int old_e = fp8_scale_exp_of(*scale);
+
+    Row8 held[kWriteHold];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kWriteHold; ++j) {
+      const int r = j * RPI + lr;
+      const int w = r < bs ? winner[r] : -1;
+      if (w >= 0) {
+        held[j] = load_row8<T>(src + (size_t)w * stride, p.aligned);
+        m = amax8(held[j], m);
+      }
+    }
+    for (int r = kWriteHold * RPI + lr; r < bs; r += RPI) {
+      const int w = winner[r];
+      if (w >= 0) m = amax8(load_row8<T>(src + (size_t)w * stride, p.aligned), m);
+    }
+    m = group_max<64>(m);
+    const int own_e = fp8_scale_exp(m);
+    const int e = restart ? own_e : max(own_e, old_e);
+    const float inv = exp2_int(-e);
+    const float again = exp2_int(max(old_e - e, -126));   // of held rows, where the exponent grew
+
+    auto put = [&](int r, const Row8& x) {
+      *reinterpret_cast<u32x2*>(dst + (size_t)r * D) = round_row8(x, inv);
+    };
+    auto keep = [&](int r) {
+      u32x2* q = reinterpret_cast<u32x2*>(dst + (size_t)r * D);
+      if (restart) {
+        *q = u32x2{0, 0};
+      } else if (e != old_e) {
+        const u32x2 w = *q;
+        *q = u32x2{f32x4_to_fp8(fp8_to_f32x4(w[0]) * again), f32x4_to_fp8(fp8_to_f32x4(w[1]) * again)};
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kWriteHold; ++j) {
+      const int r = j * RPI + lr;
+      if (r < bs) {
+        if (winner[r] >= 0) put(r, held[j]);
+        else keep(r);
+      }
+    }
+    for (int r = kWriteHold * RPI + lr; r < bs; r += RPI) {
+      const int w = winner[r];
+      if (w >= 0) put(r, load_row8<T>(src + (size_t)w * stride, p.aligned));
+      else keep(r);
+    }
+    if (lane == 0) *scale = exp2_int(e);
+  }
+}
+
+// Row t of the listed blocks as values q * 2^e; fp16 results are limited to
+// +-65504 (an e4m3 rounding of up to 2^-4 can pass fp16's largest number).  Ids
+// outside the cache read as 0.  Eight elements a lane, both caches.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_gather_fp8_kernel(const KVGatherFp8Params p) {
+  const int vec = p.head_dim / 8;
+  const long long row = (long long)p.num_kv_heads * vec;
+  const long long total = (long long)p.context_len * row;
+  for (long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x; idx < total;
+       idx += (long long)gridDim.x * blockDim.x) {
+    const int t = (int)(idx / row);
+    const int rest = (int)(idx - (long long)t * row);
+    const int h = rest / vec;
+    const int c = (rest - h * vec) * 8;
+    const int bi = t / p.block_size;
+    const int blk = p.block_ids[bi];
+    const bool ok = (unsigned)blk < (unsigned)p.num_blocks;
+    const size_t unit = (size_t)(ok ? blk : 0) * p.num_kv_heads + h;
+    const size_t at = (unit * p.block_size + (t - bi * p.block_size)) * p.head_dim + c;
+    const float f[2] = {ok ? exp2_int(fp8_scale_exp_of(p.k_scale[unit])) : 0.0f,
+                        ok ? exp2_int(fp8_scale_exp_of(p.v_scale[unit])) : 0.0f};
+    u32x2 w[2] = {u32x2{0, 0}, u32x2{0, 0}};
+    if (ok) {
+      w[0] = *reinterpret_cast<const u32x2*>(p.k_cache + at);
+      w[1] = *reinterpret_cast<const u32x2*>(p.v_cache + at);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f32x4 a = fp8_to_f32x4(w[i][0]) * f[i], b = fp8_to_f32x4(w[i][1]) * f[i];
+      T* out = reinterpret_cast<T*>(i ? p.v_out : p.k_out) + idx * 8;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4*>(out) = a;
+        *reinterpret_cast<f32x4*>(out + 4) = b;
+      } else {
+        if constexpr (ElemTraits<T>::kCode == kF16) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (fabsf(a[j]) > 65504.0f) a[j] = __builtin_copysignf(65504.0f, a[j]);
+            if (fabsf(b[j]) > 65504.0f) b[j] = __builtin_copysignf(65504.0f, b[j]);
+          }
+        }
+        *reinterpret_cast<u32x4*>(out) =
+            u32x4{pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]), pack2<T>(b[0], b[1]), pack2<T>(b[2], b[3])};
+      }
+    }
+  }
+}
+
+namespace {
+
+template <typename T>
+void write_of(const KVWriteFp8Params& p, dim3 grid, hipStream_t stream) {
+  if (p.head_dim == 64) hipLaunchKernelGGL((kv_write_fp8_kernel<T, 64>), grid, dim3(kWriteThreads), 0, stream, p);
+  else if (p.head_dim == 128) hipLaunchKernelGGL((kv_write_fp8_kernel<T, 128>), grid, dim3(kWriteThreads), 0, stream, p);
+  else hipLaunchKernelGGL((kv_write_fp8_kernel<T, 256>), grid, dim3(kWriteThreads), 0, stream, p);
+}
+
+}  // namespace
+
+void launch_kv_write_fp8(KVWriteFp8Params p, int dtype, hipStream_t stream) {
+  p.heads_per_group = 2;            // four (head, cache) pairs: one a wave
+  const dim3 grid(p.num_tokens, (p.num_kv_heads + p.heads_per_group - 1) / p.heads_per_group);
+  if (dtype == kF32) write_of<float>(p, grid, stream);
+  else if (dtype == kF16) write_of<_Float16>(p, grid, stream);
+  else write_of<__bf16>(p, grid, stream);
+}
+
+void launch_kv_gather_fp8(const KVGatherFp8Params& p, int dtype, hipStream_t stream) {
+  const long long total = (long long)p.context_len * p.num_kv_heads * (p.head_dim / 8);
+  const long long g = (total + 255) / 256;
+  const dim3 grid((unsigned)(g > 65536 ? 65536 : g));
+  if (dtype == kF32) hipLaunchKernelGGL(kv_gather_fp8_kernel<float>, grid, dim3(256), 0, stream, p);
+  else if (dtype == kF16) hipLaunchKernelGGL(kv_gather_fp8_kernel<_Float16>, grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL(kv_gather_fp8_kernel<__bf16>, grid, dim3(256), 0, stream, p);
+}
+
+}  // namespace tv

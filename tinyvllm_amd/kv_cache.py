@@ -118,6 +118,144 @@ class KVCache:
                                  slot_mapping, err_count=err_count)
 
 
+class FP8KVCache:
+    """Block-based K/V cache held in 8 bits, with ``KVCache``'s interface (no reference counterpart).
+
+    ``k_cache`` / ``v_cache`` hold e4m3 numbers [num_blocks, n_kv_heads, block_size, head_dim] per layer
+    and ``k_scale`` / ``v_scale`` a power of two for each block and KV head [num_blocks, n_kv_heads]
+    (float32); an element stands for number * scale.  ``dtype`` is the model's: rows are written from it
+    and read back in it.  A block's scale fits the rows written so far: writing its row 0 starts it
+    anew (rows that the call does not write become zero), and a later row that needs a larger scale has
+    the rows before it rounded again.  NaN and infinite elements are stored as NaN.  head_dim 64, 128
+    or 256, block_size at most 1024.
+    """
+
+    def __init__(self, num_layers, num_blocks, block_size, n_kv_heads, head_dim, dtype, device="cuda"):
+        self.num_layers = num_layers
+        self.num_blocks = num_blocks
+        self.block_size = block_size
+        self.n_kv_heads = n_kv_heads
+        self.head_dim = head_dim
+        self.dtype = as_torch_dtype(dtype)
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("FP8KVCache storage must be on a HIP device")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"FP8KVCache: head_dim {head_dim} not supported (64, 128, 256)")
+        if not 1 <= block_size <= 1024:
+            raise ValueError(f"FP8KVCache: block_size {block_size} not in 1..1024")
+        shape = (num_blocks, n_kv_heads, block_size, head_dim)
+
+        def zeros():
+            return [torch.zeros(shape, dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
+                    for _ in range(num_layers)]
+
+        def scales():      # the least scale: any row raises it
+            return [torch.full(shape[:2], 2.0 ** -100, dtype=torch.float32, device=self.device)
+                    for _ in range(num_layers)]
+
+        self.k_cache, self.v_cache = zeros(), zeros()
+        self.k_scale, self.v_scale = scales(), scales()
+
+    _rows = KVCache._rows
+
+    def write_kv(self, layer_idx, block_id, start_offset, k, v):
+        """Write k/v [T, Hkv, D] to rows start_offset .. start_offset + T - 1 of a block."""
+        k, ks = self._rows(k, "k")
+        v, vs = self._rows(v, "v")
+        if k.shape[0] != v.shape[0]:
+            raise ValueError("k and v must hold the same number of tokens")
+        lib = _lib.load()
+        rc = lib.tv_write_kv_fp8(
+            self.k_cache[layer_idx].data_ptr(), self.v_cache[layer_idx].data_ptr(),
+            self.k_scale[layer_idx].data_ptr(), self.v_scale[layer_idx].data_ptr(), k.data_ptr(), v.data_ptr(),
+            int(block_id), int(start_offset), k.shape[0], self.n_kv_heads, self.head_dim, self.block_size,
+            self.num_blocks, ks, vs, _lib.dtype_code(self.dtype), _lib.stream_ptr(self.k_cache[layer_idx].device))
+        _lib.check(rc, "FP8KVCache.write_kv")
+
+    def write_kv_slots(self, layer_idx, slot_mapping, k, v, err_count=None):
+        """Write token t of k/v [T, Hkv, D] to flat slot ``slot_mapping[t]`` (int32 device tensor) in one
+        launch; negative slots are skipped, of equal slots the last token is written, and ``err_count``
+        counts tokens whose slot is past the cache."""
+        return reshape_and_cache_fp8(self.k_cache[layer_idx], self.v_cache[layer_idx], self.k_scale[layer_idx],
+                                     self.v_scale[layer_idx], k, v, slot_mapping, err_count=err_count)
+
+    def read_kv_blocks(self, layer_idx, block_ids, context_len):
+        """(k, v) [context_len, Hkv, D] of ``dtype``: the rows of ``block_ids`` (a list, or an int32 tensor
+        on the device, which is read without a host copy) as values."""
+        kc = self.k_cache[layer_idx]
+        if isinstance(block_ids, torch.Tensor):
+            if block_ids.dtype != torch.int32 or block_ids.device != kc.device or not block_ids.is_contiguous():
+                raise ValueError("block_ids must be a contiguous int32 tensor on the cache's device")
+            count = block_ids.numel()
+        else:
+            count = len(block_ids)
+        n = min(int(context_len), count * self.block_size)
+        if n < 0:
+            raise ValueError("context_len must be >= 0")
+        k_out = torch.empty((n, self.n_kv_heads, self.head_dim), dtype=self.dtype, device=kc.device)
+        v_out = torch.empty_like(k_out)
+        if n == 0:
+            return k_out, v_out
+        ids = block_ids if isinstance(block_ids, torch.Tensor) else \
+            torch.tensor(list(block_ids), dtype=torch.int32).to(kc.device)
+        lib = _lib.load()
+        rc = lib.tv_read_kv_blocks_fp8(
+            k_out.data_ptr(), v_out.data_ptr(), kc.data_ptr(), self.v_cache[layer_idx].data_ptr(),
+            self.k_scale[layer_idx].data_ptr(), self.v_scale[layer_idx].data_ptr(), ids.data_ptr(), count, n,
+            self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, _lib.dtype_code(self.dtype),
+            _lib.stream_ptr(kc.device))
+        _lib.check(rc, "FP8KVCache.read_kv_blocks")
+        return k_out, v_out
+
+    def get_memory_bytes(self):
+        """Total bytes of the numbers and scales over all layers."""
+        return self.num_layers * self.num_blocks * self.n_kv_heads * 2 * (self.block_size * self.head_dim + 4)
+
+
+def check_fp8_cache(k_cache, v_cache, k_scale, v_scale):
+    """Shape [NB, Hkv, bs, D] of the tensors of one layer's 8-bit cache; raises ValueError."""
+    if k_cache.dim() != 4 or tuple(v_cache.shape) != tuple(k_cache.shape) or \
+            not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache / v_cache must be dense [NB, Hkv, bs, D] tensors of one shape")
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("k_cache / v_cache must be float8_e4m3fn")
+    nb, hkv, bs, d = k_cache.shape
+    for t in (k_scale, v_scale):
+        if t.dtype != torch.float32 or tuple(t.shape) != (nb, hkv) or not t.is_contiguous():
+            raise ValueError(f"k_scale / v_scale must be dense float32 [{nb}, {hkv}]")
+    for t in (v_cache, k_scale, v_scale):
+        if t.device != k_cache.device:
+            raise ValueError("all tensors must be on the cache's device")
+    return nb, hkv, bs, d
+
+
+def reshape_and_cache_fp8(k_cache, v_cache, k_scale, v_scale, k, v, slot_mapping, err_count=None):
+    """``reshape_and_cache`` into an 8-bit cache (one layer's tensors of ``FP8KVCache``)."""
+    nb, hkv, bs, d = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    if k.dim() != 3 or tuple(k.shape[1:]) != (hkv, d) or tuple(v.shape) != tuple(k.shape):
+        raise ValueError(f"k/v must be [T, {hkv}, {d}]")
+    if not (k.stride(2) == 1 and k.stride(1) == d and v.stride(2) == 1 and v.stride(1) == d):
+        raise ValueError("k/v heads and head_dim must be contiguous")
+    if k.dtype != v.dtype:
+        raise ValueError("k and v must share a dtype")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != k.shape[0] or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int32 with one entry per token")
+    dev = k_cache.device
+    for t in (k, v, slot_mapping):
+        if t.device != dev:
+            raise ValueError("all tensors must be on the cache's device")
+    if err_count is not None and (err_count.device != dev or err_count.dtype not in (torch.int32, torch.uint32)):
+        raise ValueError("err_count must be an int32/uint32 tensor on the cache's device")
+    t = k.shape[0]
+    rc = _lib.load().tv_reshape_and_cache_fp8(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(),
+        slot_mapping.data_ptr(), t, hkv, d, bs, nb, k.stride(0) if t > 1 else hkv * d,
+        v.stride(0) if t > 1 else hkv * d, _lib.dtype_code(k.dtype),
+        err_count.data_ptr() if err_count is not None else None, _lib.stream_ptr(dev))
+    _lib.check(rc, "reshape_and_cache_fp8")
+
+
 def reshape_and_cache(k_cache, v_cache, k, v, slot_mapping, err_count=None):
     """Fused cache write: ``cache[slot // bs, slot % bs] = row`` for every token."""
     nb, bs, hkv, d = k_cache.shape
