@@ -290,6 +290,25 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
                         int dtype, int out_dtype, int partition_size, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/*
+ * tv_flash_prefill_paged over the 8-bit cache; arguments as there.  Any block
+ * size the cache may have, any number of blocks and of query heads per KV head;
+ * fp16 / bf16 queries (TV_EUNSUPPORTED otherwise), 16-byte aligned rows.  A row
+ * that attends a key in a block outside [0, num_blocks), or a NaN in K or V, is
+ * NaN in that head; other rows are not touched by it.  workspace: of
+ * tv_flash_prefill_paged_fp8_workspace_bytes bytes (0 for grids that fill the
+ * device without it; depends on the current device), 16-byte aligned, lets the
+ * keys of few rows be split between work-groups; NULL runs them unsplit.
+ */
+size_t tv_flash_prefill_paged_fp8_workspace_bytes(int q_len, int start_pos, int num_heads, int num_kv_heads,
+                                                  int head_dim);
+int tv_flash_prefill_paged_fp8(void* out, const void* q, const void* k_cache, const void* v_cache,
+                               const float* k_scale, const float* v_scale, const int32_t* block_table,
+                               int num_blocks, int block_size, int q_len, int start_pos, int num_heads,
+                               int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride, int causal,
+                               float scale, int dtype, int out_dtype, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,21 +62,29 @@ def rows_ref(cache, scale, table, count):
     return x.transpose(0, 2, 1, 3).reshape(-1, cache.shape[1], cache.shape[3])[:count]
 
 
-def attend_ref(q, k, v, start, scale):
+def attend_ref(q, k, v, start, scale, causal=True, spread=False):
     """q [n, Hq, D] at positions start + i over keys j <= start + i of k, v [m, Hkv, D]: (out, bound),
-    where ``bound`` [n, Hq] is max_j sum_d |q k| * scale, the size of the sums behind a score."""
+    where ``bound`` [n, Hq] is max_j sum_d |q k| * scale, the size of the sums behind a score; with
+    ``spread`` also [n, Hq, D] sum_j p_j |v_j - out|, p the weights."""
     n, hq, d = q.shape
     m, hkv, _ = k.shape
     out = np.empty((n, hq, v.shape[2]))
+    dev = np.empty_like(out)
     bound = np.empty((n, hq))
     seen = np.arange(m)[None, :] <= np.arange(n)[:, None] + start
+    if not causal:
+        seen = np.ones_like(seen)
     for h in range(hq):
         kh, vh = k[:, h // (hq // hkv)], v[:, h // (hq // hkv)]
         s = np.where(seen, q[:, h] @ kh.T * scale, -np.inf)
         p = np.exp(s - s.max(1, keepdims=True))
-        out[:, h] = p @ vh / p.sum(1, keepdims=True)
+        p /= p.sum(1, keepdims=True)
+        out[:, h] = p @ vh
         bound[:, h] = (np.abs(q[:, h]) @ np.abs(kh).T * scale * seen).max(1)
-    return out, bound
+        if spread:
+            for i in range(n):
+                dev[i, h] = p[i] @ np.abs(vh - out[i, h])
+    return (out, bound, dev) if spread else (out, bound)
 
 
 def decode_ref(q, k8, v8, ks, vs, tables, ctx, scale):

@@ -21,3 +21,15 @@ def attention_bound(want, bound, vmax, n, d, dtype, out_dtype):
     parts = 2.0 ** -25 if dtype == "float32" else 2.0 ** -17
     rel = (terms + 8) * 2.0 ** -23 * bound[..., None] + 2.0 ** -22 + parts + n * 2.0 ** -23
     return 2 * vmax * rel + HALF_STEP[out_dtype] * (np.abs(want) + 2 * vmax * rel) + 2.0 ** -25   # fp16's least step / 2
+
+
+def rounded_weights_bound(want, bound, dev, vmax, n, d, dtype, out_dtype):
+    """The same where each weight is rounded to ``dtype`` (u = half a step of it) and the row sum is that of
+    the rounded weights: out = sum p (1 + e_j) v / sum p (1 + e_j) with |e_j| <= u is off by at most
+    2 u sum_j p_j |v_j - out| = 2 u dev (to first order; u^2 and an fp16 weight below its normal numbers,
+    2^-25 of one each, are covered by the margin of 1.05 and the n 2^-25 term).  Rescaled partial sums of
+    split keys are fp32."""
+    u = HALF_STEP[dtype]
+    rel = (d + 8) * 2.0 ** -23 * bound[..., None] + 2.0 ** -22 + n * 2.0 ** -23
+    off = 2.1 * u * dev + 2 * vmax * rel + (n * 2.0 ** -24 * vmax if dtype == "float16" else 0.0)
+    return off + HALF_STEP[out_dtype] * (np.abs(want) + off) + 2.0 ** -25

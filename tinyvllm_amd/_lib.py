@@ -43,6 +43,9 @@ SIGNATURES = {
     "tv_paged_decode_fp8_partition_size": (_I, [_I, _I, _I, _I, _I, _I, _I]),
     "tv_paged_decode_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I,
                                  _P, _S, _P]),
+    "tv_flash_prefill_paged_fp8_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
+    "tv_flash_prefill_paged_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _L, _L, _I, _F, _I,
+                                        _I, _P, _S, _P]),
     # include/tv_llama.h
     "tv_linear_k_split": (_I, [_I, _I, _I]),
     "tv_linear_kernel": (_I, [_I, _I, _I, _I, _I, _I]),

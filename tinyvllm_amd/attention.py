@@ -344,6 +344,39 @@ def paged_decode_attention_fp8(queries, k_cache, v_cache, k_scale, v_scale, bloc
     return plan.run()
 
 
+def flash_prefill_paged_fp8(queries, k_cache, v_cache, k_scale, v_scale, block_table, start_pos, causal=True, *,
+                            out_dtype=None):
+    """``flash_prefill_paged`` over an 8-bit cache (one layer's tensors of ``kv_cache.FP8KVCache``; no
+    reference counterpart): the chunk's rows attend the cached keys and the chunk's own, all as the
+    cache holds them.  fp16 / bf16 queries [1, n, Hq, D] or [n, Hq, D], head_dim 64, 128 or 256, any
+    block size.  Returns [1, n, Hq, D]."""
+    lib = _lib.load()
+    dev = _on_gpu(queries, k_cache, v_cache, k_scale, v_scale, block_table)
+    nb, hkv, bs, d2 = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    _require(queries.dim() in (3, 4) and (queries.dim() == 3 or queries.shape[0] == 1),
+             "queries must be [1, n, Hq, D] or [n, Hq, D]")
+    q = queries[0] if queries.dim() == 4 else queries
+    _require(q.stride(2) == 1 and q.stride(1) == q.shape[2], "queries: heads and head_dim must be contiguous")
+    n, hq, d = q.shape
+    _require(d == d2, "cache shape does not match the queries")
+    _require(hq % hkv == 0, "query heads must be a multiple of KV heads")
+    _require(block_table.dtype == torch.int32 and block_table.is_contiguous(), "block_table must be contiguous int32")
+    start_pos = int(start_pos)
+    _require(start_pos >= 0 and n > 0, "start_pos must be >= 0 and the chunk non-empty")
+    _require(block_table.numel() * bs >= start_pos + n, "block_table does not cover the sequence")
+    out_dtype = q.dtype if out_dtype is None else out_dtype
+    out = torch.empty((1, n, hq, d), dtype=out_dtype, device=dev)
+    ws_bytes = lib.tv_flash_prefill_paged_fp8_workspace_bytes(n, start_pos, hq, hkv, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    rc = lib.tv_flash_prefill_paged_fp8(
+        out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        block_table.data_ptr(), nb, bs, n, start_pos, hq, hkv, d, q.stride(0) if n > 1 else hq * d, hq * d,
+        1 if causal else 0, 1.0 / math.sqrt(d), _lib.dtype_code(q.dtype), _lib.dtype_code(out_dtype),
+        ws.data_ptr() if ws is not None else None, ws_bytes, _lib.stream_ptr(dev))
+    _lib.check(rc, "flash_prefill_paged_fp8")
+    return out
+
+
 class PrefillPlan:
     """Pre-validated, pointer-stable causal prefill for fixed [1, L, H, D] inputs."""
 

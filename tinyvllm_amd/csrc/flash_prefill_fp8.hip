@@ -1,0 +1,381 @@
+// Attention of a prompt's chunk over the 8-bit paged cache (format, scales and
+// layout: tv_fp8.h): query row i at position start_pos + i attends keys j <=
+// start_pos + i (causal) or all start_pos + q_len keys.
+//
+// Bound: the matrix cores, 4 D operations per (row, query head, key), and beside
+// them the vector unit (an exponential per score).  An 8-bit key or value costs a
+// conversion more than a 16-bit one, so it is made once per work-group, on the
+// way from registers to LDS, and the work-group's rows are as many as the shape
+// has: the query heads of a KV head are packed into one row index, row r = query
+// r / G of head r % G, so that a chunk of few rows still fills its tiles and all
+// G heads share one conversion.
+//
+// A work-group of 4 waves owns BM = 64 RB rows of one KV head, RB blocks of 16 a
+// wave, and walks tiles of BN keys: S^T = K Q^T with the key rows as operand A;
+// its accumulator layout is the B operand of O^T = V^T P^T (V read transposed
+// from LDS), so P stays in registers.  Tiles are double-buffered in LDS and one
+// more is on the way in registers: one barrier a tile.  Where the tiles of rows
+// are too few for the GPU, the keys are split between work-groups and a second
+// kernel joins their parts.
+// Numbers: K and V enter as their dequantised values in T, exact but for fp16's
+// range (values are limited to +-65504; below fp16's normal numbers they are
+// rounded as fp16 inputs that small are).  Scores, maxima, sums, accumulators are
+// fp32; a weight is rounded to T for the second product, as in the 16-bit prefill
+// kernels, and the row sum is that of the rounded weights.
+// A NaN in a key or value and a block id outside the cache show in the rows that
+// attend that key and in no others: the key's score becomes NaN, which the mask
+// replaces for rows that do not see it, and a NaN value is zero in LDS, since a
+// weight of zero would not hide it.  (The row is then NaN in every dim.)
+#include "tv_fp8.h"
+
+#include <algorithm>
+
+namespace tv {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T> constexpr uint32_t kNan2 = ElemTraits<T>::kCode == kF16 ? 0x7E007E00u : 0x7FC07FC0u;
+
+// Two e4m3 numbers times a power of two in T.
+template <typename T, bool HI> __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
+  if constexpr (ElemTraits<T>::kCode == kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+
+// Four e4m3 numbers as T; fp16 limited to its range (only scales of 2^8 and more leave it).
+template <typename T> __device__ __forceinline__ u32x2 dequant4(uint32_t w, float scale) {
+  if (ElemTraits<T>::kCode == kF16 && scale > 128.0f) {
+    f32x4 x = fp8_to_f32x4(w) * scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (fabsf(x[i]) > 65504.0f) x[i] = __builtin_copysignf(65504.0f, x[i]);
+    return u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+  }
+  return u32x2{scaled_pair<T, false>(w, scale), scaled_pair<T, true>(w, scale)};
+}
+
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+template <typename T, int D, int RB, int BN>
+__global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillFp8Params p) {
+  constexpr int BM = 64 * RB;
+  constexpr int KB = BN / 16;
+  constexpr int KSD = D / 32;
+  constexpr int DB = D / 16;
+  constexpr int P = D + 16;               // LDS row pitch (elements): conflict-free reads of both operands
+  constexpr int SKT = BN * P;
+  constexpr int BUF = 2 * SKT;            // K tile, then V tile
+  constexpr int CPR = D / 16;             // 16-number vectors of a row
+  constexpr int NV = BN * CPR / kThreads; // vectors per thread and tile, each of K and V
+  constexpr int RPP = kThreads / CPR;     // tile rows of one pass over the threads
+  static_assert(NV * kThreads == BN * CPR && NV >= 1, "tile shape");
+  __shared__ __attribute__((aligned(16))) uint16_t smem[2 * BUF];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int g = lane >> 4, col = lane & 15;
+  const int kh = blockIdx.x;
+  // the longest rows first: later row tiles see more keys
+  const int rt = gridDim.y - 1 - blockIdx.y;
+  const int split = blockIdx.z;
+  const int G = p.group;
+  const int rows = p.q_len * G;
+  const int kv_len = p.start_pos + p.q_len;
+  const int last_pos = min((rt + 1) * BM, rows) - 1;
+  const int kfull = p.causal ? min(kv_len, p.start_pos + last_pos / G + 1) : kv_len;
+  const int nkt = (kfull + BN - 1) / BN;
+  const int per = (nkt + p.splits - 1) / p.splits;
+  const int t0 = split * per, t1 = min(t0 + per, nkt);
+  const int row0 = rt * BM + wave * RB * 16;
+
+  int qrow[RB], qpos[RB];
+  u32x4 qf[RB][KSD];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    qrow[r] = row0 + r * 16 + col;
+    qpos[r] = qrow[r] / G;
+    const T* qg = reinterpret_cast<const T*>(p.q) + (size_t)qpos[r] * p.q_stride +
+                  (size_t)(kh * G + qrow[r] - qpos[r] * G) * D + g * 8;
+#pragma unroll
+    for (int ks = 0; ks < KSD; ++ks)
+      qf[r][ks] = qrow[r] < rows ? *reinterpret_cast<const u32x4*>(qg + ks * 32) : u32x4{0, 0, 0, 0};
+  }
+
+  // staging: this thread's vectors are chunk ch of tile rows sr + RPP i
+  const int sr = tid / CPR, ch = tid % CPR;
+  const int bs = p.block_size, lg = p.bs_log2;
+  auto column = [&](int key) { return lg >= 0 ? key >> lg : key / bs; };
+  struct Ids { int id[NV]; };
+  struct Stage { u32x4 k[NV], v[NV]; float ks[NV], vs[NV]; bool ok[NV], in[NV]; };
+  auto ids_of = [&](int t, Ids& x) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x.id[i] = p.block_table[column(min(t * BN + sr + RPP * i, kv_len - 1))];
+  };
+  auto gload = [&](int t, const Ids& x, Stage& s) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int key = t * BN + sr + RPP * i;
+      s.in[i] = key < kv_len && t < t1;
+      s.ok[i] = (unsigned)x.id[i] < (unsigned)p.num_blocks;
+      const size_t unit = (size_t)(s.ok[i] ? x.id[i] : 0) * p.num_kv_heads + kh;
+      const int k1 = min(key, kv_len - 1);
+      const size_t at = (unit * bs + (k1 - column(k1) * bs)) * D + ch * 16;
+      s.k[i] = *reinterpret_cast<const u32x4*>(p.k_cache + at);
+      s.v[i] = *reinterpret_cast<const u32x4*>(p.v_cache + at);
+      s.ks[i] = p.k_scale[unit];
+      s.vs[i] = p.v_scale[unit];
+    }
+  };
+  auto lstore = [&](const Stage& s, int b) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint16_t* dk = smem + b * BUF + (sr + RPP * i) * P + ch * 16;
+      u32x4 k = s.k[i], v = s.v[i];
+      if (!s.in[i]) k = v = u32x4{0, 0, 0, 0};   // keys past the last: masked, and their values zero
+      bool poison = s.in[i] && !s.ok[i];
+      if (poison || (nan_bytes(v[0]) | nan_bytes(v[1]) | nan_bytes(v[2]) | nan_bytes(v[3]))) {
+        poison = true;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t bad = (nan_bytes(v[j]) >> 7) * 0xffu;
+          v[j] = s.ok[i] ? v[j] & ~bad : 0u;
+        }
+      }
+      u32x2 kw[4], vw[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        kw[j] = dequant4<T>(k[j], s.ks[i]);
+        vw[j] = dequant4<T>(v[j], s.vs[i]);
+      }
+      if (poison) kw[0][0] = kNan2<T>;
+      *reinterpret_cast<u32x4*>(dk) = u32x4{kw[0][0], kw[0][1], kw[1][0], kw[1][1]};
+      *reinterpret_cast<u32x4*>(dk + 8) = u32x4{kw[2][0], kw[2][1], kw[3][0], kw[3][1]};
+      *reinterpret_cast<u32x4*>(dk + SKT) = u32x4{vw[0][0], vw[0][1], vw[1][0], vw[1][1]};
+      *reinterpret_cast<u32x4*>(dk + SKT + 8) = u32x4{vw[2][0], vw[2][1], vw[3][0], vw[3][1]};
+    }
+  };
+
+  f32x4 oacc[RB][DB + 1];
+  float m[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+#pragma unroll
+    for (int db = 0; db <= DB; ++db) oacc[r][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[r] = kNegInf;
+  }
+  const u32x4 ones = u32x4{kOnes2<T>, kOnes2<T>, kOnes2<T>, kOnes2<T>};
+  const float c = p.scale * kLog2e;
+  const int first_seen = p.causal ? p.start_pos + row0 / G : kv_len - 1;   // last key that all of the wave's rows see
+
+  auto compute = [&](int b, int t) {
+    const uint16_t* sk = smem + b * BUF;
+    const uint16_t* sv = sk + SKT;
+    const int k0 = t * BN;
+    f32x4 st[RB][KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int ks = 0; ks < KSD; ++ks) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + (kb * 16 + col) * P + ks * 32 + g * 8);
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+          st[r][kb] = mfma16x16x32<T>(kf, qf[r][ks], ks ? st[r][kb] : f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+    }
+    float base[RB];
+    bool need = false;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      base[r] = m[r] == kNegInf ? 0.0f : m[r];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st[r][kb][i] = fmaf(st[r][kb][i], c, -base[r]);
+    }
+    if (k0 + BN - 1 > first_seen) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const int rel = (p.causal ? min(kv_len - 1, p.start_pos + qpos[r]) : kv_len - 1) - (k0 + 4 * g);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[r][kb][i] = kb * 16 + i <= rel ? st[r][kb][i] : kNegInf;
+      }
+    }
+    // the running maximum is raised only when a tile passes it by 2^8
+    float mt[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      mt[r] = kNegInf;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        mt[r] = fmaxf(mt[r], fmaxf(fmaxf(st[r][kb][0], st[r][kb][1]), fmaxf(st[r][kb][2], st[r][kb][3])));
+      need |= mt[r] > (m[r] == kNegInf ? kNegInf : 8.0f);
+    }
+    if (__builtin_amdgcn_ballot_w64(need) != 0) {
+      __asm__ volatile("" ::: "memory");   // keeps this rare block a branch
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const float mm = max_over_g(mt[r]);               // relative to base
+        const bool raise = mm > (m[r] == kNegInf ? kNegInf : 8.0f);
+        const float delta = raise ? mm : 0.0f;
+        const float alpha = raise && m[r] != kNegInf ? fast_exp2(-delta) : 1.0f;
+        m[r] = raise ? base[r] + delta : m[r];
+#pragma unroll
+        for (int db = 0; db <= DB; ++db) oacc[r][db] *= alpha;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) st[r][kb] -= delta;
+      }
+    }
+    u32x4 pf[RB][BN / 32];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        // reduction index 8g + j: key 4g + j of block 2 x (j < 4), 4g + j - 4 of block 2 x + 1
+        pf[r][kb >> 1][(kb & 1) * 2] = pack2<T>(fast_exp2(st[r][kb][0]), fast_exp2(st[r][kb][1]));
+        pf[r][kb >> 1][(kb & 1) * 2 + 1] = pack2<T>(fast_exp2(st[r][kb][2]), fast_exp2(st[r][kb][3]));
+      }
+#pragma unroll
+    for (int x = 0; x < BN / 32; ++x) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint16_t* a = sv + (x * 32 + 4 * g + (col >> 2)) * P + db * 16 + 4 * (col & 3);
+        const u32x2 lo = lds_read_tr16(a);
+        const u32x2 hi = lds_read_tr16(a + 16 * P);
+        const u32x4 vf = u32x4{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int r = 0; r < RB; ++r) oacc[r][db] = mfma16x16x32<T>(vf, pf[r][x], oacc[r][db]);
+      }
+#pragma unroll
+      for (int r = 0; r < RB; ++r) oacc[r][DB] = mfma16x16x32<T>(ones, pf[r][x], oacc[r][DB]);
+    }
+  };
+
+  if (t0 < t1) {
+    Ids ids;
+    Stage s;
+    ids_of(t0, ids);
+    gload(t0, ids, s);
+    ids_of(t0 + 1, ids);
+    lstore(s, 0);
+    gload(t0 + 1, ids, s);
+    ids_of(t0 + 2, ids);
+    lds_barrier();
+    for (int t = t0; t < t1; ++t) {
+      const int b = (t - t0) & 1;
+      compute(b, t);
+      if (t + 1 < t1) {
+        lstore(s, b ^ 1);
+        gload(t + 2, ids, s);
+        ids_of(t + 3, ids);
+      }
+      lds_barrier();
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    if (qrow[r] >= rows) continue;
+    const float l = oacc[r][DB][0];
+    const float inv = 1.0f / l;
+    if (p.splits == 1) {
+      const size_t at = (size_t)qpos[r] * p.out_stride + (size_t)(kh * G + qrow[r] - qpos[r] * G) * D + 4 * g;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const f32x4 x = oacc[r][db] * inv;
+        if (p.out_dtype == kF32)
+          *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at + db * 16) = x;
+        else
+          *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at + db * 16) =
+              u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+      }
+    } else {
+      const size_t slot = ((size_t)split * p.num_kv_heads + kh) * rows + qrow[r];
+      if (g == 0) {
+        p.part_ml[2 * slot] = m[r];
+        p.part_ml[2 * slot + 1] = l;      // zero: no keys of this row, and no output row
+      }
+      if (l != 0.0f) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          *reinterpret_cast<f32x4*>(p.part_o + slot * D + db * 16 + 4 * g) = oacc[r][db] * inv;
+      }
+    }
+  }
+}
+
+// Joins the key splits of a row: out = sum w_s o_s / sum w_s, w_s = l_s 2^(m_s - max m).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prefill_fp8_merge_kernel(const PrefillFp8Params p) {
+  constexpr int TPR = D / 4;              // threads of a row
+  const int rows = p.q_len * p.group;
+  const long long item = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (item >= (long long)rows * p.num_kv_heads) return;
+  const int kh = (int)(item / rows), row = (int)(item - (long long)kh * rows);
+  const int d = (threadIdx.x % TPR) * 4;
+  const size_t step = (size_t)p.num_kv_heads * rows;
+  const size_t slot0 = (size_t)kh * rows + row;
+  float M = kNegInf;
+  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[2 * (slot0 + s * step)]);
+  f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
+  float den = 0.0f;
+  for (int s = 0; s < p.splits; ++s) {
+    const size_t slot = slot0 + s * step;
+    const float l = p.part_ml[2 * slot + 1];
+    if (l == 0.0f) continue;
+    const float w = l * fast_exp2(p.part_ml[2 * slot] - M);
+    den += w;
+    num += *reinterpret_cast<const f32x4*>(p.part_o + slot * D + d) * w;
+  }
+  const f32x4 x = num * (1.0f / den);
+  const int pos = row / p.group;
+  const size_t at = (size_t)pos * p.out_stride + (size_t)(kh * p.group + row - pos * p.group) * D + d;
+  if (p.out_dtype == kF32)
+    *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at) = x;
+  else
+    *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+}
+
+int block_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
+int tile_keys(int head_dim) { return head_dim == 256 ? 32 : 64; }
+
+template <typename T, int D, int RB, int BN>
+void launch_of(const PrefillFp8Params& p, hipStream_t stream) {
+  const long long rows = (long long)p.q_len * p.group;
+  const dim3 grid(p.num_kv_heads, (unsigned)((rows + 64 * RB - 1) / (64 * RB)), p.splits);
+  hipLaunchKernelGGL((prefill_fp8_kernel<T, D, RB, BN>), grid, dim3(kThreads), 0, stream, p);
+  if (p.splits > 1) {
+    const long long items = rows * p.num_kv_heads, per = 256 / (D / 4);
+    hipLaunchKernelGGL((prefill_fp8_merge_kernel<T, D>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, stream, p);
+  }
+}
+
+template <typename T> void launch_dims(const PrefillFp8Params& p, int head_dim, hipStream_t stream) {
+  if (head_dim == 64) launch_of<T, 64, 2, 64>(p, stream);
+  else if (head_dim == 128) launch_of<T, 128, 2, 64>(p, stream);
+  else launch_of<T, 256, 1, 32>(p, stream);
+}
+
+}  // namespace
+
+// Key splits: as many as fill two work-groups per CU, each of at least four key tiles.
+int prefill_fp8_splits(int q_len, int start_pos, int num_heads, int num_kv_heads, int head_dim, int cus) {
+  const long long rows = (long long)q_len * (num_heads / num_kv_heads);
+  const long long wgs = (rows + block_rows(head_dim) - 1) / block_rows(head_dim) * num_kv_heads;
+  const int tiles = (int)(((long long)start_pos + q_len + tile_keys(head_dim) - 1) / tile_keys(head_dim));
+  const long long want = 2LL * cus / std::max(1LL, wgs);
+  return (int)std::max(1LL, std::min({want, (long long)tiles / 4, 64LL}));
+}
+
+void launch_prefill_fp8(const PrefillFp8Params& p, int head_dim, int dtype, hipStream_t stream) {
+  if (dtype == kF16) launch_dims<_Float16>(p, head_dim, stream);
+  else launch_dims<__bf16>(p, head_dim, stream);
+}
+
+}  // namespace tv

@@ -256,4 +256,69 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
   return check_launch(who);
 }
 
+size_t tv_flash_prefill_paged_fp8_workspace_bytes(int q_len, int start_pos, int num_heads, int num_kv_heads,
+                                                  int head_dim) {
+  if (q_len <= 0 || start_pos < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      !valid_head_dim(head_dim))
+    return 0;
+  const int splits = tv::prefill_fp8_splits(q_len, start_pos, num_heads, num_kv_heads, head_dim, device_cus());
+  return splits > 1 ? (size_t)splits * q_len * num_heads * (head_dim + 2) * sizeof(float) : 0;
+}
+
+int tv_flash_prefill_paged_fp8(void* out, const void* q, const void* k_cache, const void* v_cache,
+                               const float* k_scale, const float* v_scale, const int32_t* block_table,
+                               int num_blocks, int block_size, int q_len, int start_pos, int num_heads,
+                               int num_kv_heads, int head_dim, int64_t q_stride, int64_t out_stride, int causal,
+                               float scale, int dtype, int out_dtype, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  const char* who = "tv_flash_prefill_paged_fp8";
+  if (!out || !q || !block_table) return fail(TV_EINVAL, "%s: null pointer argument", who);
+  int rc = check_cache(who, k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim, block_size, num_blocks, dtype);
+  if (rc != TV_OK) return rc;
+  if (!(out_dtype == dtype || out_dtype == TV_F32))
+    return fail(TV_EINVAL, "%s: bad dtype %d / out_dtype %d", who, dtype, out_dtype);
+  if (dtype == TV_F32) return fail(TV_EUNSUPPORTED, "%s: fp16 / bf16 queries only", who);
+  if (q_len <= 0 || start_pos < 0 || (long long)start_pos + q_len > (1LL << 30))
+    return fail(TV_EINVAL, "%s: bad sizes (q_len=%d, start_pos=%d)", who, q_len, start_pos);
+  if (num_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(TV_EINVAL, "%s: bad head counts (%d, %d)", who, num_heads, num_kv_heads);
+  if (q_stride < (int64_t)num_heads * head_dim || out_stride < (int64_t)num_heads * head_dim)
+    return fail(TV_EINVAL, "%s: token stride smaller than a token row", who);
+  if (!aligned(q, 16) || q_stride % 8 || !aligned(out, 16) || out_stride % 4 || !aligned(block_table, 4))
+    return fail(TV_EINVAL, "%s: query and output rows must be 16-byte aligned", who);
+  const int group = num_heads / num_kv_heads;
+  if ((long long)q_len * group > 65535LL * 64) return fail(TV_EINVAL, "%s: grid too large", who);
+  const size_t need = tv_flash_prefill_paged_fp8_workspace_bytes(q_len, start_pos, num_heads, num_kv_heads, head_dim);
+  if (workspace && (workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(TV_EINVAL, "%s: workspace of %zu bytes, 16-byte aligned, required (got %zu)", who, need, workspace_bytes);
+  tv::PrefillFp8Params p{};
+  p.out = out;
+  p.q = q;
+  p.k_cache = static_cast<const uint8_t*>(k_cache);
+  p.v_cache = static_cast<const uint8_t*>(v_cache);
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.block_table = block_table;
+  p.q_len = q_len;
+  p.start_pos = start_pos;
+  p.num_kv_heads = num_kv_heads;
+  p.group = group;
+  p.block_size = block_size;
+  p.bs_log2 = log2_or_minus1(block_size);
+  p.num_blocks = num_blocks;
+  p.q_stride = q_stride;
+  p.out_stride = out_stride;
+  p.causal = causal ? 1 : 0;
+  p.scale = scale;
+  p.out_dtype = out_dtype;
+  p.splits = 1;
+  if (workspace && need) {
+    p.splits = tv::prefill_fp8_splits(q_len, start_pos, num_heads, num_kv_heads, head_dim, device_cus());
+    p.part_o = reinterpret_cast<float*>(workspace);
+    p.part_ml = p.part_o + (size_t)p.splits * q_len * num_heads * head_dim;
+  }
+  tv::launch_prefill_fp8(p, head_dim, dtype, reinterpret_cast<hipStream_t>(stream));
+  return check_launch(who);
+}
+
 }  // extern "C"

@@ -129,6 +129,35 @@ struct DecodeFp8Params {
 int decode_fp8_slots(int head_dim, int dtype);   // work-groups resident at once on the current device
 void launch_paged_decode_fp8(const DecodeFp8Params& p, int head_dim, int dtype, bool wide, hipStream_t stream);
 
+// Attention of a chunk's rows over the 8-bit cache (flash_prefill_fp8.hip).
+struct PrefillFp8Params {
+  void* out;
+  const void* q;             // [q_len, Hq, D], token stride q_stride
+  const uint8_t* k_cache;    // [NB, Hkv, bs, D]
+  const uint8_t* v_cache;
+  const float* k_scale;      // [NB, Hkv]
+  const float* v_scale;
+  const int* block_table;
+  int q_len;
+  int start_pos;
+  int num_kv_heads;
+  int group;                 // query heads of a KV head
+  int block_size;
+  int bs_log2;               // log2(block_size) or -1
+  int num_blocks;
+  long long q_stride;        // elements between consecutive tokens
+  long long out_stride;
+  int causal;
+  float scale;
+  int out_dtype;
+  int splits;                // work-groups that share a row tile's keys
+  float* part_o;             // [splits, Hkv, q_len * group, D] normalised parts
+  float* part_ml;            // [splits, Hkv, q_len * group, 2] (max in log2 units, sum)
+};
+
+int prefill_fp8_splits(int q_len, int start_pos, int num_heads, int num_kv_heads, int head_dim, int cus);
+void launch_prefill_fp8(const PrefillFp8Params& p, int head_dim, int dtype, hipStream_t stream);
+
 void launch_kv_write_fp8(KVWriteFp8Params p, int dtype, hipStream_t stream);
 void launch_kv_gather_fp8(const KVGatherFp8Params& p, int dtype, hipStream_t stream);
 
