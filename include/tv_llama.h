@@ -110,6 +110,27 @@ int tv_qkv_rope_cache(void* q, void* k_out, void* v_out, void* k_cache, void* v_
 int tv_argmax_advance(int32_t* tokens, int32_t* positions, int32_t* context_lens, int32_t* history,
                       int history_len, const uint64_t* keys, int nparts, int M, void* stream);
 
+/*
+ * Log-probabilities of given tokens under rows of logits, with the rows' entropy
+ * and their top_k most likely tokens.  No counterpart in the reference, whose
+ * sampling returns tokens only (sampling.py:131-134).
+ *   logprobs[m] = log softmax(logits[m])[tokens[m]]
+ *   entropy[m]  = -sum_i softmax_i log softmax_i  (natural logarithms)
+ *   top_ids / top_logprobs [M, top_k]: most likely first, equal logits by lowest id
+ * logits [M, vocab] of dtype (TV_F32 / TV_F16 / TV_BF16) at row_stride elements;
+ * all sums fp32, the probability of the most likely token taken out of them, so
+ * values near 0 keep their digits.  A logit of -inf has probability 0.  A token
+ * outside [0, vocab) gives a NaN log-probability.  A row with a NaN, with +inf, or
+ * with no finite logit gives NaN everywhere but in top_ids, where NaN ranks above
+ * every number.  0 <= top_k <= min(64, vocab); with 0 top_ids and top_logprobs may
+ * be NULL.  workspace: of tv_token_logprobs_workspace_bytes bytes (0 where a row
+ * fits one work-group), 8-byte aligned, one per launch that may overlap.
+ */
+size_t tv_token_logprobs_workspace_bytes(int M, int vocab, int top_k, int dtype);
+int tv_token_logprobs(float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, const void* logits,
+                      const int32_t* tokens, int M, int vocab, int64_t row_stride, int top_k, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- model-level step ------------------------------------------------------ */
 
 /* Weights in device memory; per-layer fields are host arrays of n_layers device pointers. */

@@ -1,0 +1,219 @@
+"""Token log-probabilities, entropy and top alternatives of rows of logits."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from tests.random_cases import case_count, case_seed
+
+DTYPES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
+gpu = pytest.mark.gpu
+
+
+def reference(x, tokens, k):
+    """float64, with the maximum's own term left out of the sums so that values near 0 keep their digits."""
+    x = x.astype(np.float64)
+    n = x.shape[1]
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        rows = np.arange(len(x))
+        order = np.lexsort((np.broadcast_to(np.arange(n), x.shape), np.where(np.isnan(x), -np.inf, -(x + 0.0)),
+                            ~np.isnan(x)), axis=1)[:, :k]
+        top = np.where(np.isnan(x), -np.inf, x).argmax(1)
+        d = x[rows, top][:, None] - x
+        e = np.exp(-d)
+        e[rows, top] = 0.0
+        e[np.isnan(x).any(1) | ~np.isfinite(x[rows, top])] = np.nan
+        s = e.sum(1)
+        t = np.where(e > 0, d * e, 0.0 * e).sum(1)
+        given = np.where((tokens >= 0) & (tokens < n), -d[rows, np.clip(tokens, 0, n - 1)], np.nan)
+        total = np.log1p(s)
+        return given - total, total + t / (1 + s), order, -np.take_along_axis(d, order, 1) - total[:, None], s, t
+
+
+def check(out, x, tokens, k):
+    """The sums are fp32 with positive terms: relative error of an exponential 2^-22 plus 2^-23 of its
+    argument, at most 2^-23 a partial sum over V / 64 additions (the terms of a thread, its wave and the
+    work-group's); m - x and the last subtraction round once each.  An exponential below fp32's least
+    normal number, 2^-126, is zero (v_exp_f32 gives no subnormal ones), which leaves out at most V 2^-126
+    of s and 100 times that of t (beyond a distance of 100 a term is below 2^-137 with its factor)."""
+    lp, entropy, ids, top = (a.cpu().numpy() for a in out)
+    want_lp, want_h, want_ids, want_top, s, t = reference(x, tokens, k)
+    n = x.shape[1]
+    assert np.array_equal(ids, want_ids)
+    finite = np.where(np.isfinite(x), x, 0.0)
+    span = finite.max(1) - finite.min(1)
+    # far terms weigh nothing: an argument above 100 belongs to a term below 2^-144
+    rel = 2.0 ** -22 + np.minimum(span, 100) * 2.0 ** -22 + (64 + n / 64) * 2.0 ** -24
+    off_total = rel * s / (1 + s) + 2.0 ** -22 * np.log1p(s)            # of log(1 + s)
+    off_h = off_total + 3 * rel * t / (1 + s) + 2.0 ** -22 * want_h
+    for got, want, off in ((lp, want_lp, off_total), (entropy, want_h, off_h), (top, want_top, off_total[:, None])):
+        assert got.dtype == np.float32
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        ok = np.isfinite(want)
+        assert np.array_equal(got[~ok & ~np.isnan(want)], want[~ok & ~np.isnan(want)])
+        with np.errstate(invalid="ignore"):
+            diff = np.abs(got - want)
+            tol = off + 2.0 ** -23 * np.abs(want) + 101 * n * 2.0 ** -126
+        assert np.all(diff[ok] <= np.broadcast_to(tol, want.shape)[ok]), float((diff / tol)[ok].max())
+
+
+def run(x, tokens, k, dtype):
+    from tinyvllm_amd.sampling import token_logprobs
+    logits = torch.from_numpy(x).to("cuda", DTYPES[dtype])
+    out = token_logprobs(logits, torch.from_numpy(tokens.astype(np.int32)).cuda(), k)
+    return out, logits.double().cpu().numpy()
+
+
+def test_entry_point_validates_on_the_host():
+    from tinyvllm_amd import _lib
+    lib, p = _lib.load(), ctypes.c_void_p(256)
+    base = [p, p, p, p, p, p, 4, 1000, 1000, 5, 0, None, 0, None]
+
+    def call(**kw):
+        a = list(base)
+        for i, v in kw.items():
+            a[int(i[1:])] = v
+        return lib.tv_token_logprobs(*a)
+
+    assert call(_0=None) == _lib.TV_EINVAL and b"null pointer" in lib.tv_last_error()
+    assert call(_2=None) == _lib.TV_EINVAL and b"null pointer" in lib.tv_last_error()
+    assert call(_6=0) == _lib.TV_OK
+    assert call(_6=-1) == _lib.TV_EINVAL
+    assert call(_8=999) == _lib.TV_EINVAL and b"bad shape" in lib.tv_last_error()
+    assert call(_9=65) == _lib.TV_EINVAL and b"top_k" in lib.tv_last_error()
+    assert call(_7=4, _8=4) == _lib.TV_EINVAL and b"top_k" in lib.tv_last_error()
+    assert call(_10=3) == _lib.TV_EUNSUPPORTED
+    assert call(_4=ctypes.c_void_p(258)) == _lib.TV_EINVAL and b"misaligned" in lib.tv_last_error()
+    assert call(_7=200000, _8=200000) == _lib.TV_EINVAL and b"workspace" in lib.tv_last_error()
+    assert lib.tv_token_logprobs_workspace_bytes(7, 32000, 5, 0) == 0
+    assert lib.tv_token_logprobs_workspace_bytes(7, 128256, 5, 0) == 7 * 4 * 52
+    assert lib.tv_token_logprobs_workspace_bytes(7, 128256, 5, 2) == 7 * 2 * 52
+
+
+def test_python_refusals():
+    from tinyvllm_amd.sampling import token_logprobs
+    with pytest.raises(ValueError, match="HIP device"):
+        token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32))
+
+
+@gpu
+def test_python_refusals_on_the_gpu():
+    from tinyvllm_amd.sampling import token_logprobs
+    x = torch.zeros((2, 8), device="cuda")
+    t = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for args, what in (((x, t[:1]), "tokens must be"), ((x, t.long()), "int32"), ((x, t, 9), "top_k"), ((x, t, -1), "top_k"),
+                       ((x.double(), t), "dtype"), ((x.t().contiguous().t(), t), "contiguous"),
+                       ((x.expand(3, 2, 8).transpose(0, 1), t[:1].expand(2, 3)), "evenly")):
+        with pytest.raises(ValueError, match=what):
+            token_logprobs(*args)
+    out = token_logprobs(x[:0], t[:0], 3)
+    assert out.top_ids.shape == (0, 3)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("rows,vocab,k", [(1, 1, 1), (3, 2, 0), (5, 63, 63), (2, 1000, 64), (4, 8192, 5), (3, 8193, 20),
+                                          (2, 16385, 1), (5, 32000, 20), (2, 32769, 64), (3, 70001, 7), (2, 128256, 20)])
+def test_sizes(dtype, rows, vocab, k):
+    rng = np.random.Generator(np.random.PCG64(61))
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    x[:, rng.integers(0, vocab, 3)] += 9
+    tokens = rng.integers(0, vocab, rows)
+    out, seen = run(x, tokens, k, dtype)
+    check(out, seen, tokens, k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("vocab", [300, 32000, 70000])
+def test_ties_masks_and_non_finite_rows(dtype, vocab):
+    """Equal logits, signed zeros, -inf masks, the type's lowest value, rows of one kind only, NaN, +inf."""
+    rng = np.random.Generator(np.random.PCG64(62))
+    x = np.zeros((14, vocab), np.float32)
+    x[1] = -np.inf
+    x[2] = -np.inf
+    x[2, vocab - 1] = 3.0
+    x[3] = rng.integers(0, 3, vocab)
+    x[4] = torch.finfo(DTYPES[dtype]).min
+    x[4, vocab // 2] = 1.0
+    x[5] = rng.standard_normal(vocab)
+    x[5, 7] = np.nan
+    x[6] = rng.standard_normal(vocab)
+    x[6, [0, vocab - 1]] = np.inf
+    x[7] = np.nan
+    x[8, ::2] = -0.0
+    x[9] = rng.standard_normal(vocab)
+    x[9, : vocab - 3] = -np.inf
+    x[10] = -30.0
+    x[10, 11] = 40.0                                   # probability of all but one: e^-70 each
+    x[11] = -np.arange(vocab) / 64
+    x[12] = np.arange(vocab) / 64
+    x[13] = -1e4
+    x[13, 0] = np.nan
+    tokens = np.array([0, 1, vocab - 1, 2, vocab // 2, 3, 4, 5, 6, 0, 11, 0, -1, vocab])
+    for k in (0, 5, 64):
+        out, seen = run(x, tokens, k, dtype)
+        check(out, seen, tokens, k)
+
+
+@gpu
+def test_certain_tokens_keep_their_digits():
+    """log p of a token with nearly all of the probability, and the entropy of its row, are small numbers."""
+    x = np.full((6, 5000), -40.0, np.float32)
+    x[np.arange(6), [0, 9, 77, 256, 4097, 4999]] = [0.0, -10.0, 3.0, 20.0, -25.0, 60.0]
+    tokens = np.array([0, 9, 77, 256, 4097, 4999])
+    out, seen = run(x, tokens, 2, "float32")
+    check(out, seen, tokens, 2)
+    assert out.logprobs[0] < 0 and out.entropy[0] > 0
+
+
+@gpu
+def test_strided_rows_shapes_and_unaligned_vocabularies():
+    from tinyvllm_amd.sampling import token_logprobs
+    rng = np.random.Generator(np.random.PCG64(63))
+    wide = torch.from_numpy((rng.standard_normal((1, 9, 1010)) * 2).astype(np.float32)).cuda()
+    tokens = torch.from_numpy(rng.integers(0, 1003, (1, 8)).astype(np.int32)).cuda()
+    view = wide[:, :-1, 3:1006]                        # rows at 12-byte offsets, stride 1010
+    out = token_logprobs(view, tokens, 4)
+    assert out.logprobs.shape == (1, 8) and out.top_ids.shape == (1, 8, 4)
+    check([o[0] for o in out], view[0].double().cpu().numpy(), tokens[0].cpu().numpy(), 4)
+    one = token_logprobs(view[0, 0], tokens[0, 0], 4)
+    assert torch.equal(one.top_ids, out.top_ids[0, 0]) and torch.equal(one.logprobs, out.logprobs[0, 0])
+
+
+@gpu
+def test_in_a_graph_beside_eager_calls():
+    """Two captured calls with segments (each its own workspace), replayed between eager ones."""
+    from tinyvllm_amd.sampling import token_logprobs
+    rng = np.random.Generator(np.random.PCG64(64))
+    a, b = (torch.from_numpy((rng.standard_normal((3, 70000)) * 2).astype(np.float32)).cuda() for _ in range(2))
+    tokens = torch.tensor([1, 2, 69999], dtype=torch.int32, device="cuda")
+    token_logprobs(a, tokens, 6)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [token_logprobs(x, tokens, 6) for x in (a, b)]
+    for _ in range(3):
+        a.copy_(torch.from_numpy((rng.standard_normal((3, 70000)) * 2).astype(np.float32)))
+        g.replay()
+        eager = [token_logprobs(x, tokens, 6) for x in (a, b)]
+        torch.cuda.synchronize()
+        for x, y, z in zip(outs, eager, (a, b)):
+            assert all(torch.equal(i, j) for i, j in zip(x, y))
+            check(x, z.double().cpu().numpy(), tokens.cpu().numpy(), 6)
+
+
+@gpu
+def test_random_rows():
+    rng = np.random.Generator(np.random.PCG64(case_seed(65)))
+    for i in range(case_count(12)):
+        dtype = sorted(DTYPES)[rng.integers(3)]
+        rows, vocab = int(rng.integers(1, 9)), int(np.exp(rng.uniform(0, np.log(140000))))
+        k = int(rng.integers(0, min(64, vocab) + 1))
+        print("logprobs", i, dtype, rows, vocab, k, flush=True)
+        x = (rng.standard_normal((rows, vocab)) * rng.choice([0.01, 1, 8])).astype(np.float32)
+        tokens = rng.integers(-1, vocab + 1, rows)
+        out, seen = run(x, tokens, k, dtype)
+        check(out, seen, tokens, k)

@@ -55,6 +55,8 @@ SIGNATURES = {
     "tv_qkv_rope_cache": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I,
                                _I, _P, _P, _P]),
     "tv_argmax_advance": (_I, [_P, _P, _P, _P, _I, _P, _I, _I, _P]),
+    "tv_token_logprobs_workspace_bytes": (_S, [_I, _I, _I, _I]),
+    "tv_token_logprobs": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _P, _S, _P]),
     "tv_llama_decode_workspace_bytes": (_S, [_P, _I, _I, _I, _I]),
     "tv_llama_decode_step": (_I, [_P, _P, _P, _P]),
     "tv_llama_graph_create": (_I, [_P, _P, _P, _P, _P]),

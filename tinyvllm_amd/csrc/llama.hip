@@ -20,6 +20,7 @@
 #include "../../include/tv_llama.h"
 #include "tv_dense.h"
 #include "tv_error.h"
+#include "tv_logprobs.h"
 #include "tv_paged_keys.h"
 #include "tv_params.h"
 
@@ -514,6 +515,51 @@ int tv_argmax_advance(int32_t* tokens, int32_t* positions, int32_t* context_lens
   p.history_len = history_len;
   tv::launch_advance(p, reinterpret_cast<hipStream_t>(stream));
   return check_launch("tv_argmax_advance");
+}
+
+size_t tv_token_logprobs_workspace_bytes(int M, int vocab, int top_k, int dtype) {
+  if (M <= 0 || vocab <= 0 || top_k < 0 || top_k > tv::kLogprobTopMax || !step_dtype(dtype)) return 0;
+  const int segs = tv::logprob_segments(vocab, (int)elem_bytes(dtype));
+  return segs > 1 ? (size_t)M * segs * ((size_t)top_k * 8 + 12) : 0;
+}
+
+int tv_token_logprobs(float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, const void* logits,
+                      const int32_t* tokens, int M, int vocab, int64_t row_stride, int top_k, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "tv_token_logprobs";
+  if (M < 0 || vocab <= 0 || row_stride < vocab)
+    return fail(TV_EINVAL, "%s: bad shape (M=%d, vocab=%d, row_stride=%lld)", who, M, vocab, (long long)row_stride);
+  if (!step_dtype(dtype)) return fail(TV_EUNSUPPORTED, "%s: dtype %d (float32 / float16 / bfloat16)", who, dtype);
+  if (top_k < 0 || top_k > tv::kLogprobTopMax || top_k > vocab)
+    return fail(TV_EINVAL, "%s: top_k %d outside 0..min(%d, vocab)", who, top_k, tv::kLogprobTopMax);
+  if (M == 0) return ok();
+  if (!logprobs || !entropy || !logits || !tokens || (top_k > 0 && (!top_ids || !top_logprobs)))
+    return fail(TV_EINVAL, "%s: null pointer argument", who);
+  const int es = (int)elem_bytes(dtype);
+  if ((uintptr_t)logits % es || (uintptr_t)tokens % 4 || (uintptr_t)logprobs % 4 || (uintptr_t)entropy % 4 ||
+      (top_k > 0 && ((uintptr_t)top_ids % 4 || (uintptr_t)top_logprobs % 4)))
+    return fail(TV_EINVAL, "%s: misaligned buffer", who);
+  const size_t need = tv_token_logprobs_workspace_bytes(M, vocab, top_k, dtype);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
+    return fail(TV_EINVAL, "%s: workspace of %zu bytes, 8-byte aligned, required (got %zu)", who, need, workspace_bytes);
+  const int segs = tv::logprob_segments(vocab, es);
+  if (segs > 65535) return fail(TV_EINVAL, "%s: grid too large", who);
+  tv::LogprobParams p{};
+  p.logits = logits;
+  p.tokens = tokens;
+  p.row_stride = row_stride;
+  p.rows = M;
+  p.vocab = vocab;
+  p.top_k = top_k;
+  p.aligned = aligned16(logits) && (M == 1 || row_stride * es % 16 == 0);
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  p.part_keys = reinterpret_cast<unsigned long long*>(workspace);
+  p.part = reinterpret_cast<float*>(p.part_keys + (size_t)M * segs * top_k);
+  tv::launch_logprobs(p, dtype, reinterpret_cast<hipStream_t>(stream));
+  return check_launch(who);
 }
 
 size_t tv_llama_decode_workspace_bytes(const tv_llama_model* model, int batch, int max_blocks, int block_size,
