@@ -151,11 +151,18 @@ typedef struct tv_llama_model {
   int rope_len;
 } tv_llama_model;
 
-/* Paged K/V caches: host arrays of n_layers device pointers [num_blocks, block_size, Hkv, D]. */
+/*
+ * Paged K/V caches: host arrays of n_layers device pointers [num_blocks, block_size, Hkv, D] of the model
+ * dtype (k_scales and v_scales NULL), or 8-bit caches (tv_attn.h): e4m3 numbers [num_blocks, Hkv,
+ * block_size, D] with scales [num_blocks, Hkv].  Over an 8-bit cache head_dim is 64, 128 or 256, a decode
+ * step's partition_size a multiple of 32, and a sequence of context 0 attends to nothing.
+ */
 typedef struct tv_llama_cache {
   void* const* k_caches;
   void* const* v_caches;
   int num_blocks, block_size;
+  float* const* k_scales;
+  float* const* v_scales;
 } tv_llama_cache;
 
 typedef struct tv_llama_decode_args {
@@ -214,7 +221,11 @@ typedef struct tv_llama_prefill_args {
   int attend_prefix;
 } tv_llama_prefill_args;
 
-/* Workspace of tv_llama_prefill for up to num_tokens tokens.  Host-only. */
+/*
+ * Workspace of tv_llama_prefill for up to num_tokens tokens.  Host-only.  With an 8-bit cache and
+ * attend_prefix, tv_flash_prefill_paged_fp8_workspace_bytes of the chunk on top lets a few rows over a
+ * long prefix be split; without it they run unsplit.
+ */
 size_t tv_llama_prefill_workspace_bytes(const tv_llama_model* model, int num_tokens);
 
 /*

@@ -126,7 +126,7 @@ StepLayout step_layout(const tv_llama_model* m, int B, int max_blocks, int block
   L.keys = c.take((size_t)((m->vocab_size + tv::kLinBN - 1) / tv::kLinBN) * B * 8);
   L.kst = c.take((size_t)B * kd * es);
   L.vst = c.take((size_t)B * kd * es);
-  L.slots = c.take((size_t)B * 4);
+  L.slots = c.take((size_t)B * 8);   // slots or context lengths, then the slots of an 8-bit cache's write
   // prefill: room for a prefix-attending chunk's unsplit paged-decode launch
   // (its only workspace is the schedule of B + 1 ints)
   L.attn_ws_bytes = decode ? tv_paged_decode_workspace_bytes(B, m->n_heads, m->head_dim, max_blocks, block_size,
@@ -193,6 +193,8 @@ struct LayerIO {
   int* slots;
   void* attn_ws;
   size_t attn_ws_bytes;
+  void* extra_ws;            // what the caller's workspace holds beyond the layout (prefill, 8-bit cache)
+  size_t extra_ws_bytes;
   int ks_qkv, ks_o, ks_2;
 };
 
@@ -354,17 +356,105 @@ int attend_unfused(const tv_llama_model* m, const tv_llama_cache* c, const Layer
   return TV_OK;
 }
 
+// A layer over an 8-bit cache: qkv_rope into staging, the quantising write, and
+// attention over the cache (decode and chunks with a prefix) or over the staged
+// rows themselves (a chunk that attends to itself only).
+int attend_fp8(const tv_llama_model* m, const tv_llama_cache* c, const LayerIO& io, int l, hipStream_t s) {
+  const int dt = m->dtype;
+  const int qd = m->n_heads * m->head_dim;
+  const int kd = m->n_kv_heads * m->head_dim;
+  const float scale = 1.0f / std::sqrt((float)m->head_dim);
+  const int M = io.M;
+  int* write_slots = io.slots + M;
+  tv::QKVParams qp{};
+  qp.q = io.q;
+  qp.k_out = io.kst;
+  qp.v_out = io.vst;
+  qp.slots = write_slots;
+  qp.part = io.part;
+  qp.splits = splits_of(m->dim, io.ks_qkv);
+  qp.rope = m->rope;
+  qp.rope_len = m->rope_len;
+  qp.block_size = c->block_size;
+  qp.num_blocks = c->num_blocks;
+  qp.M = M;
+  qp.Hq = m->n_heads;
+  qp.Hkv = m->n_kv_heads;
+  qp.D = m->head_dim;
+  if (io.decode) {
+    qp.positions = io.dargs->positions;
+    qp.block_tables = io.dargs->block_tables;
+    qp.bt_row_step = io.dargs->bt_stride;
+    qp.bt_width = io.dargs->bt_stride;
+  } else {
+    qp.pos_base = io.pargs->start_pos;
+    qp.block_tables = io.pargs->block_table;
+    qp.bt_width = io.pargs->bt_width;
+  }
+  tv::launch_qkv_rope(qp, dt, s);
+  int rc = check_launch("qkv_rope");
+  if (rc != TV_OK) return rc;
+  auto write = [&]() {
+    return tv_reshape_and_cache_fp8(c->k_caches[l], c->v_caches[l], c->k_scales[l], c->v_scales[l], io.kst, io.vst,
+                                    write_slots, M, m->n_kv_heads, m->head_dim, c->block_size, c->num_blocks, kd, kd,
+                                    dt, nullptr, s);
+  };
+  if (!io.decode || io.dargs->write_before_attend) {
+    rc = write();
+    if (rc != TV_OK) return rc;
+  }
+  if (io.decode) {
+    const tv_llama_decode_args* a = io.dargs;
+    rc = tv_paged_decode_fp8(io.attn, io.q, c->k_caches[l], c->v_caches[l], c->k_scales[l], c->v_scales[l],
+                             a->block_tables, a->context_lens, a->batch, m->n_heads, m->n_kv_heads, m->head_dim,
+                             c->block_size, c->num_blocks, a->bt_stride, a->max_blocks, scale, dt, dt,
+                             a->partition_size, io.attn_ws, io.attn_ws_bytes, s);
+    if (rc == TV_OK && !a->write_before_attend) rc = write();
+    return rc;
+  }
+  const tv_llama_prefill_args* a = io.pargs;
+  if (!a->attend_prefix || a->start_pos == 0)
+    return tv_flash_prefill(io.attn, io.q, io.kst, io.vst, M, M, m->n_heads, m->n_kv_heads, m->head_dim, m->head_dim,
+                            qd, kd, kd, qd, 1, scale, dt, dt, 0, nullptr, 0, s);
+  if (dt == TV_F32) {
+    // row i is a single-token attention of context start_pos + i + 1 over the sequence's one table row
+    const int width = a->bt_width * c->block_size;
+    return tv_paged_decode_fp8(io.attn, io.q, c->k_caches[l], c->v_caches[l], c->k_scales[l], c->v_scales[l],
+                               a->block_table, io.slots, M, m->n_heads, m->n_kv_heads, m->head_dim, c->block_size,
+                               c->num_blocks, 0, a->bt_width, scale, dt, dt, (width + 31) / 32 * 32, io.attn_ws,
+                               io.attn_ws_bytes, s);
+  }
+  const size_t need = tv_flash_prefill_paged_fp8_workspace_bytes(M, a->start_pos, m->n_heads, m->n_kv_heads, m->head_dim);
+  const bool room = need > 0 && io.extra_ws_bytes >= need;
+  return tv_flash_prefill_paged_fp8(io.attn, io.q, c->k_caches[l], c->v_caches[l], c->k_scales[l], c->v_scales[l],
+                                    a->block_table, c->num_blocks, c->block_size, M, a->start_pos, m->n_heads,
+                                    m->n_kv_heads, m->head_dim, qd, qd, 1, scale, dt, dt, room ? io.extra_ws : nullptr,
+                                    room ? io.extra_ws_bytes : 0, s);
+}
+
+// A cache's pointers; an 8-bit one has both scale arrays and slots that fit 32 bits.
+int validate_cache(const tv_llama_cache* c, const char* who) {
+  if (!c || !c->k_caches || !c->v_caches || c->num_blocks <= 0 || c->block_size <= 0)
+    return fail(TV_EINVAL, "%s: bad cache", who);
+  if (!c->k_scales != !c->v_scales) return fail(TV_EINVAL, "%s: give both scale arrays of an 8-bit cache or neither", who);
+  if (c->k_scales && (long long)c->num_blocks * c->block_size > 0x7fffffffLL)
+    return fail(TV_EUNSUPPORTED, "%s: an 8-bit cache of %d blocks of %d has slots past 32 bits", who, c->num_blocks,
+                c->block_size);
+  return TV_OK;
+}
+
 int run_layers(const tv_llama_model* m, const tv_llama_cache* c, const LayerIO& io, hipStream_t s) {
   const int dt = m->dtype;
   const int qd = m->n_heads * m->head_dim;
   const int nqkv = qkv_width(m);
   const int M = io.M;
   // the fused step attention runs on 16-bit MFMA; fp32 models take qkv_rope + tv_paged_decode
-  const bool fused_attn = io.decode && dt != TV_F32 &&
+  const bool fp8 = c->k_scales != nullptr;
+  const bool fused_attn = !fp8 && io.decode && dt != TV_F32 &&
                           tv::step_attn_supported(m->head_dim, m->n_heads / m->n_kv_heads, c->block_size);
   for (int l = 0; l < m->n_layers; ++l) {
     linear(io.xh, m->wqkv[l], M, nqkv, m->dim, m->dim, io.ks_qkv, tv::kEpiPartial, io.part, 0, nullptr, dt, s);
-    int rc = fused_attn ? attend_fused(m, c, io, l, s) : attend_unfused(m, c, io, l, s);
+    int rc = fp8 ? attend_fp8(m, c, io, l, s) : fused_attn ? attend_fused(m, c, io, l, s) : attend_unfused(m, c, io, l, s);
     if (rc != TV_OK) return rc;
 
     linear(io.attn, m->wo[l], M, m->dim, qd, qd, io.ks_o, tv::kEpiPartial, io.part, 0, nullptr, dt, s);
@@ -573,8 +663,7 @@ int tv_llama_decode_step(const tv_llama_model* m, const tv_llama_cache* c, const
                          void* stream) {
   int rc = validate_model(m, "tv_llama_decode_step");
   if (rc != TV_OK) return rc;
-  if (!c || !c->k_caches || !c->v_caches || c->num_blocks <= 0 || c->block_size <= 0)
-    return fail(TV_EINVAL, "tv_llama_decode_step: bad cache");
+  if ((rc = validate_cache(c, "tv_llama_decode_step")) != TV_OK) return rc;
   if (!a || a->batch <= 0 || !a->tokens || !a->positions || !a->context_lens || !a->block_tables ||
       a->bt_stride <= 0 || a->max_blocks <= 0 || a->max_blocks > a->bt_stride || a->partition_size <= 0)
     return fail(TV_EINVAL, "tv_llama_decode_step: bad decode arguments");
@@ -674,8 +763,7 @@ size_t tv_llama_prefill_workspace_bytes(const tv_llama_model* model, int num_tok
 int tv_llama_prefill(const tv_llama_model* m, const tv_llama_cache* c, const tv_llama_prefill_args* a, void* stream) {
   int rc = validate_model(m, "tv_llama_prefill");
   if (rc != TV_OK) return rc;
-  if (!c || !c->k_caches || !c->v_caches || c->num_blocks <= 0 || c->block_size <= 0)
-    return fail(TV_EINVAL, "tv_llama_prefill: bad cache");
+  if ((rc = validate_cache(c, "tv_llama_prefill")) != TV_OK) return rc;
   if (!a || a->num_tokens <= 0 || !a->tokens || !a->block_table || a->bt_width <= 0 || a->start_pos < 0)
     return fail(TV_EINVAL, "tv_llama_prefill: bad prefill arguments");
   if (a->logits && !aligned16(a->logits)) return fail(TV_EINVAL, "tv_llama_prefill: logits must be 16-byte aligned");
@@ -706,6 +794,8 @@ int tv_llama_prefill(const tv_llama_model* m, const tv_llama_cache* c, const tv_
   io.slots = at<int>(ws, L.slots);
   io.attn_ws = at<void>(ws, L.attn_ws);
   io.attn_ws_bytes = L.attn_ws_bytes;
+  io.extra_ws = at<void>(ws, L.total);
+  io.extra_ws_bytes = a->workspace_bytes - L.total;
   io.ks_qkv = L.ks_qkv;
   io.ks_o = L.ks_o;
   io.ks_2 = L.ks_2;

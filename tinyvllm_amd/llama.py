@@ -19,6 +19,10 @@ only owns buffers and copies inputs into them.  The model dtype is float32
 three, and fp32 decode attention takes the separate RoPE and paged-decode
 kernels (the fused step attention is 16-bit only).
 
+``kv_cache`` is a ``KVCache`` of the model dtype or an ``FP8KVCache`` of it.  Over the
+latter a prompt's first chunk attends to its own K/V in the model dtype, everything
+else to what the cache holds.
+
 K/V order: the reference attends first and writes the step's K/V afterwards
 (llama.py:378-386), so with the engine's ``context_len = position + 1``
 (engine.py:251) the last attended slot has not been written yet.  The default
@@ -35,7 +39,7 @@ import torch
 
 from . import _lib
 from .attention import default_partition_size
-from .kv_cache import as_torch_dtype
+from .kv_cache import FP8KVCache, as_torch_dtype
 
 _lib.load()
 
@@ -166,7 +170,8 @@ class _Model(ctypes.Structure):
 
 
 class _Cache(ctypes.Structure):
-    _fields_ = [("k_caches", _PP), ("v_caches", _PP), ("num_blocks", _I), ("block_size", _I)]
+    _fields_ = [("k_caches", _PP), ("v_caches", _PP), ("num_blocks", _I), ("block_size", _I), ("k_scales", _PP),
+                ("v_scales", _PP)]
 
 
 class _DecodeArgs(ctypes.Structure):
@@ -312,9 +317,12 @@ class Llama:
         if kv_cache.num_layers != c.n_layers or kv_cache.n_kv_heads != c.n_kv_heads or \
                 kv_cache.head_dim != c.head_dim or kv_cache.dtype != c.dtype:
             raise ValueError("KV cache shape / dtype does not match the model")
-        keep = (_ptr_array(kv_cache.k_cache), _ptr_array(kv_cache.v_cache))
+        keep = [_ptr_array(kv_cache.k_cache), _ptr_array(kv_cache.v_cache)]
         s = _Cache(ctypes.cast(keep[0], _PP), ctypes.cast(keep[1], _PP), kv_cache.num_blocks, kv_cache.block_size)
-        return s, keep
+        if isinstance(kv_cache, FP8KVCache):
+            keep += [_ptr_array(kv_cache.k_scale), _ptr_array(kv_cache.v_scale)]
+            s.k_scales, s.v_scales = (ctypes.cast(x, _PP) for x in keep[2:])
+        return s, tuple(keep)
 
     # ---- prefill ---------------------------------------------------------------
     def prefill(self, tokens, kv_cache, block_manager, seq_id, start_pos=0, *, logits="all", attend_prefix=False):
@@ -348,6 +356,8 @@ class Llama:
             raise ValueError("block table does not cover the prompt")
         lib = _lib.load()
         need = lib.tv_llama_prefill_workspace_bytes(ctypes.byref(self._model), n)
+        if attend_prefix and start_pos > 0 and isinstance(kv_cache, FP8KVCache):
+            need += lib.tv_flash_prefill_paged_fp8_workspace_bytes(n, start_pos, c.n_heads, c.n_kv_heads, c.head_dim)
         if self._prefill_ws is None or self._prefill_ws.numel() < need:
             self._prefill_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         rows = 0 if logits is None else (1 if logits == "last" else n)
@@ -469,9 +479,13 @@ class DecodeGraph:
         self.logits = torch.zeros((batch, c.vocab_size), dtype=torch.float32, device=dev) if keep_logits else None
         self.history_len = history_len
         self.history = torch.zeros((batch, history_len), dtype=torch.int32, device=dev) if history_len else None
+        lib = _lib.load()
+        if partition_size is None and isinstance(kv_cache, FP8KVCache):
+            partition_size = lib.tv_paged_decode_fp8_partition_size(batch, c.n_heads, c.n_kv_heads, c.head_dim, max_blocks,
+                                                                    kv_cache.block_size, _lib.dtype_code(c.dtype))
+            _lib.check(0 if partition_size > 0 else _lib.TV_EINVAL, "DecodeGraph")
         self.partition_size = partition_size or default_partition_size(batch, c.n_heads, c.n_kv_heads, c.head_dim,
                                                                        max_blocks, kv_cache.block_size, c.dtype)
-        lib = _lib.load()
         need = lib.tv_llama_decode_workspace_bytes(ctypes.byref(model._model), batch, max_blocks,
                                                    kv_cache.block_size, self.partition_size)
         if need == 0:
