@@ -23,37 +23,49 @@ namespace tv {
 
 constexpr int kWriteThreads = 256;
 constexpr int kWriteHold = 4;
+constexpr int kWriteFewTokens = 512;
+constexpr long long kWriteGroups = 512;   // work-groups that a prompt's write is cut into
 
 struct Row8 {
   f32x4 a, b;
 };
 
-// Eight elements; `aligned` (uniform over the launch): their addresses are multiples of 16 bytes.
-template <typename T> __device__ __forceinline__ Row8 load_row8(const T* p, bool aligned) {
-  if (!aligned) {
-    Row8 r;
+// Eight elements as they lie in memory.  `aligned` (uniform over the launch):
+// their addresses are multiples of 16 bytes.
+template <typename T> struct Raw8 { u32x4 w[sizeof(T) == 4 ? 2 : 1]; };
+
+template <typename T> __device__ __forceinline__ Raw8<T> load_row8(const T* p, bool aligned) {
+  Raw8<T> r;
+  if (aligned) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      r.a[i] = to_float<T>(p[i]);
-      r.b[i] = to_float<T>(p[4 + i]);
-    }
-    return r;
-  }
-  if constexpr (sizeof(T) == 4) {
-    return Row8{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i >> 2][i & 3] = reinterpret_cast<const uint32_t*>(p)[i];
   } else {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-    Row8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.w[0][i] = reinterpret_cast<const uint16_t*>(p)[2 * i] | (uint32_t)reinterpret_cast<const uint16_t*>(p)[2 * i + 1] << 16;
+  }
+  return r;
+}
+
+template <typename T> __device__ __forceinline__ Row8 as_floats(const Raw8<T>& raw) {
+  Row8 r;
+  if constexpr (sizeof(T) == 4) {
+    r.a = __builtin_bit_cast(f32x4, raw.w[0]);
+    r.b = __builtin_bit_cast(f32x4, raw.w[1]);
+  } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float x, y;
-      unpack2<T>(w[i], x, y);
+      unpack2<T>(raw.w[0][i], x, y);
       r.a[2 * i] = x; r.a[2 * i + 1] = y;
-      unpack2<T>(w[2 + i], x, y);
+      unpack2<T>(raw.w[0][2 + i], x, y);
       r.b[2 * i] = x; r.b[2 * i + 1] = y;
     }
-    return r;
   }
+  return r;
 }
 
 __device__ __forceinline__ float finite_abs(float x) {
@@ -69,103 +81,173 @@ __device__ __forceinline__ u32x2 round_row8(const Row8& r, float inv) {
   return u32x2{f32x4_to_fp8(r.a * inv), f32x4_to_fp8(r.b * inv)};
 }
 
+// Marks the rows of the block that starts at slot `first` with their tokens (winner[r] becomes the last
+// token of row r) and returns whether any is before token t.  Sixteen slots a thread are on the way at once.
+__device__ __forceinline__ bool find_rows(const KVWriteFp8Params& p, int t, int first, int* winner) {
+  constexpr int kStep = 4;
+  const int n = p.num_tokens;
+  bool earlier = false;
+  const bool vec = (uintptr_t)p.slots % 16 == 0;
+  for (int i0 = threadIdx.x * 4; i0 < n; i0 += kWriteThreads * 4 * kStep) {
+    u32x4 s[kStep];
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      const int i = i0 + u * kWriteThreads * 4;
+      if (vec && i + 4 <= n) {
+        s[u] = *reinterpret_cast<const u32x4*>(p.slots + i);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][e] = (uint32_t)p.slots[min(i + e, n - 1)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      s[u] -= (uint32_t)first;
+      const uint32_t least = min(min(s[u][0], s[u][1]), min(s[u][2], s[u][3]));
+      if (least < (unsigned)p.block_size) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = i0 + u * kWriteThreads * 4 + e;
+          if (i < n && s[u][e] < (unsigned)p.block_size) {
+            earlier |= i < t;
+            atomicMax(&winner[s[u][e]], i);
+          }
+        }
+      }
+    }
+  }
+  return earlier;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads) kv_write_fp8_kernel(const KVWriteFp8Params p) {
   constexpr int LPR = D / 8;        // lanes of a row
   constexpr int RPI = 64 / LPR;     // rows a wave covers at once
+  constexpr int NW = kWriteThreads / 64;
   __shared__ int winner[kFp8MaxBlock];   // token that writes row r of the block, or -1
-  const int t = blockIdx.x;
   const int bs = p.block_size;
   const long long num_slots = (long long)p.num_blocks * bs;
-  auto slot_of = [&](int i) { return p.slots ? (long long)p.slots[i] : (long long)p.base_slot + i; };
-
-  const long long slot = slot_of(t);
-  if (slot < 0) return;
-  if (slot >= num_slots) {
-    if (threadIdx.x == 0 && blockIdx.y == 0 && p.err_count) atomicAdd(p.err_count, 1u);
-    return;
-  }
-  const int blk = (int)(slot / bs);
-  const long long first = (long long)blk * bs;      // slots [first, first + bs) are the block's
-  if (t > 0) {
-    const long long before = slot_of(t - 1) - first;
-    if (before >= 0 && before < bs) return;         // an earlier token's work-group owns the block
-  }
-  for (int r = threadIdx.x; r < bs; r += kWriteThreads) winner[r] = -1;
-  __syncthreads();
-  bool earlier = false;
-  for (int i = threadIdx.x; i < p.num_tokens; i += kWriteThreads) {
-    const long long r = slot_of(i) - first;
-    if (r >= 0 && r < bs) {
-      earlier |= i < t;
-      atomicMax(&winner[(int)r], i);
-    }
-  }
-  if (__syncthreads_or(earlier ? 1 : 0)) return;
-
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int lr = lane / LPR;
   const int lc = (lane % LPR) * 8;
   const int h0 = blockIdx.y * p.heads_per_group;
   const int units = 2 * min(p.heads_per_group, p.num_kv_heads - h0);
-  const bool restart = winner[0] >= 0;
-  for (int u = wave; u < units; u += kWriteThreads / 64) {
-    const int h = h0 + (u >> 1);
-    const bool is_v = u & 1;
-    const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (size_t)h * D + lc;
-    const long long stride = is_v ? p.v_stride : p.k_stride;
-    uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + ((size_t)blk * p.num_kv_heads + h) * bs * D + lc;
-    float* scale = (is_v ? p.v_scale : p.k_scale) + (size_t)blk * p.num_kv_heads + h;
-    const int old_e = fp8_scale_exp_of(*scale);
 
-    Row8 held[kWriteHold];
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kWriteHold; ++j) {
-      const int r = j * RPI + lr;
-      const int w = r < bs ? winner[r] : -1;
-      if (w >= 0) {
-        held[j] = load_row8<T>(src + (size_t)w * stride, p.aligned);
-        m = amax8(held[j], m);
-      }
+  // first tokens of runs in one block, found by every wave for the tokens that the work-group looks after
+  const int t0 = blockIdx.x * p.tokens_per_group;
+  int my_slot = -1;
+  bool head = false;
+  if (lane < p.tokens_per_group && t0 + lane < p.num_tokens) {
+    const int t = t0 + lane;
+    my_slot = p.slots ? p.slots[t] : p.base_slot + t;
+    const int before = t == 0 ? -1 : p.slots ? p.slots[t - 1] : my_slot - 1;
+    if (my_slot >= num_slots) {
+      if (wave == 0 && blockIdx.y == 0 && p.err_count) atomicAdd(p.err_count, 1u);
+    } else if (my_slot >= 0) {
+      const int first = my_slot / bs * bs;          // the block's slots: first .. first + bs - 1
+      head = (unsigned)before - (unsigned)first >= (unsigned)bs;
     }
-    for (int r = kWriteHold * RPI + lr; r < bs; r += RPI) {
-      const int w = winner[r];
-      if (w >= 0) m = amax8(load_row8<T>(src + (size_t)w * stride, p.aligned), m);
+  }
+  unsigned long long heads = __builtin_amdgcn_ballot_w64(head);
+  while (heads) {
+    const int at = __builtin_ctzll(heads);
+    heads &= heads - 1;
+    const int t = t0 + at;
+    const int slot = __builtin_amdgcn_readlane(my_slot, at);
+    const int blk = slot / bs;
+    const int first = blk * bs;
+    __syncthreads();                                // the run before is done with winner
+    for (int r = threadIdx.x; r < bs; r += kWriteThreads) {
+      const int from_base = r - (slot - first);
+      winner[r] = !p.slots && from_base >= 0 && from_base < p.num_tokens ? from_base : -1;
     }
-    m = group_max<64>(m);
-    const int own_e = fp8_scale_exp(m);
-    const int e = restart ? own_e : max(own_e, old_e);
-    const float inv = exp2_int(-e);
-    const float again = exp2_int(max(old_e - e, -126));   // of held rows, where the exponent grew
+    __syncthreads();
+    if (__syncthreads_or(p.slots && find_rows(p, t, first, winner) ? 1 : 0)) continue;
 
-    auto put = [&](int r, const Row8& x) {
-      *reinterpret_cast<u32x2*>(dst + (size_t)r * D) = round_row8(x, inv);
+    const bool restart = winner[0] >= 0;
+    struct Rows {
+      Raw8<T> x[kWriteHold];
+      float scale;
     };
-    auto keep = [&](int r) {
-      u32x2* q = reinterpret_cast<u32x2*>(dst + (size_t)r * D);
-      if (restart) {
-        *q = u32x2{0, 0};
-      } else if (e != old_e) {
-        const u32x2 w = *q;
-        *q = u32x2{f32x4_to_fp8(fp8_to_f32x4(w[0]) * again), f32x4_to_fp8(fp8_to_f32x4(w[1]) * again)};
+    auto source = [&](int u) {
+      return reinterpret_cast<const T*>(u & 1 ? p.v : p.k) + (size_t)(h0 + (u >> 1)) * D + lc;
+    };
+    auto scale_of = [&](int u) {
+      return (u & 1 ? p.v_scale : p.k_scale) + (size_t)blk * p.num_kv_heads + h0 + (u >> 1);
+    };
+    auto request = [&](int u, Rows& rows) {
+      const T* src = source(u);
+      const long long stride = u & 1 ? p.v_stride : p.k_stride;
+      rows.scale = *scale_of(u);
+#pragma unroll
+      for (int j = 0; j < kWriteHold; ++j) {
+        const int r = j * RPI + lr;
+        const int w = r < bs ? winner[r] : -1;
+        if (w >= 0) rows.x[j] = load_row8<T>(src + (size_t)w * stride, p.aligned);
       }
     };
+    auto write = [&](int u, const Rows& rows) {
+      const T* src = source(u);
+      const long long stride = u & 1 ? p.v_stride : p.k_stride;
+      uint8_t* dst = (u & 1 ? p.v_cache : p.k_cache) + ((size_t)blk * p.num_kv_heads + h0 + (u >> 1)) * bs * D + lc;
+      const int old_e = fp8_scale_exp_of(rows.scale);
+      float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kWriteHold; ++j) {
-      const int r = j * RPI + lr;
-      if (r < bs) {
-        if (winner[r] >= 0) put(r, held[j]);
+      for (int j = 0; j < kWriteHold; ++j) {
+        const int r = j * RPI + lr;
+        if (r < bs && winner[r] >= 0) m = amax8(as_floats<T>(rows.x[j]), m);
+      }
+      for (int r = kWriteHold * RPI + lr; r < bs; r += RPI) {
+        const int w = winner[r];
+        if (w >= 0) m = amax8(as_floats<T>(load_row8<T>(src + (size_t)w * stride, p.aligned)), m);
+      }
+      m = group_max<64>(m);
+      const int own_e = fp8_scale_exp(m);
+      const int e = restart ? own_e : max(own_e, old_e);
+      const float inv = exp2_int(-e);
+      const float again = exp2_int(max(old_e - e, -126));   // of held rows, where the exponent grew
+
+      auto put = [&](int r, const Row8& x) {
+        *reinterpret_cast<u32x2*>(dst + (size_t)r * D) = round_row8(x, inv);
+      };
+      auto keep = [&](int r) {
+        u32x2* q = reinterpret_cast<u32x2*>(dst + (size_t)r * D);
+        if (restart) {
+          *q = u32x2{0, 0};
+        } else if (e != old_e) {
+          const u32x2 w = *q;
+          *q = u32x2{f32x4_to_fp8(fp8_to_f32x4(w[0]) * again), f32x4_to_fp8(fp8_to_f32x4(w[1]) * again)};
+        }
+      };
+#pragma unroll
+      for (int j = 0; j < kWriteHold; ++j) {
+        const int r = j * RPI + lr;
+        if (r < bs) {
+          if (winner[r] >= 0) put(r, as_floats<T>(rows.x[j]));
+          else keep(r);
+        }
+      }
+      for (int r = kWriteHold * RPI + lr; r < bs; r += RPI) {
+        const int w = winner[r];
+        if (w >= 0) put(r, as_floats<T>(load_row8<T>(src + (size_t)w * stride, p.aligned)));
         else keep(r);
       }
+      if (lane == 0) *scale_of(u) = exp2_int(e);
+    };
+    // the wave's next (head, cache) pair is on its way while one is rounded
+    if (wave < units) {
+      Rows ra, rb;
+      request(wave, ra);
+      for (int u = wave;; u += 2 * NW) {
+        if (u + NW < units) request(u + NW, rb);
+        write(u, ra);
+        if (u + NW >= units) break;
+        if (u + 2 * NW < units) request(u + 2 * NW, ra);
+        write(u + NW, rb);
+        if (u + 2 * NW >= units) break;
+      }
     }
-    for (int r = kWriteHold * RPI + lr; r < bs; r += RPI) {
-      const int w = winner[r];
-      if (w >= 0) put(r, load_row8<T>(src + (size_t)w * stride, p.aligned));
-      else keep(r);
-    }
-    if (lane == 0) *scale = exp2_int(e);
   }
 }
 
@@ -229,8 +311,16 @@ void write_of(const KVWriteFp8Params& p, dim3 grid, hipStream_t stream) {
 }  // namespace
 
 void launch_kv_write_fp8(KVWriteFp8Params p, int dtype, hipStream_t stream) {
-  p.heads_per_group = 2;            // four (head, cache) pairs: one a wave
-  const dim3 grid(p.num_tokens, (p.num_kv_heads + p.heads_per_group - 1) / p.heads_per_group);
+  // A step's tokens lie in blocks of their own: one token and four (head, cache)
+  // pairs, one a wave, per work-group.  A prompt's are in runs: sixteen tokens, and
+  // all heads once that gives every CU two work-groups, since each reads the slots.
+  p.tokens_per_group = p.num_tokens <= kWriteFewTokens ? 1 : 16;
+  const int groups = (p.num_tokens + p.tokens_per_group - 1) / p.tokens_per_group;
+  p.heads_per_group = 2;
+  while (p.tokens_per_group > 1 && p.heads_per_group < p.num_kv_heads &&
+         (long long)groups * p.num_kv_heads >= kWriteGroups * 2 * p.heads_per_group)
+    p.heads_per_group *= 2;
+  const dim3 grid(groups, (p.num_kv_heads + p.heads_per_group - 1) / p.heads_per_group);
   if (dtype == kF32) write_of<float>(p, grid, stream);
   else if (dtype == kF16) write_of<_Float16>(p, grid, stream);
   else write_of<__bf16>(p, grid, stream);

@@ -79,6 +79,7 @@ struct KVWriteFp8Params {
   long long k_stride;    // elements between consecutive tokens
   long long v_stride;
   int heads_per_group;   // KV heads of one work-group
+  int tokens_per_group;  // tokens whose blocks one work-group looks after
   bool aligned;          // rows of k and v start at multiples of 16 bytes
   unsigned* err_count;   // may be null
 };
