@@ -64,6 +64,19 @@ __device__ __forceinline__ void buffer_load_v(__amdgpu_buffer_rsrc_t r, int off,
   }
 }
 
+// Buffer resource of `bytes` bytes from a wave-uniform address.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* base, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), (short)0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
+// What no kernel writes while this one runs, at a wave-uniform address: a scalar load.
+template <typename V> __device__ __forceinline__ V uniform_load(const V* p) {
+  return *(const __attribute__((address_space(4))) V*)(p);
+}
+
 // Bytes d of four words (tokens) to four words of tokens (dims).
 __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4]) {
   const uint32_t ab01 = __builtin_amdgcn_perm(b, a, 0x05010400u);   // a0 b0 a1 b1
@@ -81,8 +94,8 @@ template <int D, int NW> struct Smem {
   float m[NW][kCols], l[NW][kCols];
 };
 
-// T: the queries' type.  UB: every 16-token half tile lies in one block
-// (block_size % 16 == 0), so its id, its scales and its address are uniform.
+// T: the queries' type.  UB: the block size is 16 or a larger power of two, so
+// every 16-token half tile lies in one block whose id, scales and address are uniform.
 template <typename T, int D, int NW, bool UB>
 __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeFp8Params p) {
   using S = typename ScoreType<T>::type;
@@ -97,7 +110,7 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
   int part = 0, b, ky;
   if (p.sched) {
     const int rows = p.num_kv_heads * p.head_chunks;
-    b = p.sched[1 + blockIdx.x / rows];
+    b = __builtin_amdgcn_readfirstlane(p.sched[1 + blockIdx.x / rows]);
     ky = blockIdx.x % rows;
   } else {
     part = blockIdx.x;
@@ -160,7 +173,7 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
 #pragma unroll
   for (int i = 0; i < VB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = kNegInf, l = 0.0f;        // of query c, the same in its four lanes (m), a lane's own share (l)
-  bool bad = false;
+  int bad = 0;
   const float sc = p.scale * kLog2e;
 
   struct Tile {
@@ -168,27 +181,28 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
     uint32_t v[2][4][VW];
     f32x4 ks[2], vs[2];               // scales of tokens 4 g .. 4 g + 3 of each half
   };
-  auto column = [&](int t) { return p.bs_log2 >= 0 ? t >> p.bs_log2 : t / bs; };
-  auto block_of = [&](int t) { return bt[column(min(t, end - 1))]; };   // the last token's past the end
+  auto column = [&](int t) { return UB ? t >> p.bs_log2 : t / bs; };
+  auto block_of = [&](int t) { return uniform_load(bt + column(min(t, end - 1))); };   // the last token's past the end
 
   auto load = [&](int t0, const int (&ids)[2], Tile& w) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int ts = t0 + 16 * s;
       if constexpr (UB) {
-        const bool ok = (unsigned)ids[s] < (unsigned)p.num_blocks;
-        bad |= !ok && ts < end;
-        const int rows = ok ? max(0, min(16, end - ts)) : 0;
-        const size_t unit = (size_t)(ok ? ids[s] : 0) * p.num_kv_heads + kh;
-        const size_t at = unit * unit_bytes + (size_t)(ts - column(ts) * bs) * D;
-        const auto kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.k_cache + at), (short)0, rows * D, 0x00020000);
-        const auto vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.v_cache + at), (short)0, rows * D, 0x00020000);
+        const int id = __builtin_amdgcn_readfirstlane(ids[s]);
+        const int ok = (unsigned)id < (unsigned)p.num_blocks ? -1 : 0;
+        const int rows = max(0, min(16, end - ts));
+        bad |= rows & ~ok;
+        const size_t unit = (size_t)(id & ok) * p.num_kv_heads + kh;
+        const size_t at = unit * unit_bytes + (size_t)(ts & (bs - 1)) * D;
+        const auto kr = rows_rsrc(p.k_cache + at, (rows & ok) * D);
+        const auto vr = rows_rsrc(p.v_cache + at, (rows & ok) * D);
 #pragma unroll
         for (int i = 0; i < KV; ++i)
           w.k[s][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, c * D + 64 * i + 16 * g, 0, 2));
 #pragma unroll
         for (int i = 0; i < 4; ++i) buffer_load_v<VB>(vr, (4 * g + i) * D + c * VB, w.v[s][i]);
-        const float ks = p.k_scale[unit], vs = p.v_scale[unit];
+        const float ks = uniform_load(p.k_scale + unit), vs = uniform_load(p.v_scale + unit);
         w.ks[s] = f32x4{ks, ks, ks, ks};
         w.vs[s] = f32x4{vs, vs, vs, vs};
       } else {
@@ -199,7 +213,7 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
         if (ok) {
           const int col = column(tk), id = bt[col];
           ok = (unsigned)id < (unsigned)p.num_blocks;
-          bad |= !ok;
+          bad |= ok ? 0 : 1;
           at = ((size_t)(ok ? id : 0) * p.num_kv_heads + kh) * unit_bytes + (size_t)(tk - col * bs) * D;
         }
 #pragma unroll
@@ -257,7 +271,7 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
 #pragma unroll
     for (int s = 0; s < 2; ++s) mt = fmaxf(mt, fmaxf(fmaxf(st[s][0], st[s][1]), fmaxf(st[s][2], st[s][3])));
     if (__builtin_amdgcn_ballot_w64(mt > m + kSlack) != 0) {
-      __asm__ volatile("" ::: "memory");   // keeps this rare block a branch
+      __asm__ volatile("");   // keeps this rare block a branch (no memory clobber: table and scales stay scalar loads)
       const float mm = max_over_g(mt);
       const float mn = mm > m + kSlack ? mm : m;
       const float alpha = mn == m ? 1.0f : fast_exp2(m - mn);
@@ -309,25 +323,21 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
     load(t, ids, ta);
     ids[0] = block_of(t + step);
     ids[1] = block_of(t + step + 16);
+    // Requests past the end ask for no rows: a branch around them would have the
+    // present tile wait for the next one's loads where the paths meet.
     for (;;) {
-      const bool more = t + step < end;
-      if (more) {
-        load(t + step, ids, tb);
-        ids[0] = block_of(t + 2 * step);
-        ids[1] = block_of(t + 2 * step + 16);
-      }
+      load(t + step, ids, tb);
+      ids[0] = block_of(t + 2 * step);
+      ids[1] = block_of(t + 2 * step + 16);
       compute(t, ta);
-      if (!more) break;
       t += step;
-      const bool again = t + step < end;
-      if (again) {
-        load(t + step, ids, ta);
-        ids[0] = block_of(t + 2 * step);
-        ids[1] = block_of(t + 2 * step + 16);
-      }
+      if (t >= end) break;
+      load(t + step, ids, ta);
+      ids[0] = block_of(t + 2 * step);
+      ids[1] = block_of(t + 2 * step + 16);
       compute(t, tb);
-      if (!again) break;
       t += step;
+      if (t >= end) break;
     }
   }
 
@@ -412,7 +422,7 @@ template <typename T, int D, int NW>
 void launch_of(const DecodeFp8Params& p, hipStream_t stream) {
   const int rows = p.num_kv_heads * p.head_chunks;
   const dim3 grid = p.sched ? dim3(p.num_seqs * rows) : dim3(p.max_parts, rows, p.num_seqs);
-  if (p.block_size % 16 == 0)
+  if (p.bs_log2 >= 4)
     hipLaunchKernelGGL((paged_decode_fp8_kernel<T, D, NW, true>), grid, dim3(64 * NW), 0, stream, p);
   else
     hipLaunchKernelGGL((paged_decode_fp8_kernel<T, D, NW, false>), grid, dim3(64 * NW), 0, stream, p);
