@@ -174,10 +174,11 @@ int tv_paged_decode_fp8_partition_size(int num_seqs, int num_heads, int num_kv_h
   const long long width = (long long)max_blocks * block_size;
   const int whole = (int)((width + 31) / 32 * 32);
   const long long rows = decode_rows(num_seqs, num_heads, num_kv_heads);
-  if (rows >= 4LL * cus) return whole;
-  if (rows <= cus && width <= tv::kFp8WideTokens) return whole;
-  const int slots = tv::decode_fp8_slots(head_dim, dtype);
-  const long long parts = ((long long)slots + rows - 1) / rows;
+  // One work-group per CU keeps enough loads on the way; more of them only add
+  // parts to write and join (MI355X, 32 / 8 heads of 128: 16 x 32768 tokens in 2
+  // partitions 169, 4 171, 12 177 us; 1 x 8000 in 32 partitions 10.8, 63 13.4).
+  if (rows >= cus || width <= tv::kFp8WideTokens) return whole;
+  const long long parts = (cus + rows - 1) / rows;
   long long p = (width + parts - 1) / parts;
   p = std::max(128LL, (p + 31) / 32 * 32);
   return p < whole ? (int)p : whole;
@@ -211,10 +212,12 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
                                                           partition_size);
   if (max_parts > 1 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
     return fail(TV_EINVAL, "%s: workspace of %zu bytes required (got %zu)", who, need, workspace_bytes);
-  const bool ordered = max_parts == 1 && need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4);
+  // longest first only where work-groups wait for others to end (two are resident per CU)
+  const bool ordered = max_parts == 1 && need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4) &&
+                       decode_rows(num_seqs, num_heads, num_kv_heads) > 2LL * device_cus();
   const int group = num_heads / num_kv_heads;
   const int chunks = (group + 15) / 16;
-  if (num_seqs > 65535 || (long long)num_kv_heads * chunks > 65535 || num_heads > 0x7fffffff / 256)
+  if (num_seqs > 65535 || max_parts > 65535 || num_heads > 0x7fffffff / 256)
     return fail(TV_EINVAL, "%s: grid too large", who);
 
   tv::DecodeFp8Params p{};

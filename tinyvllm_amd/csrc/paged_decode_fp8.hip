@@ -31,7 +31,6 @@
 // one is used, and its block ids one tile before that.
 #include "tv_fp8.h"
 
-#include "tv_device_cache.h"
 #include "tv_split.h"
 
 namespace tv {
@@ -113,9 +112,13 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
     b = __builtin_amdgcn_readfirstlane(p.sched[1 + blockIdx.x / rows]);
     ky = blockIdx.x % rows;
   } else {
-    part = blockIdx.x;
-    ky = blockIdx.y;
-    b = blockIdx.z;
+    // Heads fastest: they lie side by side in a block.  Partitions slowest: later
+    // ones are shorter or empty, and work-groups are dealt to the CU groups in turn,
+    // so with partitions next to each other some of these get only the short ones
+    // (256 sequences of 512..4096 tokens in partitions of 1024: 314 us).
+    ky = blockIdx.x;
+    b = blockIdx.y;
+    part = blockIdx.z;
   }
   const int width = p.max_blocks * p.block_size;
   const int len = min(p.context_lens[b], width);
@@ -382,52 +385,90 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
 }
 
 // Merges the partitions of a (query head, sequence): out = sum_p w_p o_p / sum_p
-// w_p, w_p = L_p 2^(M_p - max M).  One thread a dim; a partition's weight is the
-// same for all of them and comes from LDS.
-template <int D>
-__global__ void __launch_bounds__(D) paged_decode_fp8_merge_kernel(const DecodeFp8Params p) {
-  constexpr int CH = 256;
+// w_p, w_p = L_p 2^(M_p - max M).  NT threads: a dim each, and NT / D groups that
+// take partitions g, g + groups, ...; eight partitions a thread are on the way at
+// once (a loop of single dependent reads took most of a split call's time).
+template <int D, int NT>
+__global__ void __launch_bounds__(NT) paged_decode_fp8_merge_kernel(const DecodeFp8Params p) {
+  constexpr int CH = 1024;          // partitions whose weights are in LDS at once
+  constexpr int G = NT / D;
   __shared__ float sw[CH];
-  const int h = blockIdx.x, b = blockIdx.y;
+  __shared__ float red[NT / 64];
+  __shared__ float snum[NT], sden[NT];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int len = min(p.context_lens[b], p.max_blocks * p.block_size);
   const int nparts = (len + p.partition_size - 1) / p.partition_size;
   if (nparts <= 1) return;
   const size_t row = (size_t)b * p.num_heads + h;
   const float* ml = p.part_ml + row * p.max_parts * 2;
   const float* po = p.part_o + row * p.max_parts * D;
-  const int d = threadIdx.x;
   float M = kNegInf;
   bool nan = false;
-  for (int i = 0; i < nparts; ++i) {
+  for (int i = tid; i < nparts; i += NT) {
     const float mi = ml[2 * i];
     nan |= mi != mi;
     M = fmaxf(M, mi);
   }
+  M = group_max<64>(M);
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  nan = __syncthreads_or(nan ? 1 : 0) != 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) M = fmaxf(M, red[i]);
+  const int d = tid % D, g = tid / D;
   float num = 0.0f, den = 0.0f;
   for (int c0 = 0; c0 < nparts; c0 += CH) {
     const int cn = min(CH, nparts - c0);
     __syncthreads();
-    for (int i = d; i < cn; i += D) sw[i] = ml[2 * (c0 + i) + 1] * fast_exp2(ml[2 * (c0 + i)] - M);
+    for (int i = tid; i < cn; i += NT) sw[i] = ml[2 * (c0 + i) + 1] * fast_exp2(ml[2 * (c0 + i)] - M);
     __syncthreads();
-#pragma unroll 4
-    for (int i = 0; i < cn; ++i) {
+    int i = g;
+    for (; i + 7 * G < cn; i += 8 * G) {
+      float o[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) o[u] = po[(size_t)(c0 + i + u * G) * D + d];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        den += sw[i + u * G];
+        num = fmaf(sw[i + u * G], o[u], num);
+      }
+    }
+    for (; i < cn; i += G) {
       den += sw[i];
       num = fmaf(sw[i], po[(size_t)(c0 + i) * D + d], num);
+    }
+  }
+  if constexpr (G > 1) {
+    snum[tid] = num;
+    sden[tid] = den;
+    __syncthreads();
+    if (g != 0) return;
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+      num += snum[tid + k * D];
+      den += sden[tid + k * D];
     }
   }
   store_as(p.out, row * D + d, nan ? __builtin_nanf("") : num / den, p.out_dtype);
 }
 
+// Few partitions want few threads (64 heads' worth of 4: 13.9 against 15.8 us for a
+// whole call), many want all of them (63 partitions of 8 heads: 13.4 against 18.9).
+template <int D> void launch_merge(const DecodeFp8Params& p, hipStream_t stream) {
+  const dim3 grid(p.num_heads, p.num_seqs);
+  if (p.max_parts <= 16) hipLaunchKernelGGL((paged_decode_fp8_merge_kernel<D, D>), grid, dim3(D), 0, stream, p);
+  else hipLaunchKernelGGL((paged_decode_fp8_merge_kernel<D, 256>), grid, dim3(256), 0, stream, p);
+}
+
 template <typename T, int D, int NW>
 void launch_of(const DecodeFp8Params& p, hipStream_t stream) {
   const int rows = p.num_kv_heads * p.head_chunks;
-  const dim3 grid = p.sched ? dim3(p.num_seqs * rows) : dim3(p.max_parts, rows, p.num_seqs);
+  const dim3 grid = p.sched ? dim3(p.num_seqs * rows) : dim3(rows, p.num_seqs, p.max_parts);
   if (p.bs_log2 >= 4)
     hipLaunchKernelGGL((paged_decode_fp8_kernel<T, D, NW, true>), grid, dim3(64 * NW), 0, stream, p);
   else
     hipLaunchKernelGGL((paged_decode_fp8_kernel<T, D, NW, false>), grid, dim3(64 * NW), 0, stream, p);
   if (p.max_parts > 1)
-    hipLaunchKernelGGL(paged_decode_fp8_merge_kernel<D>, dim3(p.num_heads, p.num_seqs), dim3(D), 0, stream, p);
+    launch_merge<D>(p, stream);
 }
 
 template <typename T>
@@ -437,20 +478,7 @@ void launch_dims(const DecodeFp8Params& p, int head_dim, bool wide, hipStream_t 
   else launch_of<T, 256, 4>(p, stream);
 }
 
-template <typename T, int D> int slots_of() {
-  static std::atomic<long long> slots[kMaxDevices];
-  return (int)resident_work_groups(slots, paged_decode_fp8_kernel<T, D, 4, true>, 256);
-}
-template <typename T> int slots_dims(int head_dim) {
-  return head_dim == 64 ? slots_of<T, 64>() : head_dim == 128 ? slots_of<T, 128>() : slots_of<T, 256>();
-}
-
 }  // namespace
-
-int decode_fp8_slots(int head_dim, int dtype) {
-  return dtype == kF32 ? slots_dims<float>(head_dim)
-         : dtype == kF16 ? slots_dims<_Float16>(head_dim) : slots_dims<__bf16>(head_dim);
-}
 
 void launch_paged_decode_fp8(const DecodeFp8Params& p, int head_dim, int dtype, bool wide, hipStream_t stream) {
   if (dtype == kF32) launch_dims<float>(p, head_dim, wide, stream);

@@ -127,7 +127,6 @@ struct DecodeFp8Params {
   const int* sched;          // unsplit launch of many sequences: [1 ..] their longest-first order
 };
 
-int decode_fp8_slots(int head_dim, int dtype);   // work-groups resident at once on the current device
 void launch_paged_decode_fp8(const DecodeFp8Params& p, int head_dim, int dtype, bool wide, hipStream_t stream);
 
 // Attention of a chunk's rows over the 8-bit cache (flash_prefill_fp8.hip).
