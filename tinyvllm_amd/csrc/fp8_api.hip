@@ -174,11 +174,19 @@ int tv_paged_decode_fp8_partition_size(int num_seqs, int num_heads, int num_kv_h
   const long long width = (long long)max_blocks * block_size;
   const int whole = (int)((width + 31) / 32 * 32);
   const long long rows = decode_rows(num_seqs, num_heads, num_kv_heads);
-  // One work-group per CU keeps enough loads on the way; more of them only add
-  // parts to write and join (MI355X, 32 / 8 heads of 128: 16 x 32768 tokens in 2
-  // partitions 169, 4 171, 12 177 us; 1 x 8000 in 32 partitions 10.8, 63 13.4).
-  if (rows >= cus || width <= tv::kFp8WideTokens) return whole;
-  const long long parts = (cus + rows - 1) / rows;
+  if (rows >= 2LL * cus || width <= tv::kFp8WideTokens) return whole;
+  // Enough parts that every CU has one (of 32 KiB and more; two parts gain less
+  // than joining them costs), and, for contexts of more than 256 KiB a head, four
+  // per CU, whose ends even out.  MI355X, us, whole / this rule (equal lengths, and
+  // lengths down to half): 40 x 8000 tokens of 32 / 8 heads of 128 143 / 113, 121 /
+  // 94; 20 x 16000 138 / 113, 130 / 99; 24 x 4000 39 / 39, 37 / 40; 60 x 12000 234 /
+  // 245, 209 / 195; 16 x 32768 in 2 parts 171, in 8 175; 1 x 8000 30 / 11; 32 / 4
+  // heads of 64: 32 x 1000 stays whole, 9.4, in 2 parts 11.2.
+  const long long least = std::max(1LL, width * head_dim / 16384);
+  long long fill = std::min(cus / rows, least);
+  if (fill < 3) fill = 1;
+  const long long even = std::min((4LL * cus + rows - 1) / rows, (width * head_dim + 131071) / 131072);
+  const long long parts = std::max({1LL, fill, even});
   long long p = (width + parts - 1) / parts;
   p = std::max(128LL, (p + 31) / 32 * 32);
   return p < whole ? (int)p : whole;
