@@ -60,8 +60,14 @@ template <typename T> __device__ __forceinline__ u32x2 dequant4(uint32_t w, floa
 
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-template <typename T, int D, int RB, int BN>
-__global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillFp8Params p) {
+// NaN stays NaN (v_maximum3_f32): fmaxf would first have every operand made quiet.
+// A query with a NaN score raises no maximum; its row is NaN whatever the others are.
+__device__ __forceinline__ float max4(f32x4 x) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[0], x[1]), __builtin_elementwise_maximum(x[2], x[3]));
+}
+
+template <typename T, int D, int RB, int BN, int KS>
+__global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const PrefillFp8Params p) {
   constexpr int BM = 64 * RB;
   constexpr int KB = BN / 16;
   constexpr int KSD = D / 32;
@@ -73,9 +79,13 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillF
   constexpr int NV = BN * CPR / kThreads; // vectors per thread and tile, each of K and V
   constexpr int RPP = kThreads / CPR;     // tile rows of one pass over the threads
   static_assert(NV * kThreads == BN * CPR && NV >= 1, "tile shape");
-  __shared__ __attribute__((aligned(16))) uint16_t smem[2 * BUF];
+  constexpr int MP = D + 4;               // row pitch (floats) of the merge of two key groups
+  static_assert(KS == 1 || (KS == 2 && BM * (MP + 2) * 2 <= KS * 2 * BUF), "the merge fits the tiles' space");
+  __shared__ __attribute__((aligned(16))) uint16_t smem_all[KS * 2 * BUF];
 
-  const int tid = threadIdx.x;
+  const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  const int tid = threadIdx.x % kThreads;
+  uint16_t* const smem = smem_all + grp * 2 * BUF;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int g = lane >> 4, col = lane & 15;
@@ -177,16 +187,30 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillF
     const uint16_t* sv = sk + SKT;
     const int k0 = t * BN;
     f32x4 st[RB][KB];
+    // independent products next to each other: the sums of one score are KB RB apart
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+    for (int ks = 0; ks < KSD; ++ks) {
 #pragma unroll
-      for (int ks = 0; ks < KSD; ++ks) {
+      for (int kb = 0; kb < KB; ++kb) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + (kb * 16 + col) * P + ks * 32 + g * 8);
 #pragma unroll
         for (int r = 0; r < RB; ++r)
           st[r][kb] = mfma16x16x32<T>(kf, qf[r][ks], ks ? st[r][kb] : f32x4{0.f, 0.f, 0.f, 0.f});
       }
     }
+    __builtin_amdgcn_sched_barrier(0);   // all products before the first use of one: no waits between them
+    // V^T operands of the first 32 keys: from LDS while the softmax runs
+    u32x4 vf[DB];
+    auto values = [&](int x) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint16_t* a = sv + (x * 32 + 4 * g + (col >> 2)) * P + db * 16 + 4 * (col & 3);
+        const u32x2 lo = lds_read_tr16(a);
+        const u32x2 hi = lds_read_tr16(a + 16 * P);
+        vf[db] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    };
+    values(0);
     float base[RB];
     bool need = false;
 #pragma unroll
@@ -198,6 +222,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillF
         for (int i = 0; i < 4; ++i) st[r][kb][i] = fmaf(st[r][kb][i], c, -base[r]);
     }
     if (k0 + BN - 1 > first_seen) {
+      __asm__ volatile("");                // a branch, not 32 selects in every tile
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
         const int rel = (p.causal ? min(kv_len - 1, p.start_pos + qpos[r]) : kv_len - 1) - (k0 + 4 * g);
@@ -211,10 +236,9 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillF
     float mt[RB];
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      mt[r] = kNegInf;
+      mt[r] = max4(st[r][0]);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-        mt[r] = fmaxf(mt[r], fmaxf(fmaxf(st[r][kb][0], st[r][kb][1]), fmaxf(st[r][kb][2], st[r][kb][3])));
+      for (int kb = 1; kb < KB; ++kb) mt[r] = __builtin_elementwise_maximum(mt[r], max4(st[r][kb]));
       need |= mt[r] > (m[r] == kNegInf ? kNegInf : 8.0f);
     }
     if (__builtin_amdgcn_ballot_w64(need) != 0) {
@@ -244,38 +268,70 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_fp8_kernel(const PrefillF
 #pragma unroll
     for (int x = 0; x < BN / 32; ++x) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const uint16_t* a = sv + (x * 32 + 4 * g + (col >> 2)) * P + db * 16 + 4 * (col & 3);
-        const u32x2 lo = lds_read_tr16(a);
-        const u32x2 hi = lds_read_tr16(a + 16 * P);
-        const u32x4 vf = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int r = 0; r < RB; ++r) oacc[r][db] = mfma16x16x32<T>(vf, pf[r][x], oacc[r][db]);
-      }
+        for (int r = 0; r < RB; ++r) oacc[r][db] = mfma16x16x32<T>(vf[db], pf[r][x], oacc[r][db]);
+      if (x + 1 < BN / 32) values(x + 1);
 #pragma unroll
       for (int r = 0; r < RB; ++r) oacc[r][DB] = mfma16x16x32<T>(ones, pf[r][x], oacc[r][DB]);
     }
   };
 
-  if (t0 < t1) {
+  // group grp takes tiles t0 + grp, t0 + grp + KS, ...
+  const int steps = (t1 - t0 + KS - 1) / KS;
+  if (steps > 0) {
     Ids ids;
     Stage s;
-    ids_of(t0, ids);
-    gload(t0, ids, s);
-    ids_of(t0 + 1, ids);
+    const int first = t0 + grp;
+    ids_of(first, ids);
+    gload(first, ids, s);
+    ids_of(first + KS, ids);
     lstore(s, 0);
-    gload(t0 + 1, ids, s);
-    ids_of(t0 + 2, ids);
+    gload(first + KS, ids, s);
+    ids_of(first + 2 * KS, ids);
     lds_barrier();
-    for (int t = t0; t < t1; ++t) {
-      const int b = (t - t0) & 1;
-      compute(b, t);
-      if (t + 1 < t1) {
-        lstore(s, b ^ 1);
-        gload(t + 2, ids, s);
-        ids_of(t + 3, ids);
+    for (int j = 0; j < steps; ++j) {
+      const int t = first + j * KS;
+      if (t < t1) compute(j & 1, t);
+      if (j + 1 < steps) {
+        lstore(s, (j & 1) ^ 1);
+        gload(t + 2 * KS, ids, s);
+        ids_of(t + 3 * KS, ids);
       }
       lds_barrier();
+    }
+  }
+  if constexpr (KS == 2) {
+    // the second group's rows join the first's through LDS
+    float* so = reinterpret_cast<float*>(smem_all);
+    float* sml = so + BM * MP;
+    if (grp == 1) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const int row = (wave * RB + r) * 16 + col;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(so + row * MP + db * 16 + 4 * g) = oacc[r][db];
+        if (g == 0) {
+          sml[2 * row] = m[r];
+          sml[2 * row + 1] = oacc[r][DB][0];
+        }
+      }
+    }
+    lds_barrier();
+    if (grp == 1) return;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int row = (wave * RB + r) * 16 + col;
+      const float m1 = sml[2 * row], l1 = sml[2 * row + 1];
+      const float M = fmaxf(m[r], m1);
+      // without a maximum a group has no keys of this row (zeros) or only NaN
+      const float f0 = m[r] == kNegInf ? 1.0f : fast_exp2(m[r] - M);
+      const float f1 = m1 == kNegInf ? 1.0f : fast_exp2(m1 - M);
+      m[r] = M;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        oacc[r][db] = oacc[r][db] * f0 + *reinterpret_cast<const f32x4*>(so + row * MP + db * 16 + 4 * g) * f1;
+      oacc[r][DB][0] = oacc[r][DB][0] * f0 + l1 * f1;
     }
   }
 
@@ -342,40 +398,47 @@ __global__ void __launch_bounds__(256) prefill_fp8_merge_kernel(const PrefillFp8
     *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
 }
 
-int block_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
 int tile_keys(int head_dim) { return head_dim == 256 ? 32 : 64; }
 
-template <typename T, int D, int RB, int BN>
+template <typename T, int D, int RB, int BN, int KS>
 void launch_of(const PrefillFp8Params& p, hipStream_t stream) {
   const long long rows = (long long)p.q_len * p.group;
   const dim3 grid(p.num_kv_heads, (unsigned)((rows + 64 * RB - 1) / (64 * RB)), p.splits);
-  hipLaunchKernelGGL((prefill_fp8_kernel<T, D, RB, BN>), grid, dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL((prefill_fp8_kernel<T, D, RB, BN, KS>), grid, dim3(kThreads * KS), 0, stream, p);
   if (p.splits > 1) {
     const long long items = rows * p.num_kv_heads, per = 256 / (D / 4);
     hipLaunchKernelGGL((prefill_fp8_merge_kernel<T, D>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, stream, p);
   }
 }
 
-template <typename T> void launch_dims(const PrefillFp8Params& p, int head_dim, hipStream_t stream) {
-  if (head_dim == 64) launch_of<T, 64, 2, 64>(p, stream);
-  else if (head_dim == 128) launch_of<T, 128, 2, 64>(p, stream);
-  else launch_of<T, 256, 1, 32>(p, stream);
+template <typename T> void launch_dims(const PrefillFp8Params& p, int head_dim, bool wide, hipStream_t stream) {
+  if (head_dim == 64) wide ? launch_of<T, 64, 2, 64, 1>(p, stream) : launch_of<T, 64, 1, 64, 2>(p, stream);
+  else if (head_dim == 128) wide ? launch_of<T, 128, 2, 64, 1>(p, stream) : launch_of<T, 128, 1, 64, 2>(p, stream);
+  else launch_of<T, 256, 1, 32, 1>(p, stream);
+}
+
+// 128-row work-groups of 4 waves where they give every CU two; else 64 rows and
+// two key groups of 4 waves, one work-group per CU.
+bool wide_rows(long long rows, int num_kv_heads, int head_dim, int cus) {
+  return head_dim != 256 && (rows + 127) / 128 * num_kv_heads * 4 >= 7LL * cus;
 }
 
 }  // namespace
 
-// Key splits: as many as fill two work-groups per CU, each of at least four key tiles.
+// Key splits: as many as give every CU its work-groups, each of at least four key tiles.
 int prefill_fp8_splits(int q_len, int start_pos, int num_heads, int num_kv_heads, int head_dim, int cus) {
   const long long rows = (long long)q_len * (num_heads / num_kv_heads);
-  const long long wgs = (rows + block_rows(head_dim) - 1) / block_rows(head_dim) * num_kv_heads;
+  if (wide_rows(rows, num_kv_heads, head_dim, cus)) return 1;
+  const long long wgs = (rows + 63) / 64 * num_kv_heads;
   const int tiles = (int)(((long long)start_pos + q_len + tile_keys(head_dim) - 1) / tile_keys(head_dim));
-  const long long want = 2LL * cus / std::max(1LL, wgs);
+  const long long want = (head_dim == 256 ? 2LL : 1LL) * cus / std::max(1LL, wgs);
   return (int)std::max(1LL, std::min({want, (long long)tiles / 4, 64LL}));
 }
 
-void launch_prefill_fp8(const PrefillFp8Params& p, int head_dim, int dtype, hipStream_t stream) {
-  if (dtype == kF16) launch_dims<_Float16>(p, head_dim, stream);
-  else launch_dims<__bf16>(p, head_dim, stream);
+void launch_prefill_fp8(const PrefillFp8Params& p, int head_dim, int dtype, int cus, hipStream_t stream) {
+  const bool wide = p.splits == 1 && wide_rows((long long)p.q_len * p.group, p.num_kv_heads, head_dim, cus);
+  if (dtype == kF16) launch_dims<_Float16>(p, head_dim, wide, stream);
+  else launch_dims<__bf16>(p, head_dim, wide, stream);
 }
 
 }  // namespace tv

@@ -328,7 +328,7 @@ int tv_flash_prefill_paged_fp8(void* out, const void* q, const void* k_cache, co
     p.part_o = reinterpret_cast<float*>(workspace);
     p.part_ml = p.part_o + (size_t)p.splits * q_len * num_heads * head_dim;
   }
-  tv::launch_prefill_fp8(p, head_dim, dtype, reinterpret_cast<hipStream_t>(stream));
+  tv::launch_prefill_fp8(p, head_dim, dtype, device_cus(), reinterpret_cast<hipStream_t>(stream));
   return check_launch(who);
 }
 

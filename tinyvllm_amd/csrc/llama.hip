@@ -632,8 +632,8 @@ int tv_token_logprobs(float* logprobs, float* entropy, int32_t* top_ids, float* 
   const size_t need = tv_token_logprobs_workspace_bytes(M, vocab, top_k, dtype);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
     return fail(TV_EINVAL, "%s: workspace of %zu bytes, 8-byte aligned, required (got %zu)", who, need, workspace_bytes);
+  if ((long long)vocab * es > (1LL << 30)) return fail(TV_EINVAL, "%s: rows of %d logits are too long", who, vocab);
   const int segs = tv::logprob_segments(vocab, es);
-  if (segs > 65535) return fail(TV_EINVAL, "%s: grid too large", who);
   tv::LogprobParams p{};
   p.logits = logits;
   p.tokens = tokens;

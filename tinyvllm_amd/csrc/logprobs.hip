@@ -91,7 +91,7 @@ __device__ __forceinline__ void finish_row(const LogprobParams& p, int row, floa
 }
 
 template <typename T, int NT, bool ALIGNED>
-__global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) logprobs_kernel(const LogprobParams p) {
   constexpr int NW = NT / 64;
   constexpr int EPV = 16 / (int)sizeof(T);
   constexpr int SEG = NT * kVecs * EPV;
@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
   float tmax = kNegInf;
 #pragma unroll
   for (int j = 0; j < kVecs; ++j) {
+    __asm__ volatile("" : "+v"(tmax), "+v"(w[j]));
     vmax[j] = element<T>(w[j], 0);
 #pragma unroll
     for (int e = 1; e < EPV; ++e) vmax[j] = fmaxf(vmax[j], element<T>(w[j], e));
@@ -165,14 +166,16 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
   if (lane == 0) red[0][wave] = m;
   __syncthreads();
   m = red[0][0];
-#pragma unroll
+#pragma unroll 4
   for (int i = 1; i < NW; ++i) m = fmaxf(m, red[0][i]);
 
   // sums without the maximum's own term: elements equal to m count 1 each, less one for the row
   float s = 0.0f, t = 0.0f, eq = 0.0f;
   if (tmax < m) {
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j)
+    for (int j = 0; j < kVecs; ++j) {
+      // a vector at a time (the next one's terms depend on this): registers for two work-groups a CU
+      __asm__ volatile("" : "+v"(m), "+v"(s), "+v"(t), "+v"(w[j]));
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
         const float d = m - element<T>(w[j], e);
@@ -180,10 +183,12 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
         s += q;
         t = fmaf(fminf(d, kFar), q, t);
       }
+    }
   } else {
     int equal = 0;
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j)
+    for (int j = 0; j < kVecs; ++j) {
+      __asm__ volatile("" : "+v"(m), "+v"(s), "+v"(t), "+v"(w[j]));
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
         const float v = element<T>(w[j], e);
@@ -193,6 +198,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
         s += v == m ? 0.0f : q;
         t = v == m ? t : fmaf(fminf(d, kFar), q, t);
       }
+    }
     eq = (float)equal;
   }
   again();
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
   s = red[1][0];
   t = red[2][0];
   eq = red[3][0];
-#pragma unroll
+#pragma unroll 2
   for (int i = 1; i < NW; ++i) {
     s += red[1][i];
     t += red[2][i];
@@ -231,7 +237,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobParams p) {
 
   if (k > 0) {
     uint32_t b = bound[0];
-#pragma unroll
+#pragma unroll 4
     for (int i = 1; i < NW; ++i) b = max(b, bound[i]);
     const float least = b > order_bits(kNegInf) ? from_order_bits(b) : kNegInf;
     bool slow = s != s;             // a NaN

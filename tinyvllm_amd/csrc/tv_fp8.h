@@ -156,7 +156,7 @@ struct PrefillFp8Params {
 };
 
 int prefill_fp8_splits(int q_len, int start_pos, int num_heads, int num_kv_heads, int head_dim, int cus);
-void launch_prefill_fp8(const PrefillFp8Params& p, int head_dim, int dtype, hipStream_t stream);
+void launch_prefill_fp8(const PrefillFp8Params& p, int head_dim, int dtype, int cus, hipStream_t stream);
 
 void launch_kv_write_fp8(KVWriteFp8Params p, int dtype, hipStream_t stream);
 void launch_kv_gather_fp8(const KVGatherFp8Params& p, int dtype, hipStream_t stream);
