@@ -66,7 +66,10 @@ __device__ __forceinline__ float max4(f32x4 x) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[0], x[1]), __builtin_elementwise_maximum(x[2], x[3]));
 }
 
-template <typename T, int D, int RB, int BN, int KS>
+// UB: the block size is 16 or a larger power of two.  The rows that a wave stages
+// at once (4, 8 or 16, from a multiple of their number) then lie in one block, so
+// the block id, its scales and its address are scalar and cost no vector work.
+template <typename T, int D, int RB, int BN, int KS, bool UB>
 __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const PrefillFp8Params p) {
   constexpr int BM = 64 * RB;
   constexpr int KB = BN / 16;
@@ -118,55 +121,92 @@ __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const Pre
 
   // staging: this thread's vectors are chunk ch of tile rows sr + RPP i
   const int sr = tid / CPR, ch = tid % CPR;
-  const int bs = p.block_size, lg = p.bs_log2;
-  auto column = [&](int key) { return lg >= 0 ? key >> lg : key / bs; };
+  const int wr = wave * (64 / CPR);       // first of the wave's rows
+  const int bs = p.block_size;
+  const size_t unit_bytes = (size_t)bs * D;
+  auto column = [&](int key) { return UB ? key >> p.bs_log2 : key / bs; };
+  // the key whose block a vector's rows are looked up by, and that key kept inside the sequence
+  auto key_of = [&](int t, int i) { return t * BN + (UB ? wr : sr) + RPP * i; };
   struct Ids { int id[NV]; };
-  struct Stage { u32x4 k[NV], v[NV]; float ks[NV], vs[NV]; bool ok[NV], in[NV]; };
+  struct Stage { u32x4 k[NV], v[NV]; float ks[NV], vs[NV]; int ok[NV]; };
   auto ids_of = [&](int t, Ids& x) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x.id[i] = p.block_table[column(min(t * BN + sr + RPP * i, kv_len - 1))];
+    for (int i = 0; i < NV; ++i) {
+      const int* at = p.block_table + column(min(key_of(t, i), kv_len - 1));
+      x.id[i] = UB ? uniform_load(at) : *at;
+    }
   };
   auto gload = [&](int t, const Ids& x, Stage& s) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int key = t * BN + sr + RPP * i;
-      s.in[i] = key < kv_len && t < t1;
-      s.ok[i] = (unsigned)x.id[i] < (unsigned)p.num_blocks;
-      const size_t unit = (size_t)(s.ok[i] ? x.id[i] : 0) * p.num_kv_heads + kh;
-      const int k1 = min(key, kv_len - 1);
-      const size_t at = (unit * bs + (k1 - column(k1) * bs)) * D + ch * 16;
-      s.k[i] = *reinterpret_cast<const u32x4*>(p.k_cache + at);
-      s.v[i] = *reinterpret_cast<const u32x4*>(p.v_cache + at);
-      s.ks[i] = p.k_scale[unit];
-      s.vs[i] = p.v_scale[unit];
+      const int id = UB ? __builtin_amdgcn_readfirstlane(x.id[i]) : x.id[i];
+      s.ok[i] = (unsigned)id < (unsigned)p.num_blocks ? -1 : 0;
+      const size_t unit = (size_t)(id & s.ok[i]) * p.num_kv_heads + kh;
+      if constexpr (UB) {
+        // rows past the sequence's end are the block's own (whatever it holds there)
+        const size_t at = unit * unit_bytes + (size_t)(key_of(t, i) & (bs - 1)) * D;
+        const int lane_at = (sr - wr) * D + ch * 16;
+        s.k[i] = *reinterpret_cast<const u32x4*>(p.k_cache + at + lane_at);
+        s.v[i] = *reinterpret_cast<const u32x4*>(p.v_cache + at + lane_at);
+        s.ks[i] = uniform_load(p.k_scale + unit);
+        s.vs[i] = uniform_load(p.v_scale + unit);
+      } else {
+        const int key = min(key_of(t, i), kv_len - 1);
+        const size_t at = unit * unit_bytes + (size_t)(key - column(key) * bs) * D + ch * 16;
+        s.k[i] = *reinterpret_cast<const u32x4*>(p.k_cache + at);
+        s.v[i] = *reinterpret_cast<const u32x4*>(p.v_cache + at);
+        s.ks[i] = p.k_scale[unit];
+        s.vs[i] = p.v_scale[unit];
+      }
     }
   };
-  auto lstore = [&](const Stage& s, int b) {
+  auto put = [&](int b, int i, const u32x2 (&kw)[4], const u32x2 (&vw)[4]) {
+    uint16_t* dk = smem + b * BUF + (sr + RPP * i) * P + ch * 16;
+    *reinterpret_cast<u32x4*>(dk) = u32x4{kw[0][0], kw[0][1], kw[1][0], kw[1][1]};
+    *reinterpret_cast<u32x4*>(dk + 8) = u32x4{kw[2][0], kw[2][1], kw[3][0], kw[3][1]};
+    *reinterpret_cast<u32x4*>(dk + SKT) = u32x4{vw[0][0], vw[0][1], vw[1][0], vw[1][1]};
+    *reinterpret_cast<u32x4*>(dk + SKT + 8) = u32x4{vw[2][0], vw[2][1], vw[3][0], vw[3][1]};
+  };
+  auto lstore = [&](const Stage& s, int b, int t) {
+    // Nearly every tile: all of its keys inside the sequence, in blocks of the cache, no NaN among the
+    // values and scales that fp16 holds.
+    bool special = (t + 1) * BN > kv_len;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      uint16_t* dk = smem + b * BUF + (sr + RPP * i) * P + ch * 16;
-      u32x4 k = s.k[i], v = s.v[i];
-      if (!s.in[i]) k = v = u32x4{0, 0, 0, 0};   // keys past the last: masked, and their values zero
-      bool poison = s.in[i] && !s.ok[i];
-      if (poison || (nan_bytes(v[0]) | nan_bytes(v[1]) | nan_bytes(v[2]) | nan_bytes(v[3]))) {
-        poison = true;
+      uint32_t nan = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) nan |= (s.v[i][j] & 0x7f7f7f7fu) + 0x01010101u;
+      special |= (nan & 0x80808080u) != 0 || s.ok[i] == 0;
+      if constexpr (ElemTraits<T>::kCode == kF16) special |= s.ks[i] > 128.0f || s.vs[i] > 128.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(special) == 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        u32x2 kw[4], vw[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t bad = (nan_bytes(v[j]) >> 7) * 0xffu;
-          v[j] = s.ok[i] ? v[j] & ~bad : 0u;
+          kw[j] = u32x2{scaled_pair<T, false>(s.k[i][j], s.ks[i]), scaled_pair<T, true>(s.k[i][j], s.ks[i])};
+          vw[j] = u32x2{scaled_pair<T, false>(s.v[i][j], s.vs[i]), scaled_pair<T, true>(s.v[i][j], s.vs[i])};
         }
+        put(b, i, kw, vw);
       }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32x4 k = s.k[i], v = s.v[i];
+      const bool in = t * BN + sr + RPP * i < kv_len;
+      if (!in) k = v = u32x4{0, 0, 0, 0};        // masked, and their values zero
+      const bool poison = in && (s.ok[i] == 0 || (nan_bytes(v[0]) | nan_bytes(v[1]) | nan_bytes(v[2]) | nan_bytes(v[3])));
       u32x2 kw[4], vw[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        const uint32_t bad = (nan_bytes(v[j]) >> 7) * 0xffu;
         kw[j] = dequant4<T>(k[j], s.ks[i]);
-        vw[j] = dequant4<T>(v[j], s.vs[i]);
+        vw[j] = dequant4<T>(s.ok[i] ? v[j] & ~bad : 0u, s.vs[i]);
       }
       if (poison) kw[0][0] = kNan2<T>;
-      *reinterpret_cast<u32x4*>(dk) = u32x4{kw[0][0], kw[0][1], kw[1][0], kw[1][1]};
-      *reinterpret_cast<u32x4*>(dk + 8) = u32x4{kw[2][0], kw[2][1], kw[3][0], kw[3][1]};
-      *reinterpret_cast<u32x4*>(dk + SKT) = u32x4{vw[0][0], vw[0][1], vw[1][0], vw[1][1]};
-      *reinterpret_cast<u32x4*>(dk + SKT + 8) = u32x4{vw[2][0], vw[2][1], vw[3][0], vw[3][1]};
+      put(b, i, kw, vw);
     }
   };
 
@@ -286,7 +326,7 @@ __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const Pre
     ids_of(first, ids);
     gload(first, ids, s);
     ids_of(first + KS, ids);
-    lstore(s, 0);
+    lstore(s, 0, first);
     gload(first + KS, ids, s);
     ids_of(first + 2 * KS, ids);
     lds_barrier();
@@ -294,7 +334,7 @@ __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const Pre
       const int t = first + j * KS;
       if (t < t1) compute(j & 1, t);
       if (j + 1 < steps) {
-        lstore(s, (j & 1) ^ 1);
+        lstore(s, (j & 1) ^ 1, t + KS);
         gload(t + 2 * KS, ids, s);
         ids_of(t + 3 * KS, ids);
       }
@@ -404,7 +444,10 @@ template <typename T, int D, int RB, int BN, int KS>
 void launch_of(const PrefillFp8Params& p, hipStream_t stream) {
   const long long rows = (long long)p.q_len * p.group;
   const dim3 grid(p.num_kv_heads, (unsigned)((rows + 64 * RB - 1) / (64 * RB)), p.splits);
-  hipLaunchKernelGGL((prefill_fp8_kernel<T, D, RB, BN, KS>), grid, dim3(kThreads * KS), 0, stream, p);
+  if (p.bs_log2 >= 4)
+    hipLaunchKernelGGL((prefill_fp8_kernel<T, D, RB, BN, KS, true>), grid, dim3(kThreads * KS), 0, stream, p);
+  else
+    hipLaunchKernelGGL((prefill_fp8_kernel<T, D, RB, BN, KS, false>), grid, dim3(kThreads * KS), 0, stream, p);
   if (p.splits > 1) {
     const long long items = rows * p.num_kv_heads, per = 256 / (D / 4);
     hipLaunchKernelGGL((prefill_fp8_merge_kernel<T, D>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, stream, p);

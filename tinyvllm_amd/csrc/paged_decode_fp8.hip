@@ -71,11 +71,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* base,
                                            __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
-// What no kernel writes while this one runs, at a wave-uniform address: a scalar load.
-template <typename V> __device__ __forceinline__ V uniform_load(const V* p) {
-  return *(const __attribute__((address_space(4))) V*)(p);
-}
-
 // Bytes d of four words (tokens) to four words of tokens (dims).
 __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4]) {
   const uint32_t ab01 = __builtin_amdgcn_perm(b, a, 0x05010400u);   // a0 b0 a1 b1

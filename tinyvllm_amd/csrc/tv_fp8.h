@@ -38,6 +38,11 @@ __device__ __forceinline__ int fp8_scale_exp_of(float scale) {
   return e > kFp8MinExp ? e : kFp8MinExp;
 }
 
+// What no kernel writes while this one runs, at a wave-uniform address: a scalar load.
+template <typename V> __device__ __forceinline__ V uniform_load(const V* p) {
+  return *(const __attribute__((address_space(4))) V*)(p);
+}
+
 // Four e4m3 numbers to fp32, exactly.
 __device__ __forceinline__ f32x4 fp8_to_f32x4(uint32_t w) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
