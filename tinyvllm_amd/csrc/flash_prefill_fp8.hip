@@ -70,7 +70,7 @@ __device__ __forceinline__ float max4(f32x4 x) {
 // at once (4, 8 or 16, from a multiple of their number) then lie in one block, so
 // the block id, its scales and its address are scalar and cost no vector work.
 template <typename T, int D, int RB, int BN, int KS, bool UB>
-__global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const PrefillFp8Params p) {
+__global__ void __launch_bounds__(kThreads * KS, KS == 1 ? 2 : KS) prefill_fp8_kernel(const PrefillFp8Params p) {
   constexpr int BM = 64 * RB;
   constexpr int KB = BN / 16;
   constexpr int KSD = D / 32;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const Pre
   constexpr int RPP = kThreads / CPR;     // tile rows of one pass over the threads
   static_assert(NV * kThreads == BN * CPR && NV >= 1, "tile shape");
   constexpr int MP = D + 4;               // row pitch (floats) of the merge of two key groups
-  static_assert(KS == 1 || (KS == 2 && BM * (MP + 2) * 2 <= KS * 2 * BUF), "the merge fits the tiles' space");
+  static_assert((KS - 1) * BM * (MP + 2) * 2 <= KS * 2 * BUF, "the merge fits the tiles' space");
   __shared__ __attribute__((aligned(16))) uint16_t smem_all[KS * 2 * BUF];
 
   const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
@@ -341,14 +341,14 @@ __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const Pre
       lds_barrier();
     }
   }
-  if constexpr (KS == 2) {
-    // the second group's rows join the first's through LDS
+  if constexpr (KS > 1) {
+    // the other groups' rows join the first's through LDS
     float* so = reinterpret_cast<float*>(smem_all);
-    float* sml = so + BM * MP;
-    if (grp == 1) {
+    float* sml = so + (KS - 1) * BM * MP;
+    if (grp > 0) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        const int row = (wave * RB + r) * 16 + col;
+        const int row = (grp - 1) * BM + (wave * RB + r) * 16 + col;
 #pragma unroll
         for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(so + row * MP + db * 16 + 4 * g) = oacc[r][db];
         if (g == 0) {
@@ -358,20 +358,23 @@ __global__ void __launch_bounds__(kThreads * KS, 2) prefill_fp8_kernel(const Pre
       }
     }
     lds_barrier();
-    if (grp == 1) return;
+    if (grp > 0) return;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      const int row = (wave * RB + r) * 16 + col;
-      const float m1 = sml[2 * row], l1 = sml[2 * row + 1];
-      const float M = fmaxf(m[r], m1);
-      // without a maximum a group has no keys of this row (zeros) or only NaN
-      const float f0 = m[r] == kNegInf ? 1.0f : fast_exp2(m[r] - M);
-      const float f1 = m1 == kNegInf ? 1.0f : fast_exp2(m1 - M);
-      m[r] = M;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-        oacc[r][db] = oacc[r][db] * f0 + *reinterpret_cast<const f32x4*>(so + row * MP + db * 16 + 4 * g) * f1;
-      oacc[r][DB][0] = oacc[r][DB][0] * f0 + l1 * f1;
+      for (int k = 0; k < KS - 1; ++k) {
+        const int row = k * BM + (wave * RB + r) * 16 + col;
+        const float m1 = sml[2 * row], l1 = sml[2 * row + 1];
+        const float M = fmaxf(m[r], m1);
+        // without a maximum a group has no keys of this row (zeros) or only NaN
+        const float f0 = m[r] == kNegInf ? 1.0f : fast_exp2(m[r] - M);
+        const float f1 = m1 == kNegInf ? 1.0f : fast_exp2(m1 - M);
+        m[r] = M;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          oacc[r][db] = oacc[r][db] * f0 + *reinterpret_cast<const f32x4*>(so + row * MP + db * 16 + 4 * g) * f1;
+        oacc[r][DB][0] = oacc[r][DB][0] * f0 + l1 * f1;
+      }
     }
   }
 
@@ -417,17 +420,34 @@ __global__ void __launch_bounds__(256) prefill_fp8_merge_kernel(const PrefillFp8
   const int d = (threadIdx.x % TPR) * 4;
   const size_t step = (size_t)p.num_kv_heads * rows;
   const size_t slot0 = (size_t)kh * rows + row;
+  constexpr int U = 8;                    // parts on the way at once; past the last one they are read again and weigh nothing
   float M = kNegInf;
-  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[2 * (slot0 + s * step)]);
+  for (int s0 = 0; s0 < p.splits; s0 += U) {
+    float mv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) mv[u] = p.part_ml[2 * (slot0 + min(s0 + u, p.splits - 1) * step)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) M = fmaxf(M, mv[u]);
+  }
   f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
   float den = 0.0f;
-  for (int s = 0; s < p.splits; ++s) {
-    const size_t slot = slot0 + s * step;
-    const float l = p.part_ml[2 * slot + 1];
-    if (l == 0.0f) continue;
-    const float w = l * fast_exp2(p.part_ml[2 * slot] - M);
-    den += w;
-    num += *reinterpret_cast<const f32x4*>(p.part_o + slot * D + d) * w;
+  for (int s0 = 0; s0 < p.splits; s0 += U) {
+    float mv[U], lv[U];
+    f32x4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t slot = slot0 + min(s0 + u, p.splits - 1) * step;
+      mv[u] = p.part_ml[2 * slot];
+      lv[u] = p.part_ml[2 * slot + 1];
+      o[u] = *reinterpret_cast<const f32x4*>(p.part_o + slot * D + d);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= p.splits || lv[u] == 0.0f) continue;   // no keys of this row: its part was not written
+      const float w = lv[u] * fast_exp2(mv[u] - M);
+      den += w;
+      num += o[u] * w;
+    }
   }
   const f32x4 x = num * (1.0f / den);
   const int pos = row / p.group;
@@ -455,15 +475,19 @@ void launch_of(const PrefillFp8Params& p, hipStream_t stream) {
 }
 
 template <typename T> void launch_dims(const PrefillFp8Params& p, int head_dim, bool wide, hipStream_t stream) {
-  if (head_dim == 64) wide ? launch_of<T, 64, 2, 64, 1>(p, stream) : launch_of<T, 64, 1, 64, 2>(p, stream);
-  else if (head_dim == 128) wide ? launch_of<T, 128, 2, 64, 1>(p, stream) : launch_of<T, 128, 1, 64, 2>(p, stream);
+  if (head_dim == 64) wide ? launch_of<T, 64, 2, 64, 2>(p, stream) : launch_of<T, 64, 1, 64, 4>(p, stream);
+  else if (head_dim == 128) wide ? launch_of<T, 128, 2, 64, 2>(p, stream) : launch_of<T, 128, 1, 32, 4>(p, stream);
   else launch_of<T, 256, 1, 32, 1>(p, stream);
 }
 
-// 128-row work-groups of 4 waves where they give every CU two; else 64 rows and
-// two key groups of 4 waves, one work-group per CU.
+// 128-row work-groups of two key groups (8 waves) where they give nearly every CU
+// one, else 64 rows and four key groups (16 waves).  A CU holds one of either.
+// MI355X, bf16, 32 / 8 heads of 128, us: 1024 rows after 4000 cached ones (256
+// tiles of 128) 92 / 107 (64 rows), with one group of 4 waves 132; 512 after 2000 43
+// / 34; 2048 after 6144 250, with one group 256; 32 / 4 heads of 64, 512 after 3584
+// 38 / 34, with two groups of 64 rows 40.
 bool wide_rows(long long rows, int num_kv_heads, int head_dim, int cus) {
-  return head_dim != 256 && (rows + 127) / 128 * num_kv_heads * 4 >= 7LL * cus;
+  return head_dim != 256 && (rows + 127) / 128 * num_kv_heads * 8 >= 7LL * cus;
 }
 
 }  // namespace
