@@ -163,6 +163,29 @@ def test_ties_masks_and_non_finite_rows(dtype, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_rows_of_the_types_extremes(dtype):
+    """Rows masked with the type's lowest value throughout, partly -inf, and rows of its largest."""
+    x = np.zeros((8, 40000), np.float32)
+    info = torch.finfo(DTYPES[dtype])
+    x[0] = info.min
+    x[1] = info.min
+    x[1, ::3] = -np.inf
+    x[2] = info.max
+    x[3] = info.max
+    x[3, 7:] = -np.inf
+    x[4] = info.min / 2
+    x[4, 3] = info.min / 4
+    big = 30000.0 if dtype == "float16" else 2.0 ** 29
+    for row, top in ((5, big), (6, -big), (7, 1000.0)):        # neighbours of a large maximum
+        x[row] = np.nextafter(np.float32(top), np.float32(-np.inf))
+        x[row, :9] = top
+    tokens = np.array([5, 1, 39999, 6, 3, 100, 8, 9])
+    out, seen = run(x, tokens, 3, dtype)
+    check(out, seen, tokens, 3)
+
+
+@gpu
 def test_certain_tokens_keep_their_digits():
     """log p of a token with nearly all of the probability, and the entropy of its row, are small numbers."""
     x = np.full((6, 5000), -40.0, np.float32)

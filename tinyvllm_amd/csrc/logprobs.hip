@@ -14,10 +14,10 @@
 // 32000 fp32 logits is read once and needs no second launch), so the sums are
 // taken relative to the final maximum.  Longer rows are cut into such segments,
 // and a second kernel joins their (m, s, t) and lists.
-// Top tokens of a segment: each wave takes its k-th largest thread maximum, rounded
-// down to 16 bits, by a search over bits with ballots; the largest of these is a
-// bound that at least k elements reach, few others do, and those that do go to a
-// list in LDS and are ranked by (value, then lowest index).  Where too many reach
+// Top tokens of a segment: from the threads' maxima, rounded down to 16 bits, a
+// search over bits with ballots finds a bound that at least k elements reach and few
+// others do; those that do go to a list in LDS and are ranked by (value, then lowest
+// index).  Where too many reach
 // it (equal logits) or there is a NaN, k passes over the segment take the largest
 // remaining key each.  NaN ranks above every number.
 #include "tv_logprobs.h"
@@ -28,9 +28,10 @@ namespace {
 
 constexpr int kVecs = 8;          // 16-byte vectors a thread
 constexpr int kList = 512;        // candidates of a segment
-// Distances from the maximum are limited to this in t: e^-200 is 0 in fp32, and
-// the distance of a logit of -inf must not be infinite beside it.
-constexpr float kFar = 200.0f;
+// Distances from the maximum are limited to this in t: their exponentials are 0 in
+// fp32, and the distance of a logit of -inf must not be infinite beside it.
+constexpr float kFar = 300.0f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 typedef unsigned long long u64;
 
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
   constexpr int EPV = 16 / (int)sizeof(T);
   constexpr int SEG = NT * kVecs * EPV;
   __shared__ float red[4][NW];
-  __shared__ uint32_t bound[NW];
+  __shared__ uint32_t bound[2][NW];
   __shared__ u64 cand[kList];
   __shared__ u64 best[kLogprobTopMax];
   __shared__ u64 wave_best[NW];
@@ -169,34 +170,42 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
 #pragma unroll 4
   for (int i = 1; i < NW; ++i) m = fmaxf(m, red[0][i]);
 
-  // sums without the maximum's own term: elements equal to m count 1 each, less one for the row
+  // Sums without the maximum's own term: elements equal to m count 1 each, less one
+  // for the row.  In log2 units relative to mh, m log2 e rounded: one fma an element;
+  // what the rounding left, ml, is a factor of the whole sums.
+  // From 2^30 on (a row of the type's lowest numbers, say) another number's term is
+  // below 2^-184, zero in fp32: with mh of 0 for a low m and infinity for a high one
+  // every y is far below or -inf.
+  const bool far = !(fabsf(m) < 0x1p30f);
+  float mh = far ? (m < 0.0f ? 0.0f : __builtin_inff()) : m * kLog2e;
+  const float ml = far ? 0.0f : fmaf(m, kLog2e, -mh);
   float s = 0.0f, t = 0.0f, eq = 0.0f;
   if (tmax < m) {
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
       // a vector at a time (the next one's terms depend on this): registers for two work-groups a CU
-      __asm__ volatile("" : "+v"(m), "+v"(s), "+v"(t), "+v"(w[j]));
+      __asm__ volatile("" : "+v"(mh), "+v"(s), "+v"(t), "+v"(w[j]));
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
-        const float d = m - element<T>(w[j], e);
-        const float q = fast_exp2(d * -kLog2e);
+        const float y = fmaf(element<T>(w[j], e), kLog2e, -mh);
+        const float q = fast_exp2(y);
         s += q;
-        t = fmaf(fminf(d, kFar), q, t);
+        t = fmaf(fmaxf(y, -kFar), q, t);
       }
     }
   } else {
     int equal = 0;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
-      __asm__ volatile("" : "+v"(m), "+v"(s), "+v"(t), "+v"(w[j]));
+      __asm__ volatile("" : "+v"(mh), "+v"(s), "+v"(t), "+v"(w[j]));
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
         const float v = element<T>(w[j], e);
-        const float d = m - v;
-        const float q = fast_exp2(d * -kLog2e);
+        const float y = fmaf(v, kLog2e, -mh);
+        const float q = fast_exp2(y);
         equal += v == m ? 1 : 0;
         s += v == m ? 0.0f : q;
-        t = v == m ? t : fmaf(fminf(d, kFar), q, t);
+        t = v == m ? t : fmaf(fmaxf(y, -kFar), q, t);
       }
     }
     eq = (float)equal;
@@ -211,17 +220,26 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
     red[3][wave] = eq;
   }
 
-  // the wave's bound: the largest b of 16 bits that at least top_k of its threads' maxima reach
+  // Bounds of 16 bits: the largest b that at least `lanes` of the wave's threads reach with their maxima.
+  // At least top_k elements reach every wave's bound for top_k lanes, and the lowest of the waves' bounds
+  // for top_k / NW lanes each, which is the closer one where the waves have much the same.
   const int k = p.top_k;
   if (k > 0) {
     const uint32_t key = order_bits(tmax);
-    uint32_t b = 0;
+    auto reached_by = [&](int lanes) {
+      uint32_t b = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t c = b | 1u << bit;
-      b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= c)) >= k ? c : b;
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t c = b | 1u << bit;
+        b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= c)) >= lanes ? c : b;
+      }
+      return b;
+    };
+    const uint32_t all = reached_by(k), some = reached_by((k + NW - 1) / NW);
+    if (lane == 0) {
+      bound[0][wave] = all;
+      bound[1][wave] = some;
     }
-    if (lane == 0) bound[wave] = b;
   }
   __syncthreads();
   s = red[1][0];
@@ -233,12 +251,19 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
     t += red[2][i];
     eq += red[3][i];
   }
-  s += eq - 1.0f;
+  // t in nats and positive: (m - x) e^(x - m) = -(y - ml) 2^(y - ml) ln 2
+  const float left = fast_exp2(-ml);
+  t = fmaf(ml, s, -t) * left * kLn2;
+  s = fmaf(s, left, eq - 1.0f);
 
   if (k > 0) {
-    uint32_t b = bound[0];
+    uint32_t b = bound[0][0], some = bound[1][0];
 #pragma unroll 4
-    for (int i = 1; i < NW; ++i) b = max(b, bound[i]);
+    for (int i = 1; i < NW; ++i) {
+      b = max(b, bound[0][i]);
+      some = min(some, bound[1][i]);
+    }
+    b = max(b, some);
     const float least = b > order_bits(kNegInf) ? from_order_bits(b) : kNegInf;
     bool slow = s != s;             // a NaN
     if (!slow) {
