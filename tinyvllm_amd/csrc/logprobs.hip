@@ -386,7 +386,9 @@ template <typename T, int NT> void launch_of(const LogprobParams& p, int segs, h
 
 template <typename T> void launch_type(const LogprobParams& p, hipStream_t stream) {
   const int segs = logprob_segments(p.vocab, (int)sizeof(T));
-  if (logprob_small(p.vocab, (int)sizeof(T))) launch_of<T, 256>(p, segs, stream);
+  const int threads = logprob_threads(p.vocab, (int)sizeof(T));
+  if (threads == 256) launch_of<T, 256>(p, segs, stream);
+  else if (threads == 512) launch_of<T, 512>(p, segs, stream);
   else launch_of<T, 1024>(p, segs, stream);
 }
 

@@ -23,11 +23,16 @@ struct LogprobParams {
   float* part;                 // [rows, segments, 3]: maximum, sums without its term
 };
 
-// Rows of at most 32 KiB take a work-group of 256 threads; longer ones are cut
-// into segments of 128 KiB, one of 1024 threads each.
-inline bool logprob_small(int vocab, int elem_bytes) { return (long long)vocab * elem_bytes <= 32768; }
+// Threads of a work-group, each of 128 bytes of a row: 256 for rows of at most 32
+// KiB, 1024 up to 128 KiB (a second launch costs more than the coarser work-groups);
+// longer rows are cut into segments of 64 KiB, 512 threads each.
+inline int logprob_threads(int vocab, int elem_bytes) {
+  const long long bytes = (long long)vocab * elem_bytes;
+  return bytes <= 32768 ? 256 : bytes <= 131072 ? 1024 : 512;
+}
 inline int logprob_segments(int vocab, int elem_bytes) {
-  return (int)(((long long)vocab * elem_bytes + 131071) / 131072);
+  const long long seg = 128LL * logprob_threads(vocab, elem_bytes);
+  return (int)(((long long)vocab * elem_bytes + seg - 1) / seg);
 }
 
 void launch_logprobs(const LogprobParams& p, int dtype, hipStream_t stream);
