@@ -91,8 +91,9 @@ __device__ __forceinline__ void finish_row(const LogprobParams& p, int row, floa
   }
 }
 
-template <typename T, int NT, bool ALIGNED>
-__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) logprobs_kernel(const LogprobParams p) {
+// ALIGNED: rows start at multiples of 16 bytes.  TOP: top_k > 0 (its code costs the sums registers).
+template <typename T, int NT, bool ALIGNED, bool TOP>
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP && NT < 1024 ? 6 : 8))) logprobs_kernel(const LogprobParams p) {
   constexpr int NW = NT / 64;
   constexpr int EPV = 16 / (int)sizeof(T);
   constexpr int SEG = NT * kVecs * EPV;
@@ -165,10 +166,59 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
   again();
   float m = group_max<64>(tmax);
   if (lane == 0) red[0][wave] = m;
+  // Bounds of 16 bits: the largest b that at least `lanes` of the wave's threads reach with their maxima.
+  // At least top_k elements reach every wave's bound for top_k lanes, and the lowest of the waves' bounds
+  // for top_k / NW lanes each, which is the closer one where the waves have much the same.
+  const int k = TOP ? p.top_k : 0;
+  if constexpr (TOP) {
+    const uint32_t key = order_bits(tmax);
+    auto reached_by = [&](int lanes) {
+      uint32_t b = 0;
+#pragma unroll
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t c = b | 1u << bit;
+        b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= c)) >= lanes ? c : b;
+      }
+      return b;
+    };
+    const uint32_t all = reached_by(k), some = reached_by((k + NW - 1) / NW);
+    if (lane == 0) {
+      bound[0][wave] = all;
+      bound[1][wave] = some;
+    }
+  }
   __syncthreads();
   m = red[0][0];
 #pragma unroll 4
   for (int i = 1; i < NW; ++i) m = fmaxf(m, red[0][i]);
+
+  if constexpr (TOP) {
+    // what reaches the bound, before the sums: the vectors that hold some are read again, from cache
+    uint32_t b = bound[0][0], some = bound[1][0];
+#pragma unroll 4
+    for (int i = 1; i < NW; ++i) {
+      b = max(b, bound[0][i]);
+      some = min(some, bound[1][i]);
+    }
+    b = max(b, some);
+    const float least = b > order_bits(kNegInf) ? from_order_bits(b) : kNegInf;
+    uint32_t vecs = 0;
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) vecs |= vmax[j] >= least && index_of(j) < p.vocab ? 1u << j : 0u;
+    while (vecs) {
+      const int at = index_of(__builtin_ctz(vecs));
+      vecs &= vecs - 1;
+      const u32x4 held = ALIGNED && at + EPV <= p.vocab ? *reinterpret_cast<const u32x4*>(x + at) : by_elements(at);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) {
+        const float v = element<T>(held, e);
+        if (v >= least && at + e < p.vocab) {
+          const int to = atomicAdd(&count, 1);
+          if (to < kList) cand[to] = make_key(v, at + e);
+        }
+      }
+    }
+  }
 
   // Sums without the maximum's own term: elements equal to m count 1 each, less one
   // for the row.  In log2 units relative to mh, m log2 e rounded: one fma an element;
@@ -220,27 +270,6 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
     red[3][wave] = eq;
   }
 
-  // Bounds of 16 bits: the largest b that at least `lanes` of the wave's threads reach with their maxima.
-  // At least top_k elements reach every wave's bound for top_k lanes, and the lowest of the waves' bounds
-  // for top_k / NW lanes each, which is the closer one where the waves have much the same.
-  const int k = p.top_k;
-  if (k > 0) {
-    const uint32_t key = order_bits(tmax);
-    auto reached_by = [&](int lanes) {
-      uint32_t b = 0;
-#pragma unroll
-      for (int bit = 31; bit >= 16; --bit) {
-        const uint32_t c = b | 1u << bit;
-        b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= c)) >= lanes ? c : b;
-      }
-      return b;
-    };
-    const uint32_t all = reached_by(k), some = reached_by((k + NW - 1) / NW);
-    if (lane == 0) {
-      bound[0][wave] = all;
-      bound[1][wave] = some;
-    }
-  }
   __syncthreads();
   s = red[1][0];
   t = red[2][0];
@@ -256,35 +285,8 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) lo
   t = fmaf(ml, s, -t) * left * kLn2;
   s = fmaf(s, left, eq - 1.0f);
 
-  if (k > 0) {
-    uint32_t b = bound[0][0], some = bound[1][0];
-#pragma unroll 4
-    for (int i = 1; i < NW; ++i) {
-      b = max(b, bound[0][i]);
-      some = min(some, bound[1][i]);
-    }
-    b = max(b, some);
-    const float least = b > order_bits(kNegInf) ? from_order_bits(b) : kNegInf;
-    bool slow = s != s;             // a NaN
-    if (!slow) {
-      uint32_t vecs = 0;            // vectors that hold one; their elements are read again, from cache
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j) vecs |= vmax[j] >= least ? 1u << j : 0u;
-      while (vecs) {
-        const int at = index_of(__builtin_ctz(vecs));
-        vecs &= vecs - 1;
-        const int end = min(at + EPV, p.vocab);
-        for (int o = at; o < end; ++o) {
-          const float v = to_float<T>(x[o]);
-          if (v >= least) {
-            const int to = atomicAdd(&count, 1);
-            if (to < kList) cand[to] = make_key(v, o);
-          }
-        }
-      }
-      __syncthreads();
-      slow = count > kList;
-    }
+  if constexpr (TOP) {
+    const bool slow = s != s || count > kList;      // a NaN, or too many equal logits
     if (!slow) {
       const int n = count;
       for (int i = tid; i < n; i += NT) {
@@ -378,9 +380,15 @@ __global__ void __launch_bounds__(256) logprobs_merge_kernel(const LogprobParams
   finish_row<T>(p, row, M, s, t, best, tid, 256);
 }
 
+template <typename T, int NT, bool ALIGNED> void launch_rows(const LogprobParams& p, int segs, hipStream_t stream) {
+  const dim3 grid(p.rows, segs);
+  if (p.top_k > 0) hipLaunchKernelGGL((logprobs_kernel<T, NT, ALIGNED, true>), grid, dim3(NT), 0, stream, p);
+  else hipLaunchKernelGGL((logprobs_kernel<T, NT, ALIGNED, false>), grid, dim3(NT), 0, stream, p);
+}
+
 template <typename T, int NT> void launch_of(const LogprobParams& p, int segs, hipStream_t stream) {
-  if (p.aligned) hipLaunchKernelGGL((logprobs_kernel<T, NT, true>), dim3(p.rows, segs), dim3(NT), 0, stream, p);
-  else hipLaunchKernelGGL((logprobs_kernel<T, NT, false>), dim3(p.rows, segs), dim3(NT), 0, stream, p);
+  if (p.aligned) launch_rows<T, NT, true>(p, segs, stream);
+  else launch_rows<T, NT, false>(p, segs, stream);
   if (segs > 1) hipLaunchKernelGGL(logprobs_merge_kernel<T>, dim3(p.rows), dim3(256), 0, stream, p, segs);
 }
 
