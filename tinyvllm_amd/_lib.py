@@ -5,6 +5,7 @@ there is no CPU or PyTorch fallback for any op.
 """
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -127,3 +128,24 @@ def stream_ptr(device):
     import torch
     index = device.index if device.index is not None else torch.cuda.current_device()
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
+
+
+def call(what, index, fn, *args):
+    """``fn(*args, stream)`` with device ``index`` current and its current stream; raises on a non-zero
+    status.  (The library launches on, and sizes grids for, the current device.)"""
+    import torch
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != TV_OK:
+        check(rc, what)
+
+
+@functools.lru_cache(maxsize=4096)
+def device_size(name, index, *args):
+    """The result of a size function of the library (a pure function of its numbers and the device)."""
+    import torch
+    with torch.cuda.device(index):
+        return getattr(load(), name)(*args)

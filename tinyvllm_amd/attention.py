@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .kv_cache import check_fp8_cache
+from .kv_cache import check_devices, check_fp8_cache
 
 _lib.load()
 
@@ -289,36 +289,35 @@ class PagedDecodeFP8Plan:
     def __init__(self, queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
                  n_heads, n_kv_heads, head_dim, block_size, max_context_len=None,
                  *, partition_size=None, out_dtype=None):
-        self.lib = _lib.load()
-        self.dev = _on_gpu(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
-        nb, hkv, bs, d = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
-        _require(queries.dim() == 4 and queries.shape[1] == 1,
-                 f"queries must be [B,1,Hq,D], got {tuple(queries.shape)}")
+        nb, hkv, bs, d, index = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+        _require(index >= 0, "tensors must live on a HIP device")
+        check_devices(index, queries, block_tables, context_lens)
+        self.index = index
         b = queries.shape[0]
-        _require(tuple(queries.shape) == (b, 1, n_heads, head_dim), "queries shape does not match n_heads/head_dim")
+        _require(tuple(queries.shape) == (b, 1, n_heads, head_dim), "queries must be [B, 1, n_heads, head_dim]")
         _require((hkv, bs, d) == (n_kv_heads, block_size, head_dim),
-                 f"cache shape {tuple(k_cache.shape)} does not match n_kv_heads/block_size/head_dim")
+                 "cache shape does not match n_kv_heads/block_size/head_dim")
         _require(n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
         _require(block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32,
                  "block_tables and context_lens must be int32")
         _require(block_tables.dim() == 2 and block_tables.shape[0] == b, "block_tables must be [B, max_blocks]")
         _require(context_lens.numel() == b, "context_lens must have B entries")
-        for t in (queries, block_tables, context_lens):
-            _require(t.is_contiguous(), "all inputs must be contiguous")
+        _require(queries.is_contiguous() and block_tables.is_contiguous() and context_lens.is_contiguous(),
+                 "all inputs must be contiguous")
         mb = block_tables.shape[1]
         used = mb if max_context_len is None else min((int(max_context_len) + block_size - 1) // block_size, mb)
         _require(used > 0, "no block table columns to attend over")
         code = _lib.dtype_code(queries.dtype)
         if partition_size is None:
-            partition_size = self.lib.tv_paged_decode_fp8_partition_size(b, n_heads, n_kv_heads, head_dim, used,
-                                                                         block_size, code)
-            _lib.check(0 if partition_size > 0 else _lib.TV_EINVAL, "paged_decode_attention_fp8")
+            partition_size = _lib.device_size("tv_paged_decode_fp8_partition_size", index, b, n_heads, n_kv_heads,
+                                              head_dim, used, block_size, code)
+            _require(partition_size > 0, "no partition size for this shape")
         self.partition_size = int(partition_size)
         out_dtype = queries.dtype if out_dtype is None else out_dtype
-        self.out = torch.empty((b, 1, n_heads, head_dim), dtype=out_dtype, device=self.dev)
-        self.ws_bytes = self.lib.tv_paged_decode_fp8_workspace_bytes(b, n_heads, head_dim, used, block_size,
-                                                                     self.partition_size)
-        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.dev) if self.ws_bytes else None
+        self.out = torch.empty((b, 1, n_heads, head_dim), dtype=out_dtype, device=queries.device)
+        self.ws_bytes = _lib.device_size("tv_paged_decode_fp8_workspace_bytes", index, b, n_heads, head_dim, used,
+                                         block_size, self.partition_size)
+        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=queries.device) if self.ws_bytes else None
         self._inputs = (queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens)
         self.args = (self.out.data_ptr(), queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                      k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(),
@@ -327,7 +326,7 @@ class PagedDecodeFP8Plan:
                      self.ws.data_ptr() if self.ws is not None else None, self.ws_bytes)
 
     def run(self):
-        _lib.check(self.lib.tv_paged_decode_fp8(*self.args, _lib.stream_ptr(self.dev)), "PagedDecodeFP8Plan.run")
+        _lib.call("PagedDecodeFP8Plan.run", self.index, _lib.load().tv_paged_decode_fp8, *self.args)
         return self.out
 
 
@@ -350,30 +349,30 @@ def flash_prefill_paged_fp8(queries, k_cache, v_cache, k_scale, v_scale, block_t
     reference counterpart): the chunk's rows attend the cached keys and the chunk's own, all as the
     cache holds them.  fp16 / bf16 queries [1, n, Hq, D] or [n, Hq, D], head_dim 64, 128 or 256, any
     block size.  Returns [1, n, Hq, D]."""
-    lib = _lib.load()
-    dev = _on_gpu(queries, k_cache, v_cache, k_scale, v_scale, block_table)
-    nb, hkv, bs, d2 = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    nb, hkv, bs, d2, index = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    _require(index >= 0, "tensors must live on a HIP device")
+    check_devices(index, queries, block_table)
     _require(queries.dim() in (3, 4) and (queries.dim() == 3 or queries.shape[0] == 1),
              "queries must be [1, n, Hq, D] or [n, Hq, D]")
-    q = queries[0] if queries.dim() == 4 else queries
-    _require(q.stride(2) == 1 and q.stride(1) == q.shape[2], "queries: heads and head_dim must be contiguous")
-    n, hq, d = q.shape
+    n, hq, d = queries.shape[-3:]
+    stride = queries.stride()
+    _require(stride[-1] == 1 and stride[-2] == d, "queries: heads and head_dim must be contiguous")
     _require(d == d2, "cache shape does not match the queries")
     _require(hq % hkv == 0, "query heads must be a multiple of KV heads")
     _require(block_table.dtype == torch.int32 and block_table.is_contiguous(), "block_table must be contiguous int32")
     start_pos = int(start_pos)
     _require(start_pos >= 0 and n > 0, "start_pos must be >= 0 and the chunk non-empty")
     _require(block_table.numel() * bs >= start_pos + n, "block_table does not cover the sequence")
-    out_dtype = q.dtype if out_dtype is None else out_dtype
-    out = torch.empty((1, n, hq, d), dtype=out_dtype, device=dev)
-    ws_bytes = lib.tv_flash_prefill_paged_fp8_workspace_bytes(n, start_pos, hq, hkv, d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    rc = lib.tv_flash_prefill_paged_fp8(
-        out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        block_table.data_ptr(), nb, bs, n, start_pos, hq, hkv, d, q.stride(0) if n > 1 else hq * d, hq * d,
-        1 if causal else 0, 1.0 / math.sqrt(d), _lib.dtype_code(q.dtype), _lib.dtype_code(out_dtype),
-        ws.data_ptr() if ws is not None else None, ws_bytes, _lib.stream_ptr(dev))
-    _lib.check(rc, "flash_prefill_paged_fp8")
+    out_dtype = queries.dtype if out_dtype is None else out_dtype
+    out = torch.empty((1, n, hq, d), dtype=out_dtype, device=queries.device)
+    ws_bytes = _lib.device_size("tv_flash_prefill_paged_fp8_workspace_bytes", index, n, start_pos, hq, hkv, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=queries.device) if ws_bytes else None
+    _lib.call("flash_prefill_paged_fp8", index, _lib.load().tv_flash_prefill_paged_fp8,
+              out.data_ptr(), queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+              v_scale.data_ptr(), block_table.data_ptr(), nb, bs, n, start_pos, hq, hkv, d,
+              stride[-3] if n > 1 else hq * d, hq * d, 1 if causal else 0, 1.0 / math.sqrt(d),
+              _lib.dtype_code(queries.dtype), _lib.dtype_code(out_dtype), ws.data_ptr() if ws is not None else None,
+              ws_bytes)
     return out
 
 

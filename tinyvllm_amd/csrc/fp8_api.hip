@@ -77,11 +77,14 @@ int write_common(const char* who, void* k_cache, void* v_cache, float* k_scale, 
 constexpr int kOrderMinSeqs = 32;
 constexpr int kOrderMaxSeqs = 1024;
 
+// Compute units of the current device, asked for once per device.
 int device_cus() {
+  static std::atomic<int> known[tv::kMaxDevices];
   int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-    return 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
+  if (dev < tv::kMaxDevices && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+  if (dev < tv::kMaxDevices) known[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
 

@@ -165,13 +165,12 @@ class FP8KVCache:
         v, vs = self._rows(v, "v")
         if k.shape[0] != v.shape[0]:
             raise ValueError("k and v must hold the same number of tokens")
-        lib = _lib.load()
-        rc = lib.tv_write_kv_fp8(
-            self.k_cache[layer_idx].data_ptr(), self.v_cache[layer_idx].data_ptr(),
-            self.k_scale[layer_idx].data_ptr(), self.v_scale[layer_idx].data_ptr(), k.data_ptr(), v.data_ptr(),
-            int(block_id), int(start_offset), k.shape[0], self.n_kv_heads, self.head_dim, self.block_size,
-            self.num_blocks, ks, vs, _lib.dtype_code(self.dtype), _lib.stream_ptr(self.k_cache[layer_idx].device))
-        _lib.check(rc, "FP8KVCache.write_kv")
+        kc = self.k_cache[layer_idx]
+        _lib.call("FP8KVCache.write_kv", kc.get_device(), _lib.load().tv_write_kv_fp8,
+                  kc.data_ptr(), self.v_cache[layer_idx].data_ptr(), self.k_scale[layer_idx].data_ptr(),
+                  self.v_scale[layer_idx].data_ptr(), k.data_ptr(), v.data_ptr(), int(block_id), int(start_offset),
+                  k.shape[0], self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, ks, vs,
+                  _lib.dtype_code(self.dtype))
 
     def write_kv_slots(self, layer_idx, slot_mapping, k, v, err_count=None):
         """Write token t of k/v [T, Hkv, D] to flat slot ``slot_mapping[t]`` (int32 device tensor) in one
@@ -185,7 +184,8 @@ class FP8KVCache:
         on the device, which is read without a host copy) as values."""
         kc = self.k_cache[layer_idx]
         if isinstance(block_ids, torch.Tensor):
-            if block_ids.dtype != torch.int32 or block_ids.device != kc.device or not block_ids.is_contiguous():
+            if block_ids.dtype != torch.int32 or block_ids.get_device() != kc.get_device() or \
+                    not block_ids.is_contiguous():
                 raise ValueError("block_ids must be a contiguous int32 tensor on the cache's device")
             count = block_ids.numel()
         else:
@@ -199,13 +199,10 @@ class FP8KVCache:
             return k_out, v_out
         ids = block_ids if isinstance(block_ids, torch.Tensor) else \
             torch.tensor(list(block_ids), dtype=torch.int32).to(kc.device)
-        lib = _lib.load()
-        rc = lib.tv_read_kv_blocks_fp8(
-            k_out.data_ptr(), v_out.data_ptr(), kc.data_ptr(), self.v_cache[layer_idx].data_ptr(),
-            self.k_scale[layer_idx].data_ptr(), self.v_scale[layer_idx].data_ptr(), ids.data_ptr(), count, n,
-            self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, _lib.dtype_code(self.dtype),
-            _lib.stream_ptr(kc.device))
-        _lib.check(rc, "FP8KVCache.read_kv_blocks")
+        _lib.call("FP8KVCache.read_kv_blocks", kc.get_device(), _lib.load().tv_read_kv_blocks_fp8,
+                  k_out.data_ptr(), v_out.data_ptr(), kc.data_ptr(), self.v_cache[layer_idx].data_ptr(),
+                  self.k_scale[layer_idx].data_ptr(), self.v_scale[layer_idx].data_ptr(), ids.data_ptr(), count, n,
+                  self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, _lib.dtype_code(self.dtype))
         return k_out, v_out
 
     def get_memory_bytes(self):
@@ -214,46 +211,51 @@ class FP8KVCache:
 
 
 def check_fp8_cache(k_cache, v_cache, k_scale, v_scale):
-    """Shape [NB, Hkv, bs, D] of the tensors of one layer's 8-bit cache; raises ValueError."""
-    if k_cache.dim() != 4 or tuple(v_cache.shape) != tuple(k_cache.shape) or \
-            not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    """Shape [NB, Hkv, bs, D] and device index of one layer's 8-bit cache; raises ValueError."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache / v_cache must be dense [NB, Hkv, bs, D] tensors of one shape")
     if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
         raise ValueError("k_cache / v_cache must be float8_e4m3fn")
-    nb, hkv, bs, d = k_cache.shape
     for t in (k_scale, v_scale):
-        if t.dtype != torch.float32 or tuple(t.shape) != (nb, hkv) or not t.is_contiguous():
-            raise ValueError(f"k_scale / v_scale must be dense float32 [{nb}, {hkv}]")
-    for t in (v_cache, k_scale, v_scale):
-        if t.device != k_cache.device:
+        if t.dtype != torch.float32 or t.shape != shape[:2] or not t.is_contiguous():
+            raise ValueError(f"k_scale / v_scale must be dense float32 [{shape[0]}, {shape[1]}]")
+    index = k_cache.get_device()
+    check_devices(index, v_cache, k_scale, v_scale)
+    return (*shape, index)
+
+
+def check_devices(index, *tensors):
+    """Raises ValueError for a tensor that is not on device ``index`` (-1: the CPU)."""
+    for t in tensors:
+        if t.get_device() != index:
             raise ValueError("all tensors must be on the cache's device")
-    return nb, hkv, bs, d
 
 
 def reshape_and_cache_fp8(k_cache, v_cache, k_scale, v_scale, k, v, slot_mapping, err_count=None):
     """``reshape_and_cache`` into an 8-bit cache (one layer's tensors of ``FP8KVCache``)."""
-    nb, hkv, bs, d = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
-    if k.dim() != 3 or tuple(k.shape[1:]) != (hkv, d) or tuple(v.shape) != tuple(k.shape):
+    nb, hkv, bs, d, index = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    if k.dim() != 3 or k.shape[1] != hkv or k.shape[2] != d or v.shape != k.shape:
         raise ValueError(f"k/v must be [T, {hkv}, {d}]")
-    if not (k.stride(2) == 1 and k.stride(1) == d and v.stride(2) == 1 and v.stride(1) == d):
+    t = k.shape[0]
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or ks[1] != d or vs[2] != 1 or vs[1] != d:
         raise ValueError("k/v heads and head_dim must be contiguous")
     if k.dtype != v.dtype:
         raise ValueError("k and v must share a dtype")
-    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != k.shape[0] or not slot_mapping.is_contiguous():
+    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != t or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be contiguous int32 with one entry per token")
-    dev = k_cache.device
-    for t in (k, v, slot_mapping):
-        if t.device != dev:
-            raise ValueError("all tensors must be on the cache's device")
-    if err_count is not None and (err_count.device != dev or err_count.dtype not in (torch.int32, torch.uint32)):
+    check_devices(index, k, v, slot_mapping)
+    if index < 0:
+        raise ValueError("the cache must be on a HIP device")
+    if err_count is not None and (err_count.get_device() != index or
+                                  err_count.dtype not in (torch.int32, torch.uint32)):
         raise ValueError("err_count must be an int32/uint32 tensor on the cache's device")
-    t = k.shape[0]
-    rc = _lib.load().tv_reshape_and_cache_fp8(
-        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(),
-        slot_mapping.data_ptr(), t, hkv, d, bs, nb, k.stride(0) if t > 1 else hkv * d,
-        v.stride(0) if t > 1 else hkv * d, _lib.dtype_code(k.dtype),
-        err_count.data_ptr() if err_count is not None else None, _lib.stream_ptr(dev))
-    _lib.check(rc, "reshape_and_cache_fp8")
+    _lib.call("reshape_and_cache_fp8", index, _lib.load().tv_reshape_and_cache_fp8,
+              k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(),
+              v.data_ptr(), slot_mapping.data_ptr(), t, hkv, d, bs, nb, ks[0] if t > 1 else hkv * d,
+              vs[0] if t > 1 else hkv * d, _lib.dtype_code(k.dtype),
+              err_count.data_ptr() if err_count is not None else None)
 
 
 def reshape_and_cache(k_cache, v_cache, k, v, slot_mapping, err_count=None):

@@ -30,11 +30,12 @@ def token_logprobs(logits, tokens, top_k=0):
     contiguous.  A logit of -inf has probability 0; a token outside the vocabulary (padding) gives NaN; a
     row with a NaN, with +inf or without a finite logit gives NaN, and its ``top_ids`` rank NaN first.
     """
-    lib = _lib.load()
-    if logits.device.type != "cuda" or tokens.device != logits.device:
+    index = logits.get_device()
+    if index < 0 or tokens.get_device() != index:
         raise ValueError(f"logits and tokens must be on one HIP device (got {logits.device}, {tokens.device})")
-    if logits.dim() < 1 or tuple(tokens.shape) != tuple(logits.shape[:-1]):
-        raise ValueError(f"tokens must be {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
+    shape = logits.shape[:-1]
+    if logits.dim() < 1 or tokens.shape != shape:
+        raise ValueError(f"tokens must be {tuple(shape)}, got {tuple(tokens.shape)}")
     if tokens.dtype != torch.int32:
         raise ValueError("tokens must be int32")
     v = logits.shape[-1]
@@ -44,22 +45,22 @@ def token_logprobs(logits, tokens, top_k=0):
     code = _lib.dtype_code(logits.dtype)
     if logits.stride(-1) != 1 and v > 1:
         raise ValueError("the vocabulary must be contiguous")
-    shape = tuple(tokens.shape)
-    try:
-        rows = logits.view(-1, v)
-    except RuntimeError:
-        raise ValueError("the rows of logits must be evenly spaced") from None
+    rows = logits
+    if logits.dim() != 2:
+        try:
+            rows = logits.view(-1, v)
+        except RuntimeError:
+            raise ValueError("the rows of logits must be evenly spaced") from None
     m = rows.shape[0]
     dev = logits.device
-    tokens = tokens.reshape(-1).contiguous()
+    flat = tokens.reshape(-1).contiguous()
     lp = torch.empty(shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(lp)
     ids = torch.empty((*shape, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((*shape, top_k), dtype=torch.float32, device=dev)
-    need = lib.tv_token_logprobs_workspace_bytes(m, v, top_k, code)
+    top = torch.empty_like(ids, dtype=torch.float32)
+    need = _lib.device_size("tv_token_logprobs_workspace_bytes", index, m, v, top_k, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _lib.check(lib.tv_token_logprobs(
-        lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top.data_ptr(), rows.data_ptr(), tokens.data_ptr(), m, v,
-        rows.stride(0) if m > 1 else v, top_k, code, ws.data_ptr() if ws is not None else None, need,
-        _lib.stream_ptr(dev)), "token_logprobs")
+    _lib.call("token_logprobs", index, _lib.load().tv_token_logprobs,
+              lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top.data_ptr(), rows.data_ptr(), flat.data_ptr(), m,
+              v, rows.stride(0) if m > 1 else v, top_k, code, ws.data_ptr() if ws is not None else None, need)
     return TokenLogprobs(lp, entropy, ids, top)
