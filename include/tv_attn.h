@@ -232,11 +232,13 @@ int tv_read_kv_blocks(void* k_out, void* v_out, const void* k_cache, const void*
  * No counterpart in the reference, whose caches hold the model dtype.
  * k_cache / v_cache hold e4m3 numbers [num_blocks, num_kv_heads, block_size,
  * head_dim] (the rows of a block and head contiguous), k_scale / v_scale float
- * [num_blocks, num_kv_heads] powers of two; an element stands for number *
- * scale.  A scale below 2^-100 (a zeroed one) counts as 2^-100, and of any other
- * positive number only the power of two counts.  dtype is that of the rows
- * written, of the queries and of the values read back.  head_dim 64, 128 or 256,
- * block_size at most 1024 (TV_EUNSUPPORTED otherwise).
+ * [num_blocks, num_kv_heads] powers of two of at least 2^-100 (the value of a
+ * block that was never written; the entry points below keep them so); an element
+ * stands for number * scale.  dtype is that of the rows written, of the queries
+ * and of the values read back, and need not be the same in every call.  TV_F16
+ * values and outputs are limited to +-65504, which a value's rounding to e4m3 can
+ * pass.  head_dim 64, 128 or 256, block_size at most 1024 (TV_EUNSUPPORTED
+ * otherwise).
  */
 
 /*
@@ -264,7 +266,7 @@ int tv_write_kv_fp8(void* k_cache, void* v_cache, float* k_scale, float* v_scale
 /*
  * tv_read_kv_blocks for the 8-bit cache: the first context_len rows of the listed
  * blocks as values, k_out / v_out [context_len, num_kv_heads, head_dim] of dtype
- * (16-byte aligned; TV_F16 limits values to +-65504).
+ * (16-byte aligned).
  */
 int tv_read_kv_blocks_fp8(void* k_out, void* v_out, const void* k_cache, const void* v_cache, const float* k_scale,
                           const float* v_scale, const int32_t* block_ids, int num_block_ids, int context_len,

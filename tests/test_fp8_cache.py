@@ -265,6 +265,100 @@ def test_python_refusals_need_no_gpu():
             reshape_and_cache_fp8(*args)
 
 
+@gpu
+def test_values_near_fp16s_largest_give_finite_outputs():
+    """65504 is held as 65536; an average of such values is limited to 65504, split or not."""
+    hq, hkv, d, bs = 4, 2, 64, 16
+    cache = make_cache(6, bs, hkv, d, "float16")
+    tables = np.arange(6, dtype=np.int32)[None]
+    k = torch.zeros((90, hkv, d), device="cuda", dtype=torch.float16)
+    v = torch.full_like(k, 65504.0)
+    v[:, 1] = -65504.0
+    cache.write_kv_slots(0, torch.arange(90, dtype=torch.int32, device="cuda"), k, v)
+    q = torch.zeros((1, 1, hq, d), device="cuda", dtype=torch.float16)
+    for part in (None, 32):
+        got = run_decode(cache, q, tables, np.array([90], np.int32), hq, hkv, d, bs, partition_size=part)
+        assert torch.equal(got[0, 0, :2], torch.full_like(got[0, 0, :2], 65504.0))
+        assert torch.equal(got[0, 0, 2:], torch.full_like(got[0, 0, 2:], -65504.0))
+        wide = run_decode(cache, q, tables, np.array([90], np.int32), hq, hkv, d, bs, partition_size=part,
+                          out_dtype=torch.float32)
+        assert torch.equal(wide[0, 0, 0], torch.full_like(wide[0, 0, 0], 65536.0))
+
+
+@gpu
+def test_padded_rows_of_a_batch_write_and_read_nothing():
+    """Slots of -1 and contexts of 0, as a fixed-size batch with absent sequences has them."""
+    rng = rng_of(30)
+    hq, hkv, d, bs = 8, 2, 64, 16
+    cache, held, q, tables, ctx = decode_case(rng, [33, 20], hq, hkv, d, bs, "bfloat16")
+    k, v = (torch.from_numpy(rng.standard_normal((4, hkv, d))).to("cuda", torch.bfloat16) for _ in range(2))
+    slots = [-1, int(tables[0, 32 // bs]) * bs + 32 % bs, -1, -1]
+    cache.write_kv_slots(0, torch.tensor(slots, dtype=torch.int32, device="cuda"), k, v)
+    check_write(cache, held, k, v, slots)
+    padded = np.zeros((4, tables.shape[1]), np.int32)
+    padded[1:3] = tables
+    got = run_decode(cache, torch.cat([q[:1], q, q[:1]]), padded, np.array([0, 33, 20, 0], np.int32), hq, hkv, d, bs)
+    assert torch.count_nonzero(got[0]) == 0 and torch.count_nonzero(got[3]) == 0
+    check_decode(got[1:3], held, q, tables, ctx, d, "bfloat16")
+
+
+@gpu
+def test_writes_of_two_streams_to_different_blocks():
+    rng = rng_of(33)
+    hkv, d, bs = 4, 128, 16
+    cache = make_cache(80, bs, hkv, d, "float16")
+    held = fill(cache, rng)
+    parts = []
+    for i in range(2):
+        t = 600
+        slots = (np.arange(t) + i * 640).astype(np.int32)
+        k, v = (torch.from_numpy(rng.standard_normal((t, hkv, d))).to("cuda", torch.float16) for _ in range(2))
+        parts.append((torch.from_numpy(slots).cuda(), k, v, slots))
+    streams = [torch.cuda.Stream() for _ in parts]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, (slots, k, v, _) in zip(streams, parts):
+            with torch.cuda.stream(s):
+                cache.write_kv_slots(0, slots, k, v)
+    torch.cuda.synchronize()
+    check_write(cache, held, torch.cat([p[1] for p in parts]), torch.cat([p[2] for p in parts]),
+                np.concatenate([p[3] for p in parts]))
+
+
+@gpu
+def test_decode_over_a_cache_past_32_bit_offsets():
+    """Blocks that lie more than 4 GiB into the cache's storage."""
+    hq, hkv, d, bs = 4, 2, 128, 16
+    nb = (9 << 29) // (hkv * bs * d)                      # 4.5 GiB each of K and V
+    cache = make_cache(nb, bs, hkv, d, "bfloat16")
+    rng = rng_of(34)
+    blocks = np.array([nb - 1, 3, nb - 20000, nb // 2], np.int32)
+    pos = np.arange(50)
+    slots = torch.from_numpy((blocks[pos // bs].astype(np.int64) * bs + pos % bs).astype(np.int32)).cuda()
+    k, v = (torch.from_numpy(rng.standard_normal((50, hkv, d))).to("cuda", torch.bfloat16) for _ in range(2))
+    cache.write_kv_slots(0, slots, k, v)
+    ids = torch.from_numpy(blocks.astype(np.int64)).cuda()
+    held = []
+    for c, s in ((cache.k_cache[0], cache.k_scale[0]), (cache.v_cache[0], cache.v_scale[0])):
+        held.append((numbers(c[ids]), s[ids].double().cpu().numpy()))
+    small = (held[0][0], held[1][0], held[0][1], held[1][1])
+    written = [np.zeros_like(small[0]), np.full((4, hkv), ref.SCALE_MIN)]
+    ref.write_ref(*written, k.double().cpu().numpy(), pos)
+    assert np.array_equal(written[0], small[0]) and np.array_equal(written[1], small[2])
+    q = torch.from_numpy(rng.standard_normal((1, 1, hq, d))).to("cuda", torch.bfloat16)
+    ctx = np.array([50], np.int32)
+    got = run_decode(cache, q, blocks[None], ctx, hq, hkv, d, bs)
+    check_decode(got, small, q, np.arange(4, dtype=np.int32)[None], ctx, d, "bfloat16")
+    got = cache.read_kv_blocks(0, blocks.tolist(), 50)
+    assert np.array_equal(got[1].double().cpu().numpy(), ref.rows_ref(small[1], small[3], np.arange(4), 50))
+    from tinyvllm_amd.attention import flash_prefill_paged_fp8
+    chunk = flash_prefill_paged_fp8(q, cache.k_cache[0], cache.v_cache[0], cache.k_scale[0], cache.v_scale[0],
+                                    torch.from_numpy(blocks).cuda(), 49)
+    want = ref.attend_ref(q[0].double().cpu().numpy(), ref.rows_ref(small[0], small[2], np.arange(4), 50),
+                          ref.rows_ref(small[1], small[3], np.arange(4), 50), 49, 1 / math.sqrt(d))[0]
+    assert np.abs(chunk[0].double().cpu().numpy() - want).max() <= 2.0 ** -6 * np.abs(small[1] * small[3][..., None, None]).max()
+
+
 # ---- attention of single tokens ------------------------------------------------------------
 
 def decode_case(rng, ctx, hq, hkv, d, bs, dtype, spread=1.0, extra_cols=0):

@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(64 * NW) paged_decode_fp8_kernel(const DecodeF
     }
     const size_t row = row0 + n;
     if (nparts == 1) {
-      store_as(p.out, row * D + d, any_bad ? __builtin_nanf("") : O / L, p.out_dtype);
+      store_limited(p.out, row * D + d, any_bad ? __builtin_nanf("") : O / L, p.out_dtype);
     } else {
       const size_t slot = row * p.max_parts + part;
       p.part_o[slot * D + d] = O / L;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(NT) paged_decode_fp8_merge_kernel(const Decode
       den += sden[tid + k * D];
     }
   }
-  store_as(p.out, row * D + d, nan ? __builtin_nanf("") : num / den, p.out_dtype);
+  store_limited(p.out, row * D + d, nan ? __builtin_nanf("") : num / den, p.out_dtype);
 }
 
 // Few partitions want few threads (64 heads' worth of 4: 13.9 against 15.8 us for a

@@ -66,6 +66,13 @@ template <typename T, bool HI> __device__ __forceinline__ uint32_t fp8_to_pair(u
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 
+// An output that averages cached values.  Rounding to e4m3 can lift a value near
+// fp16's largest past it (65504 becomes 65536), so fp16 outputs are limited to it.
+__device__ __forceinline__ void store_limited(void* base, size_t idx, float v, int dtype) {
+  if (dtype == kF16 && fabsf(v) > 65504.0f) v = __builtin_copysignf(65504.0f, v);
+  store_as(base, idx, v, dtype);
+}
+
 // 8-bit cache write and gather (kv_cache_fp8.hip).
 struct KVWriteFp8Params {
   uint8_t* k_cache;
