@@ -223,7 +223,11 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
                                                           partition_size);
   if (max_parts > 1 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
     return fail(TV_EINVAL, "%s: workspace of %zu bytes required (got %zu)", who, need, workspace_bytes);
-  // longest first only where work-groups wait for others to end (two are resident per CU)
+  // Longest first, at the cost of a launch, where work-groups wait for others to end
+  // (two are resident per CU).  MI355X, us, lengths from a quarter up, with / without:
+  // 32 / 8 heads of 128: 128 sequences to 4096 tokens 113 / 132, 256 230 / 247, 512 to
+  // 1152 144 / 148, 128 to 1152 39.3 / 39.9; 32 / 4 heads of 64, 256 to 4096 67 / 76,
+  // and with 256 work-groups (64 to 1152) 15.4 / 10.0.
   const bool ordered = max_parts == 1 && need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4) &&
                        decode_rows(num_seqs, num_heads, num_kv_heads) > 2LL * device_cus();
   const int group = num_heads / num_kv_heads;
@@ -264,7 +268,11 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
     hipLaunchKernelGGL(tv::decode_order_kernel, dim3(1), dim3(1024), 0, s, context_lens, num_seqs, (int)width, 0,
                        sched);
   }
-  const bool wide = !ordered && max_parts == 1 && width <= tv::kFp8WideTokens &&
+  // Eight waves where a CU has one work-group of few tiles.  MI355X, us, 8 / 4 waves,
+  // 32 / 4 heads of 64: 1 x 500 tokens 5.8 / 6.5, 8 x 250 5.1 / 5.4, 32 x 500 6.3 /
+  // 6.9; with heads of 128 the larger merge takes it back: 1 x 500 7.7 / 7.5, 32 x
+  // 500 8.3 / 7.9.
+  const bool wide = !ordered && max_parts == 1 && head_dim == 64 && width <= tv::kFp8WideTokens &&
                     decode_rows(num_seqs, num_heads, num_kv_heads) <= device_cus();
   tv::launch_paged_decode_fp8(p, head_dim, dtype, wide, s);
   return check_launch(who);

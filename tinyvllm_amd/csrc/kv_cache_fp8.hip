@@ -12,8 +12,11 @@
 // work-group of the first token whose slot lies in the block.  It finds the
 // others by reading the slot list, which also settles a slot that is named twice
 // (the last token wins).  Only tokens whose predecessor lies in another block
-// read the list, one per 16 tokens of a prompt: 8192 tokens read it 512 times,
-// 32 KiB from L2 each, under the rows' own 25 MB.
+// read the list, one per 16 tokens of a prompt, from L2.
+// Bound: the rows' bytes for long prompts, launch and the chain slots -> list ->
+// scale and rows -> maximum for short ones.  MI355X: 8192 fp16 or bf16 rows of 8
+// heads of 128, K and V, 101 MB read and written, 16.7 us (6.0 TB/s; the caches'
+// new bytes stay in the last-level cache), 16384 24.4; 64 rows of a step 5.4.
 // Wave w takes (head, cache) pairs w, w + 4, ...: D / 8 lanes cover a row with
 // eight elements each, and up to kWriteHold rows a lane stay in registers from
 // the maximum to the rounding.
@@ -24,7 +27,7 @@ namespace tv {
 constexpr int kWriteThreads = 256;
 constexpr int kWriteHold = 4;
 constexpr int kWriteFewTokens = 512;
-constexpr long long kWriteGroups = 512;   // work-groups that a prompt's write is cut into
+constexpr long long kWriteGroups = 512;   // work-groups that a long prompt's write keeps
 
 struct Row8 {
   f32x4 a, b;
@@ -312,8 +315,14 @@ void write_of(const KVWriteFp8Params& p, dim3 grid, hipStream_t stream) {
 
 void launch_kv_write_fp8(KVWriteFp8Params p, int dtype, hipStream_t stream) {
   // A step's tokens lie in blocks of their own: one token and four (head, cache)
-  // pairs, one a wave, per work-group.  A prompt's are in runs: sixteen tokens, and
-  // all heads once that gives every CU two work-groups, since each reads the slots.
+  // pairs, one a wave, per work-group.  A prompt's are in runs: sixteen tokens.  The
+  // host sees only their number.  MI355X, us, one / sixteen, 8 heads of 128, bf16:
+  // steps of 128 sequences 5.7 / 45, 512 11 / 42, 1024 20 / 43; prompts of 128 tokens
+  // 6.4 / 5.8, 512 14 / 6, 1024 26 / 6, 8192 178 / 17.
+  // Sixteen tokens take more heads a work-group, as long as two work-groups a CU
+  // remain, since each reads the slots.  8 heads of 128, rule / two heads: 8192
+  // tokens 16.7 / 17.0, 16384 24.4 / 33.8; 32 heads of 128 fp16: 4096 24 / 26, 8192
+  // 44 / 53, 16384 90 / 140; 4 heads of 64 fp32, 8192 7.9 / 9.9.
   p.tokens_per_group = p.num_tokens <= kWriteFewTokens ? 1 : 16;
   const int groups = (p.num_tokens + p.tokens_per_group - 1) / p.tokens_per_group;
   p.heads_per_group = 2;

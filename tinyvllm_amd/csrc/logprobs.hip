@@ -9,11 +9,14 @@
 // out of the sums: log1p(s) keeps its digits where one token has nearly all of
 // the probability, and nothing cancels.
 //
-// Bound: one read of the logits.  A work-group holds kVecs 16-byte vectors a
-// thread of one row in registers (32 KiB at 256 threads, 128 KiB at 1024: a row of
-// 32000 fp32 logits is read once and needs no second launch), so the sums are
-// taken relative to the final maximum.  Longer rows are cut into such segments,
-// and a second kernel joins their (m, s, t) and lists.
+// Bound: one read of the logits, and close behind it the vector unit (an
+// exponential and three more operations an element).  A work-group holds kVecs
+// 16-byte vectors a thread of one row in registers (32 KiB at 256 threads, 128 KiB
+// at 1024: a row of 32000 fp32 logits is read once and needs no second launch), so
+// the sums are taken relative to the final maximum.  Longer rows are cut into such
+// segments, and a second kernel joins their (m, s, t) and lists.  MI355X: 1000 rows
+// of 32000 fp32 26 us (4.9 TB/s), with 5 top tokens 33; of bf16 20 (3.2 TB/s); 2047
+// of 128256 bf16 with 20 top tokens 146 (3.6 TB/s), without 110 (4.8 TB/s).
 // Top tokens of a segment: from the threads' maxima, rounded down to 16 bits, a
 // search over bits with ballots finds a bound that at least k elements reach and few
 // others do; those that do go to a list in LDS and are ranked by (value, then lowest
@@ -91,7 +94,9 @@ __device__ __forceinline__ void finish_row(const LogprobParams& p, int row, floa
   }
 }
 
-// ALIGNED: rows start at multiples of 16 bytes.  TOP: top_k > 0 (its code costs the sums registers).
+// ALIGNED: rows start at multiples of 16 bytes.  TOP: top_k > 0 (its code costs registers: held to
+// the 64 of eight waves a SIMD 2047 rows of 128256 bf16 with 20 top tokens take 153 us, at six waves 146; work-groups
+// of 1024 threads need the eight for two of them per CU).
 template <typename T, int NT, bool ALIGNED, bool TOP>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP && NT < 1024 ? 6 : 8))) logprobs_kernel(const LogprobParams p) {
   constexpr int NW = NT / 64;

@@ -4,7 +4,8 @@
 // with ek, ev the exponents of key j's block.  A context of no tokens gives zeros.
 //
 // Bound: HBM, 2 D bytes per token and KV head; half of a 16-bit cache's, while
-// the arithmetic per token stays.  On the vector unit a token of D 128 and four
+// the arithmetic per token stays.  MI355X, 32 / 8 heads of 128: 256 sequences of 512
+// to 4096 tokens (1.25 GB) 200 us, 6.2 TB/s; 16 of 32768 (1.07 GB) 173 us, 6.2 TB/s.  On the vector unit a token of D 128 and four
 // query heads is 14 instructions a wave with dot2 / fma, which at 8 bits would
 // leave no slack over the conversions; both products go to the matrix cores.
 //
@@ -469,7 +470,7 @@ void launch_of(const DecodeFp8Params& p, hipStream_t stream) {
 template <typename T>
 void launch_dims(const DecodeFp8Params& p, int head_dim, bool wide, hipStream_t stream) {
   if (head_dim == 64) wide ? launch_of<T, 64, 8>(p, stream) : launch_of<T, 64, 4>(p, stream);
-  else if (head_dim == 128) wide ? launch_of<T, 128, 8>(p, stream) : launch_of<T, 128, 4>(p, stream);
+  else if (head_dim == 128) launch_of<T, 128, 4>(p, stream);
   else launch_of<T, 256, 4>(p, stream);
 }
 

@@ -21,7 +21,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kFp8MinExp = -100;       // least scale exponent (blocks of zeros, and blocks never written)
 constexpr int kFp8MaxBlock = 1024;     // rows of a block (the write kernel's row list in LDS)
-constexpr int kFp8WideTokens = 512;   // contexts that small unsplit launches serve with eight waves
+constexpr int kFp8WideTokens = 512;    // contexts of at most this many tokens stay unsplit, whatever the batch
 constexpr uint32_t kFp8Nan = 0x7f;
 
 // Exponent of the scale for rows whose largest magnitude is amax (finite, >= 0):
