@@ -15,8 +15,8 @@
 // read the list, one per 16 tokens of a prompt, from L2.
 // Bound: the rows' bytes for long prompts, launch and the chain slots -> list ->
 // scale and rows -> maximum for short ones.  MI355X: 8192 fp16 or bf16 rows of 8
-// heads of 128, K and V, 101 MB read and written, 16.7 us (6.0 TB/s; the caches'
-// new bytes stay in the last-level cache), 16384 24.4; 64 rows of a step 5.4.
+// heads of 128, K and V, 50 MB read and written, 16.7 us (3.0 TB/s), 16384 24.4
+// (4.1 TB/s); 64 rows of a step 5.4.
 // Wave w takes (head, cache) pairs w, w + 4, ...: D / 8 lanes cover a row with
 // eight elements each, and up to kWriteHold rows a lane stay in registers from
 // the maximum to the rounding.
@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_fp8_kernel(const KVWri
 
 // Row t of the listed blocks as values q * 2^e; fp16 results are limited to
 // +-65504 (an e4m3 rounding of up to 2^-4 can pass fp16's largest number).  Ids
-// outside the cache read as 0.  Eight elements a lane, both caches.
+// outside the cache read as 0.  Eight elements a lane, both caches.  Bound: HBM;
+// 8192 rows as above back to fp16 10.3 us (4.9 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) kv_gather_fp8_kernel(const KVGatherFp8Params p) {
   const int vec = p.head_dim / 8;
