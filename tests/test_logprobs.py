@@ -88,6 +88,7 @@ def test_entry_point_validates_on_the_host():
     assert call(_4=ctypes.c_void_p(258)) == _lib.TV_EINVAL and b"misaligned" in lib.tv_last_error()
     assert call(_7=200000, _8=200000) == _lib.TV_EINVAL and b"workspace" in lib.tv_last_error()
     assert call(_7=1 << 29, _8=1 << 29, _11=p, _12=1 << 40) == _lib.TV_EINVAL and b"too long" in lib.tv_last_error()
+    assert call(_6=1 << 24, _7=8, _8=8) == _lib.TV_EINVAL and b"grid too large" in lib.tv_last_error()
     assert lib.tv_token_logprobs_workspace_bytes(7, 32000, 5, 0) == 0
     assert lib.tv_token_logprobs_workspace_bytes(7, 128256, 5, 0) == 7 * 8 * 52
     assert lib.tv_token_logprobs_workspace_bytes(7, 128256, 5, 2) == 7 * 4 * 52

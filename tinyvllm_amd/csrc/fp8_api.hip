@@ -50,7 +50,8 @@ int write_common(const char* who, void* k_cache, void* v_cache, float* k_scale, 
   if (!k || !v) return fail(TV_EINVAL, "%s: null pointer argument", who);
   if (!aligned(k, es) || !aligned(v, es) || (slots && !aligned(slots, 4)))
     return fail(TV_EINVAL, "%s: misaligned input", who);
-  if ((num_kv_heads + 1) / 2 > 65535) return fail(TV_EINVAL, "%s: grid too large", who);
+  // a launch holds fewer than 2^32 threads per dimension: 16 tokens per work-group of 256
+  if ((num_kv_heads + 1) / 2 > 65535 || num_tokens >= 1 << 28) return fail(TV_EINVAL, "%s: grid too large", who);
   tv::KVWriteFp8Params p{};
   p.k_cache = static_cast<uint8_t*>(k_cache);
   p.v_cache = static_cast<uint8_t*>(v_cache);
@@ -229,7 +230,8 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
   // 1152 144 / 148, 128 to 1152 39.3 / 39.9; 32 / 4 heads of 64, 256 to 4096 67 / 76,
   // and with 256 work-groups (64 to 1152) 15.4 / 10.0.
   const bool ordered = max_parts == 1 && need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4) &&
-                       decode_rows(num_seqs, num_heads, num_kv_heads) > 2LL * device_cus();
+                       decode_rows(num_seqs, num_heads, num_kv_heads) > 2LL * device_cus() &&
+                       decode_rows(num_seqs, num_heads, num_kv_heads) < 1LL << 24;   // 256 threads each in one dimension
   const int group = num_heads / num_kv_heads;
   const int chunks = (group + 15) / 16;
   if (num_seqs > 65535 || max_parts > 65535 || num_heads > 0x7fffffff / 256)

@@ -633,6 +633,8 @@ int tv_token_logprobs(float* logprobs, float* entropy, int32_t* top_ids, float* 
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
     return fail(TV_EINVAL, "%s: workspace of %zu bytes, 8-byte aligned, required (got %zu)", who, need, workspace_bytes);
   if ((long long)vocab * es > (1LL << 30)) return fail(TV_EINVAL, "%s: rows of %d logits are too long", who, vocab);
+  if ((long long)M * std::max(256, tv::logprob_threads(vocab, es)) >= 1LL << 32)   // threads of a launch's dimension
+    return fail(TV_EINVAL, "%s: grid too large for %d rows", who, M);
   const int segs = tv::logprob_segments(vocab, es);
   tv::LogprobParams p{};
   p.logits = logits;
