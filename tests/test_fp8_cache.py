@@ -66,6 +66,7 @@ def test_entry_points_validate_on_the_host():
     assert write(_0=ctypes.c_void_p(264)) == _lib.TV_EINVAL and b"aligned" in lib.tv_last_error()
     assert write(_4=ctypes.c_void_p(257)) == _lib.TV_EINVAL and b"misaligned" in lib.tv_last_error()
     assert write(_7=-1) == _lib.TV_EINVAL
+    assert write(_7=1 << 28) == _lib.TV_EINVAL and b"grid too large" in lib.tv_last_error()
     assert write(_7=0) == _lib.TV_OK
     b = [p, p, p, p, p, p, 3, 0, 4, 2, 64, 16, 8, 128, 128, 1, None]
     assert lib.tv_write_kv_fp8(*b[:6], 8, *b[7:]) == _lib.TV_EINVAL and b"block_id" in lib.tv_last_error()
@@ -243,6 +244,25 @@ def test_read_in_fp16_is_limited_to_its_largest_number():
     cache.write_kv(0, 0, 0, x, -x)
     k, v = cache.read_kv_blocks(0, [0], 1)
     assert torch.equal(k, x) and torch.equal(v, -x)             # 65536 in e4m3
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["FP8KVCache", "KVCache"])
+def test_a_single_token_with_spread_heads_is_refused(kind):
+    """One token whose heads are not next to each other: its row is not the memory behind its first element."""
+    from tinyvllm_amd import kv_cache
+    cache = getattr(kv_cache, kind)(1, 2, 16, 2, 64, "float16")
+    x = torch.randn((2, 2, 128), device="cuda").half()[:1, :, :64]
+    with pytest.raises(ValueError, match="contiguous"):
+        cache.write_kv(0, 0, 0, x, x)
+    with pytest.raises(ValueError, match="contiguous"):
+        cache.write_kv(0, 0, 0, x.contiguous()[0], x[0])
+    cache.write_kv(0, 0, 0, x.contiguous(), x[0].contiguous())
+    one = getattr(kv_cache, kind)(1, 2, 16, 1, 64, "float16")
+    y = torch.randn((3, 5, 64), device="cuda").half()[:, 2:3]      # one head: any stride of it will do
+    one.write_kv(0, 0, 0, y, y)
+    k, v = one.read_kv_blocks(0, [0], 3)
+    assert torch.equal(k, v) and (k - y).abs().max() <= 2.0 ** -4 * y.abs().max()
 
 
 def test_python_refusals_need_no_gpu():

@@ -57,7 +57,7 @@ class KVCache:
             raise ValueError(f"{name} dtype {x.dtype} differs from cache dtype {self.dtype}")
         if x.device != self.k_cache[0].device:
             raise ValueError(f"{name} must be on {self.k_cache[0].device}")
-        if x.shape[0] > 1 and not (x.stride(2) == 1 and x.stride(1) == self.head_dim):
+        if x.shape[0] and not x[0].is_contiguous():
             raise ValueError(f"{name}: heads and head_dim must be contiguous")
         stride = x.stride(0) if x.shape[0] > 1 else self.n_kv_heads * self.head_dim
         return x, stride
