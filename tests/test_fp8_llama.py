@@ -177,6 +177,33 @@ def test_device_loop_equals_single_steps(dtype):
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+@gpu
+@pytest.mark.parametrize("kind", ["FP8KVCache", "KVCache"])
+def test_a_captured_step_keeps_its_cache(kind):
+    """The steps of a decode are kept by the cache they were captured for: neither its memory nor its
+    identity may pass to another cache before they are gone."""
+    import gc
+    import weakref
+    from tinyvllm_amd import kv_cache
+    config, model, _ = build("float16")
+
+    def make():
+        return getattr(kv_cache, kind)(config.n_layers, 4, 16, config.n_kv_heads, config.head_dim, "float16")
+    jit = model.create_jit_decode(16)
+    first = make()
+    storage = first.k_cache[0].data_ptr()
+    graph = jit.graph_for(first, 2, 2)
+    seen = weakref.ref(first)
+    del first
+    gc.collect()
+    assert seen() is not None
+    second = make()
+    assert second.k_cache[0].data_ptr() != storage and jit.graph_for(second, 2, 2) is not graph
+    del graph, jit, second
+    gc.collect()
+    assert seen() is None
+
+
 def test_cache_struct_is_validated_on_the_host():
     """One scale array of two, and slots past 32 bits, are refused before any launch."""
     from tinyvllm_amd import _lib

@@ -322,7 +322,8 @@ class Llama:
         if isinstance(kv_cache, FP8KVCache):
             keep += [_ptr_array(kv_cache.k_scale), _ptr_array(kv_cache.v_scale)]
             s.k_scales, s.v_scales = (ctypes.cast(x, _PP) for x in keep[2:])
-        return s, tuple(keep)
+        # the cache and its storage live as long as what points at them (a captured step, say)
+        return s, (*keep, kv_cache, *kv_cache.k_cache, *kv_cache.v_cache)
 
     # ---- prefill ---------------------------------------------------------------
     def prefill(self, tokens, kv_cache, block_manager, seq_id, start_pos=0, *, logits="all", attend_prefix=False):
