@@ -235,9 +235,12 @@ int tv_read_kv_blocks(void* k_out, void* v_out, const void* k_cache, const void*
  * [num_blocks, num_kv_heads] powers of two of at least 2^-100 (the value of a
  * block that was never written; the entry points below keep them so); an element
  * stands for number * scale.  dtype is that of the rows written, of the queries
- * and of the values read back, and need not be the same in every call.  TV_F16
- * values and outputs are limited to +-65504, which a value's rounding to e4m3 can
- * pass.  head_dim 64, 128 or 256, block_size at most 1024 (TV_EUNSUPPORTED
+ * and of the values read back, and need not be the same in every call.  Values
+ * read back, and TV_F16 outputs, are limited to the dtype's largest finite number,
+ * which a value's rounding to e4m3 can pass.  Attention sums weights of up to 2^8
+ * times values in fp32: elements of V of 2^89 and more in magnitude, and scores
+ * past fp32's range, may give infinities or NaN in the rows that attend them, and
+ * change no other row.  head_dim 64, 128 or 256, block_size at most 1024 (TV_EUNSUPPORTED
  * otherwise).
  */
 

@@ -21,8 +21,8 @@
 // more is on the way in registers: one barrier a tile.  Where the tiles of rows
 // are too few for the GPU, the keys are split between work-groups and a second
 // kernel joins their parts.
-// Numbers: K and V enter as their dequantised values in T, exact but for fp16's
-// range (values are limited to +-65504; below fp16's normal numbers they are
+// Numbers: K and V enter as their dequantised values in T, exact but for its range
+// (values are limited to T's largest number; below fp16's normal numbers they are
 // rounded as fp16 inputs that small are).  Scores, maxima, sums, accumulators are
 // fp32; a weight is rounded to T for the second product, as in the 16-bit prefill
 // kernels, and the row sum is that of the rounded weights.
@@ -50,13 +50,10 @@ template <typename T, bool HI> __device__ __forceinline__ uint32_t scaled_pair(u
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
 }
 
-// Four e4m3 numbers as T; fp16 limited to its range (only scales of 2^8 and more leave it).
+// Four e4m3 numbers as T, limited to its range.
 template <typename T> __device__ __forceinline__ u32x2 dequant4(uint32_t w, float scale) {
-  if (ElemTraits<T>::kCode == kF16 && scale > 128.0f) {
-    f32x4 x = fp8_to_f32x4(w) * scale;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (fabsf(x[i]) > 65504.0f) x[i] = __builtin_copysignf(65504.0f, x[i]);
+  if (scale > kSafeScale<T>) {
+    const f32x4 x = limited<T>(fp8_to_f32x4(w) * scale);
     return u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
   }
   return u32x2{scaled_pair<T, false>(w, scale), scaled_pair<T, true>(w, scale)};
@@ -173,17 +170,18 @@ __global__ void __launch_bounds__(kThreads * KS, KS == 1 ? 2 : KS) prefill_fp8_k
   };
   auto lstore = [&](const Stage& s, int b, int t) {
     // Nearly every tile: all of its keys inside the sequence, in blocks of the cache, no NaN among the
-    // values and scales that fp16 holds.
-    bool special = (t + 1) * BN > kv_len;
+    // values and scales whose values T holds.
+    uint32_t nan = 0;
+    uint32_t largest = (t + 1) * BN > kv_len ? ~0u : 0u;   // of the scales, as bits: uniform where they are
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      uint32_t nan = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) nan |= (s.v[i][j] & 0x7f7f7f7fu) + 0x01010101u;
-      special |= (nan & 0x80808080u) != 0 || s.ok[i] == 0;
-      if constexpr (ElemTraits<T>::kCode == kF16) special |= s.ks[i] > 128.0f || s.vs[i] > 128.0f;
+      largest = max(largest, max(__builtin_bit_cast(uint32_t, s.ks[i]), __builtin_bit_cast(uint32_t, s.vs[i])) | ~s.ok[i]);
     }
-    if (__builtin_amdgcn_ballot_w64(special) == 0) {
+    uint64_t special = __builtin_amdgcn_ballot_w64((nan & 0x80808080u) != 0);
+    special |= __builtin_amdgcn_ballot_w64(largest > __builtin_bit_cast(uint32_t, kSafeScale<T>));
+    if (special == 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         u32x2 kw[4], vw[4];

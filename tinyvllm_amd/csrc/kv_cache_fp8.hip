@@ -254,9 +254,8 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_fp8_kernel(const KVWri
   }
 }
 
-// Row t of the listed blocks as values q * 2^e; fp16 results are limited to
-// +-65504 (an e4m3 rounding of up to 2^-4 can pass fp16's largest number).  Ids
-// outside the cache read as 0.  Eight elements a lane, both caches.  Bound: HBM;
+// Row t of the listed blocks as values q * 2^e, limited to T's largest finite
+// number.  Ids outside the cache read as 0.  Eight elements a lane, both caches.  Bound: HBM;
 // 8192 rows as above back to fp16 10.3 us (4.9 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) kv_gather_fp8_kernel(const KVGatherFp8Params p) {
@@ -283,19 +282,12 @@ __global__ void __launch_bounds__(256) kv_gather_fp8_kernel(const KVGatherFp8Par
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      f32x4 a = fp8_to_f32x4(w[i][0]) * f[i], b = fp8_to_f32x4(w[i][1]) * f[i];
+      const f32x4 a = limited<T>(fp8_to_f32x4(w[i][0]) * f[i]), b = limited<T>(fp8_to_f32x4(w[i][1]) * f[i]);
       T* out = reinterpret_cast<T*>(i ? p.v_out : p.k_out) + idx * 8;
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<f32x4*>(out) = a;
         *reinterpret_cast<f32x4*>(out + 4) = b;
       } else {
-        if constexpr (ElemTraits<T>::kCode == kF16) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (fabsf(a[j]) > 65504.0f) a[j] = __builtin_copysignf(65504.0f, a[j]);
-            if (fabsf(b[j]) > 65504.0f) b[j] = __builtin_copysignf(65504.0f, b[j]);
-          }
-        }
         *reinterpret_cast<u32x4*>(out) =
             u32x4{pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]), pack2<T>(b[0], b[1]), pack2<T>(b[2], b[3])};
       }

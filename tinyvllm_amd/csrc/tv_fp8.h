@@ -66,6 +66,21 @@ template <typename T, bool HI> __device__ __forceinline__ uint32_t fp8_to_pair(u
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 
+// The largest finite number of T.  A value's rounding to e4m3, of up to 2^-4, can
+// lift it past that number (65504 becomes 65536, 3.3e38 becomes 2^128), and an
+// infinity in V would reach rows that give it a weight of zero: what is read back
+// as T is limited to it.  Only scales above kSafeScale need the comparison.
+template <typename T> constexpr float kLargest =
+    ElemTraits<T>::kCode == kF16 ? 65504.0f : ElemTraits<T>::kCode == kBF16 ? 0x1.fep127f : 0x1.fffffep127f;
+template <typename T> constexpr float kSafeScale = ElemTraits<T>::kCode == kF16 ? 0x1p7f : 0x1p119f;   // 448 times it is in range
+
+template <typename T> __device__ __forceinline__ f32x4 limited(f32x4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (fabsf(x[i]) > kLargest<T>) x[i] = __builtin_copysignf(kLargest<T>, x[i]);   // NaN stays
+  return x;
+}
+
 // An output that averages cached values.  Rounding to e4m3 can lift a value near
 // fp16's largest past it (65504 becomes 65536), so fp16 outputs are limited to it.
 __device__ __forceinline__ void store_limited(void* base, size_t idx, float v, int dtype) {
