@@ -1,5 +1,7 @@
 """The 8-bit cache at the edges of its number range and of its callers' contracts."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -44,3 +46,47 @@ def test_chunk_rows_do_not_see_huge_elements_that_they_do_not_attend(bs, d):
     assert int((~torch.isfinite(got[0, :60])).sum()) == 0
     check_chunk(got, held, q, table, start, "bfloat16", rows=slice(0, 60))
     assert int((~torch.isfinite(got[0, :, 2:])).sum()) == 0              # the other KV head's
+
+
+def test_model_calls_refuse_an_8_bit_caches_misuse_before_any_launch():
+    """Shapes and sizes that a layer's kernels would refuse after others have run; no workspace is given, so a
+    call that passes these checks stops at that."""
+    from tinyvllm_amd import _lib
+    from tinyvllm_amd.llama import _Cache, _DecodeArgs, _Model, _PP, _PrefillArgs
+    lib = _lib.load()
+    keep = [(ctypes.c_void_p * 2)(*x) for x in ((256, 256), (256, 264), (256, None), (256, 258))]
+    pp, off8, null, off2 = (ctypes.cast(x, _PP) for x in keep)
+
+    def model(head_dim=64, dtype=_lib.TV_F16, heads=4):
+        return _Model(2, 64, heads, 1, head_dim, 64, 64, dtype, 1e-5, 256, pp, pp, pp, pp, pp, pp, 256, 256, 256, 16)
+
+    def decode(m, cache, batch=1, blocks=4, part=64):
+        args = _DecodeArgs(batch, 256, 256, 256, 256, blocks, blocks, part, 1, None, None, 0, None, 0)
+        rc = lib.tv_llama_decode_step(ctypes.byref(m), ctypes.byref(cache), ctypes.byref(args), None)
+        return rc, lib.tv_last_error()
+
+    def prefill(m, cache, n, start, attend=1, width=1 << 24):
+        args = _PrefillArgs(n, 256, start, 256, width, None, 0, None, None, 0, attend)
+        rc = lib.tv_llama_prefill(ctypes.byref(m), ctypes.byref(cache), ctypes.byref(args), None)
+        return rc, lib.tv_last_error()
+
+    good = _Cache(pp, pp, 8, 16, pp, pp)
+    for m, cache, code, what in ((model(32), good, _lib.TV_EUNSUPPORTED, b"head_dim 32"),
+                                 (model(), _Cache(pp, pp, 8, 1040, pp, pp), _lib.TV_EUNSUPPORTED, b"block_size 1040"),
+                                 (model(), _Cache(off8, pp, 8, 16, pp, pp), _lib.TV_EINVAL, b"aligned"),
+                                 (model(), _Cache(pp, null, 8, 16, pp, pp), _lib.TV_EINVAL, b"layer 1"),
+                                 (model(), _Cache(pp, pp, 8, 16, pp, null), _lib.TV_EINVAL, b"layer 1"),
+                                 (model(), _Cache(pp, pp, 8, 16, off2, pp), _lib.TV_EINVAL, b"scales 4-byte")):
+        for rc, error in (decode(m, cache), prefill(m, cache, 4, 0)):
+            assert rc == code and what in error
+    for got in (decode(model(), good, part=48), decode(model(), good, batch=65536), decode(model(), good, blocks=1 << 27),
+                decode(model(), good, blocks=1 << 18, part=32)):
+        assert got[0] == _lib.TV_EINVAL and b"over an 8-bit cache" in got[1]
+    for got in (prefill(model(dtype=_lib.TV_F32), good, 65536, 8), prefill(model(), good, 65535 * 16 + 1, 8),
+                prefill(model(), good, 9, (1 << 30) - 8, width=1 << 27)):
+        assert got[0] == _lib.TV_EINVAL and b"too long over an 8-bit cache" in got[1]
+    # the same without a prefix, over a 16-bit cache, and at the limits: only the workspace is missing
+    plain = _Cache(pp, pp, 8, 16)
+    for got in (decode(model(), good), decode(model(), plain, part=48), prefill(model(dtype=_lib.TV_F32), good, 65536, 8, 0),
+                prefill(model(dtype=_lib.TV_F32), good, 65535, 8), prefill(model(), plain, 9, 8)):
+        assert got[0] == _lib.TV_EINVAL and b"workspace" in got[1], got[1]

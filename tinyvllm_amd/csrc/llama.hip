@@ -20,6 +20,7 @@
 #include "../../include/tv_llama.h"
 #include "tv_dense.h"
 #include "tv_error.h"
+#include "tv_fp8.h"
 #include "tv_logprobs.h"
 #include "tv_paged_keys.h"
 #include "tv_params.h"
@@ -432,14 +433,47 @@ int attend_fp8(const tv_llama_model* m, const tv_llama_cache* c, const LayerIO& 
                                     room ? io.extra_ws_bytes : 0, s);
 }
 
-// A cache's pointers; an 8-bit one has both scale arrays and slots that fit 32 bits.
-int validate_cache(const tv_llama_cache* c, const char* who) {
+// A cache's pointers; an 8-bit one has both scale arrays, slots that fit 32 bits
+// and the shape that its kernels take (each would refuse it in the middle of a layer).
+int validate_cache(const tv_llama_model* m, const tv_llama_cache* c, const char* who) {
   if (!c || !c->k_caches || !c->v_caches || c->num_blocks <= 0 || c->block_size <= 0)
     return fail(TV_EINVAL, "%s: bad cache", who);
   if (!c->k_scales != !c->v_scales) return fail(TV_EINVAL, "%s: give both scale arrays of an 8-bit cache or neither", who);
   if (c->k_scales && (long long)c->num_blocks * c->block_size > 0x7fffffffLL)
     return fail(TV_EUNSUPPORTED, "%s: an 8-bit cache of %d blocks of %d has slots past 32 bits", who, c->num_blocks,
                 c->block_size);
+  if (c->k_scales && (!(m->head_dim == 64 || m->head_dim == 128 || m->head_dim == 256) ||
+                      c->block_size > tv::kFp8MaxBlock))
+    return fail(TV_EUNSUPPORTED, "%s: an 8-bit cache of head_dim %d, block_size %d (64/128/256, at most %d)", who,
+                m->head_dim, c->block_size, tv::kFp8MaxBlock);
+  for (int l = 0; c->k_scales && l < m->n_layers; ++l)
+    if (!c->k_caches[l] || !c->v_caches[l] || !c->k_scales[l] || !c->v_scales[l] || !aligned16(c->k_caches[l]) ||
+        !aligned16(c->v_caches[l]) || (uintptr_t)c->k_scales[l] % 4 || (uintptr_t)c->v_scales[l] % 4)
+      return fail(TV_EINVAL, "%s: 8-bit caches must be 16-byte aligned, scales 4-byte aligned (layer %d)", who, l);
+  return TV_OK;
+}
+
+// The limits of a decode step over an 8-bit cache (tv_paged_decode_fp8's).
+int validate_decode_fp8(const tv_llama_cache* c, const tv_llama_decode_args* a, const char* who) {
+  if (!c->k_scales) return TV_OK;
+  if (a->partition_size % 32)
+    return fail(TV_EINVAL, "%s: partition_size %d must be a multiple of 32 over an 8-bit cache", who, a->partition_size);
+  const long long width = (long long)a->max_blocks * c->block_size;
+  if (width > 1LL << 30 || a->batch > 65535 || (width + a->partition_size - 1) / a->partition_size > 65535)
+    return fail(TV_EINVAL, "%s: %d sequences of %lld tokens in partitions of %d are too many over an 8-bit cache", who,
+                a->batch, width, a->partition_size);
+  return TV_OK;
+}
+
+// The same of a prompt's chunk that attends the cache: tv_paged_decode_fp8 for fp32 rows, tv_flash_prefill_paged_fp8 else.
+int validate_prefill_fp8(const tv_llama_model* m, const tv_llama_cache* c, const tv_llama_prefill_args* a, const char* who) {
+  if (!c->k_scales) return TV_OK;
+  const long long group = m->n_heads / m->n_kv_heads;
+  const long long most = m->dtype == TV_F32 ? 65535LL : 65535LL * 64 / group;
+  const bool attends = a->attend_prefix && a->start_pos > 0;
+  if (a->num_tokens >= 1 << 28 ||
+      (attends && (a->num_tokens > most || (long long)a->start_pos + a->num_tokens > 1LL << 30)))
+    return fail(TV_EINVAL, "%s: a chunk of %d tokens at %d is too long over an 8-bit cache", who, a->num_tokens, a->start_pos);
   return TV_OK;
 }
 
@@ -665,10 +699,11 @@ int tv_llama_decode_step(const tv_llama_model* m, const tv_llama_cache* c, const
                          void* stream) {
   int rc = validate_model(m, "tv_llama_decode_step");
   if (rc != TV_OK) return rc;
-  if ((rc = validate_cache(c, "tv_llama_decode_step")) != TV_OK) return rc;
+  if ((rc = validate_cache(m, c, "tv_llama_decode_step")) != TV_OK) return rc;
   if (!a || a->batch <= 0 || !a->tokens || !a->positions || !a->context_lens || !a->block_tables ||
       a->bt_stride <= 0 || a->max_blocks <= 0 || a->max_blocks > a->bt_stride || a->partition_size <= 0)
     return fail(TV_EINVAL, "tv_llama_decode_step: bad decode arguments");
+  if ((rc = validate_decode_fp8(c, a, "tv_llama_decode_step")) != TV_OK) return rc;
   if (a->history && a->history_len <= 0) return fail(TV_EINVAL, "tv_llama_decode_step: bad history_len");
   if ((rc = validate_widths(m, a->batch, "tv_llama_decode_step")) != TV_OK) return rc;
   if (a->logits && !aligned16(a->logits)) return fail(TV_EINVAL, "tv_llama_decode_step: logits must be 16-byte aligned");
@@ -765,9 +800,10 @@ size_t tv_llama_prefill_workspace_bytes(const tv_llama_model* model, int num_tok
 int tv_llama_prefill(const tv_llama_model* m, const tv_llama_cache* c, const tv_llama_prefill_args* a, void* stream) {
   int rc = validate_model(m, "tv_llama_prefill");
   if (rc != TV_OK) return rc;
-  if ((rc = validate_cache(c, "tv_llama_prefill")) != TV_OK) return rc;
+  if ((rc = validate_cache(m, c, "tv_llama_prefill")) != TV_OK) return rc;
   if (!a || a->num_tokens <= 0 || !a->tokens || !a->block_table || a->bt_width <= 0 || a->start_pos < 0)
     return fail(TV_EINVAL, "tv_llama_prefill: bad prefill arguments");
+  if ((rc = validate_prefill_fp8(m, c, a, "tv_llama_prefill")) != TV_OK) return rc;
   if (a->logits && !aligned16(a->logits)) return fail(TV_EINVAL, "tv_llama_prefill: logits must be 16-byte aligned");
   const int M = a->num_tokens;
   if ((rc = validate_widths(m, M, "tv_llama_prefill")) != TV_OK) return rc;
