@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests.test_fp8_cache import DTYPES, gpu, make_cache, rng_of
+from tests.test_fp8_llama import build
 from tests.test_fp8_prefill import check_chunk, chunk_case, run_chunk
 
 
@@ -90,3 +91,20 @@ def test_model_calls_refuse_an_8_bit_caches_misuse_before_any_launch():
     for got in (decode(model(), good), decode(model(), plain, part=48), prefill(model(dtype=_lib.TV_F32), good, 65536, 8, 0),
                 prefill(model(dtype=_lib.TV_F32), good, 65535, 8), prefill(model(), plain, 9, 8)):
         assert got[0] == _lib.TV_EINVAL and b"workspace" in got[1], got[1]
+
+
+@gpu
+@pytest.mark.parametrize("columns", [4, 1 << 21])
+def test_fp32_chunk_over_a_table_wider_than_it_needs(columns):
+    """2^21 columns of 1024 tokens: the table's tokens pass 32 bits, the chunk's do not."""
+    from tinyvllm_amd.kv_cache import FP8KVCache
+    config, model, _ = build("float32")
+    tokens = torch.arange(60, dtype=torch.int32)
+    out = []
+    for width in (1, columns):
+        cache = FP8KVCache(config.n_layers, 2, 1024, config.n_kv_heads, config.head_dim, "float32")
+        table = torch.zeros(width, dtype=torch.int32, device="cuda")
+        table[0] = 1
+        model.prefill_table(tokens[:20], cache, table, logits=None)
+        out.append(model.prefill_table(tokens[20:], cache, table, 20, attend_prefix=True))
+    assert torch.equal(*out)

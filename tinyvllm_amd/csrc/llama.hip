@@ -418,11 +418,13 @@ int attend_fp8(const tv_llama_model* m, const tv_llama_cache* c, const LayerIO& 
     return tv_flash_prefill(io.attn, io.q, io.kst, io.vst, M, M, m->n_heads, m->n_kv_heads, m->head_dim, m->head_dim,
                             qd, kd, kd, qd, 1, scale, dt, dt, 0, nullptr, 0, s);
   if (dt == TV_F32) {
-    // row i is a single-token attention of context start_pos + i + 1 over the sequence's one table row
-    const int width = a->bt_width * c->block_size;
+    // row i is a single-token attention of context start_pos + i + 1 over the columns of the sequence's one
+    // table row that the chunk reaches (a wider table's tokens may pass 32 bits)
+    const int columns = (a->start_pos + M + c->block_size - 1) / c->block_size;
+    const int width = columns * c->block_size;
     return tv_paged_decode_fp8(io.attn, io.q, c->k_caches[l], c->v_caches[l], c->k_scales[l], c->v_scales[l],
                                a->block_table, io.slots, M, m->n_heads, m->n_kv_heads, m->head_dim, c->block_size,
-                               c->num_blocks, 0, a->bt_width, scale, dt, dt, (width + 31) / 32 * 32, io.attn_ws,
+                               c->num_blocks, 0, columns, scale, dt, dt, (width + 31) / 32 * 32, io.attn_ws,
                                io.attn_ws_bytes, s);
   }
   const size_t need = tv_flash_prefill_paged_fp8_workspace_bytes(M, a->start_pos, m->n_heads, m->n_kv_heads, m->head_dim);
@@ -471,8 +473,8 @@ int validate_prefill_fp8(const tv_llama_model* m, const tv_llama_cache* c, const
   const long long group = m->n_heads / m->n_kv_heads;
   const long long most = m->dtype == TV_F32 ? 65535LL : 65535LL * 64 / group;
   const bool attends = a->attend_prefix && a->start_pos > 0;
-  if (a->num_tokens >= 1 << 28 ||
-      (attends && (a->num_tokens > most || (long long)a->start_pos + a->num_tokens > 1LL << 30)))
+  const long long reach = ((long long)a->start_pos + a->num_tokens + c->block_size - 1) / c->block_size * c->block_size;
+  if (a->num_tokens >= 1 << 28 || (attends && (a->num_tokens > most || reach > 1LL << 30)))
     return fail(TV_EINVAL, "%s: a chunk of %d tokens at %d is too long over an 8-bit cache", who, a->num_tokens, a->start_pos);
   return TV_OK;
 }
