@@ -108,3 +108,24 @@ def test_fp32_chunk_over_a_table_wider_than_it_needs(columns):
         model.prefill_table(tokens[:20], cache, table, logits=None)
         out.append(model.prefill_table(tokens[20:], cache, table, 20, attend_prefix=True))
     assert torch.equal(*out)
+
+
+@gpu
+def test_a_captured_step_keeps_its_scales():
+    """A step points at the scales as at the numbers: both outlive their place in the cache's lists."""
+    import gc
+    import weakref
+    from tinyvllm_amd.kv_cache import FP8KVCache
+    from tinyvllm_amd.llama import DecodeGraph
+    config, model, _ = build("bfloat16")
+    cache = FP8KVCache(config.n_layers, 4, 16, config.n_kv_heads, config.head_dim, "bfloat16")
+    graph = DecodeGraph(model, cache, 1, 4)
+    lists = (cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale)
+    seen = [weakref.ref(x[1]) for x in lists]
+    for x in lists:
+        x[1] = torch.zeros_like(x[1].view(torch.uint8)).view(x[1].dtype)
+    gc.collect()
+    assert all(r() is not None for r in seen)
+    del graph
+    gc.collect()
+    assert all(r() is None for r in seen)

@@ -319,11 +319,13 @@ class Llama:
             raise ValueError("KV cache shape / dtype does not match the model")
         keep = [_ptr_array(kv_cache.k_cache), _ptr_array(kv_cache.v_cache)]
         s = _Cache(ctypes.cast(keep[0], _PP), ctypes.cast(keep[1], _PP), kv_cache.num_blocks, kv_cache.block_size)
+        storage = [*kv_cache.k_cache, *kv_cache.v_cache]
         if isinstance(kv_cache, FP8KVCache):
             keep += [_ptr_array(kv_cache.k_scale), _ptr_array(kv_cache.v_scale)]
             s.k_scales, s.v_scales = (ctypes.cast(x, _PP) for x in keep[2:])
+            storage += [*kv_cache.k_scale, *kv_cache.v_scale]
         # the cache and its storage live as long as what points at them (a captured step, say)
-        return s, (*keep, kv_cache, *kv_cache.k_cache, *kv_cache.v_cache)
+        return s, (*keep, kv_cache, *storage)
 
     # ---- prefill ---------------------------------------------------------------
     def prefill(self, tokens, kv_cache, block_manager, seq_id, start_pos=0, *, logits="all", attend_prefix=False):
