@@ -129,3 +129,30 @@ def test_a_captured_step_keeps_its_scales():
     del graph
     gc.collect()
     assert all(r() is None for r in seen)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["FP8KVCache", "KVCache"])
+def test_a_replaced_cache_can_be_released(kind):
+    """Steps of an old cache are dropped, their memory with them; those of other caches stay."""
+    import gc
+    import weakref
+    from tinyvllm_amd import kv_cache
+    config, model, _ = build("float16")
+
+    def make():
+        return getattr(kv_cache, kind)(config.n_layers, 4, 16, config.n_kv_heads, config.head_dim, "float16")
+    jit = model.create_jit_decode(16)
+    old, new = make(), make()
+    for batch in (1, 2):
+        jit.graph_for(old, batch, 2).run(2)
+    kept = jit.graph_for(new, 2, 2)
+    jit.release(make())                              # nothing was captured for it
+    seen = [weakref.ref(old), weakref.ref(old.k_cache[0])]
+    jit.release(old)
+    del old
+    gc.collect()
+    assert all(r() is None for r in seen)
+    assert jit.graph_for(new, 2, 2) is kept
+    kept.run(1)
+    torch.cuda.synchronize()

@@ -434,7 +434,11 @@ class Llama:
 
 
 class JitDecode:
-    """Per-batch-size cache of captured decode steps (engine.py:79-81, 157-159)."""
+    """Per-batch-size cache of captured decode steps (engine.py:79-81, 157-159).
+
+    A step keeps the KV cache it was captured for, and its memory, alive: a caller that replaces its cache
+    calls ``release`` with the old one.
+    """
 
     def __init__(self, model, block_size):
         self.model = model
@@ -449,6 +453,14 @@ class JitDecode:
                 raise ValueError("KV cache block size differs from the one the decode was created for")
             self.graphs[key] = DecodeGraph(self.model, kv_cache, batch, max_blocks, table_width=width)
         return self.graphs[key]
+
+    def release(self, kv_cache):
+        """Forget the steps captured for a cache, after those under way have ended."""
+        held = [key for key in self.graphs if key[0] == id(kv_cache)]
+        if held:
+            torch.cuda.synchronize(self.model.device)
+        for key in held:
+            del self.graphs[key]
 
 
 class DecodeGraph:
