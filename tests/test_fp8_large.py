@@ -1,4 +1,5 @@
-"""The 8-bit cache's kernels at sizes where they take another form: row tiles of 128 with two key groups."""
+"""The 8-bit cache's kernels at sizes where they take another form: row tiles of 128 with two key groups,
+a longest-first batch, a merge of more than a thousand partitions."""
 
 import math
 
@@ -8,7 +9,7 @@ import torch
 
 from oracle import fp8_cache as ref
 from tests.fp8_tolerance import rounded_weights_bound
-from tests.test_fp8_cache import gpu, rng_of
+from tests.test_fp8_cache import check_decode, decode_case, gpu, rng_of, run_decode
 from tests.test_fp8_prefill import chunk_case, run_chunk
 
 
@@ -94,3 +95,63 @@ def test_peaked_softmax_in_128_row_tiles(dtype, d):
     cache, held, q, table = wide_case(rng, d, 16, dtype)
     q.mul_(16)
     check_rows_of_chunk(run_chunk(cache, q, table, 37), held, q, table, 37, dtype, [0, 30, 200, 511, 777, 900])
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [("float16", 64), ("bfloat16", 128), ("float32", 64)])
+def test_decode_of_a_longest_first_batch(dtype, d):
+    """More work-groups than two a CU run in the order of their lengths, which changes no result."""
+    from tinyvllm_amd import _lib
+    lib = _lib.load()
+    rng = rng_of(93)
+    b, hq, hkv, bs = 130, 16, 8, 16
+    ctx = rng.integers(0, 400, b)
+    ctx[[0, 7, 129]] = [0, 600, 1]
+    assert b * hkv > 2 * cus()
+    cache, held, q, tables, ctx = decode_case(rng, ctx, hq, hkv, d, bs, dtype)
+    part = -(-tables.shape[1] * bs // 32) * 32
+    assert lib.tv_paged_decode_fp8_workspace_bytes(b, hq, d, tables.shape[1], bs, part) > 0     # the order's
+    got = run_decode(cache, q, tables, ctx, hq, hkv, d, bs, partition_size=part)
+    assert torch.count_nonzero(got[torch.from_numpy(ctx == 0).cuda()]) == 0
+    check_decode(got, held, q, tables, ctx, d, dtype)
+    out = torch.full_like(q, float("nan"))
+    tb, cx = torch.from_numpy(tables).cuda(), torch.from_numpy(ctx).cuda()
+    code = _lib.dtype_code(q.dtype)
+    _lib.check(lib.tv_paged_decode_fp8(
+        out.data_ptr(), q.data_ptr(), cache.k_cache[0].data_ptr(), cache.v_cache[0].data_ptr(),
+        cache.k_scale[0].data_ptr(), cache.v_scale[0].data_ptr(), tb.data_ptr(), cx.data_ptr(), b, hq, hkv, d, bs,
+        cache.num_blocks, tables.shape[1], tables.shape[1], 1 / math.sqrt(d), code, code, part, None, 0,
+        _lib.stream_ptr(q.device)), "batch order")
+    assert torch.equal(out, got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [("bfloat16", 64), ("float16", 128), ("float32", 256)])
+def test_decode_over_more_than_1024_partitions(dtype, d):
+    """The merge holds 1024 partitions' weights at a time.  Two tokens of each sequence take most of the weight,
+    one in a partition before that and one in a partition past it (and in the last, a shorter one)."""
+    rng = rng_of(94)
+    hq, hkv, bs = 2, 1, 16
+    cache, held, q, tables, ctx = decode_case(rng, [33001, 9, 32769, 32768], hq, hkv, d, bs, dtype)
+    q[:, :, 1] = q[:, :, 0]
+    k8 = held[0]
+    for b, tokens in ((0, (300, 32900)), (2, (32767, 32768)), (3, (5, 32767))):
+        for t in tokens:
+            blk, row = int(tables[b, t // bs]), t % bs
+            one = (q[b, 0, 0].float() * 90 * 64 / d).clamp(-448, 448).to(torch.float8_e4m3fn)
+            cache.k_cache[0][blk, 0, row] = one
+            k8[blk, 0, row] = one.double().cpu().numpy()
+            for s, mine in ((cache.k_scale[0], held[2]), (cache.v_scale[0], held[3])):
+                s[blk, 0] = 2.0 ** -5
+                mine[blk, 0] = 2.0 ** -5
+    want, _ = ref.decode_ref(q[:, 0].double().cpu().numpy(), *held, tables, ctx, 1 / math.sqrt(d))
+    for b, t in ((0, 32900), (0, 300), (2, 32768), (3, 32767)):     # leaving one out would show
+        v = ref.rows_ref(held[1], held[3], tables[b], t + 1)[t, 0]
+        assert np.abs(v).max() > 2 and np.corrcoef(want[b, 0], v)[0, 1] > 0.3
+    got = run_decode(cache, q, tables, ctx, hq, hkv, d, bs, partition_size=32)
+    check_decode(got, held, q, tables, ctx, d, dtype)
+    # half a step of bf16 on outputs below 448 * 2^-5 = 14 is 0.055, and the errors above it are far smaller here; a
+    # token left out, of a weight above 0.3 and a value above 2, moves an output by more than 0.3
+    assert np.abs(got[:, 0].double().cpu().numpy() - want).max() <= 0.1
+    whole = run_decode(cache, q, tables, ctx, hq, hkv, d, bs, partition_size=33024)
+    check_decode(whole, held, q, tables, ctx, d, dtype)
