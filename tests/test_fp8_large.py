@@ -1,5 +1,5 @@
 """The 8-bit cache's kernels at sizes where they take another form: row tiles of 128 with two key groups,
-a longest-first batch, a merge of more than a thousand partitions."""
+a longest-first batch, a merge of more than a thousand partitions, several heads for a wave of the write."""
 
 import math
 
@@ -9,7 +9,7 @@ import torch
 
 from oracle import fp8_cache as ref
 from tests.fp8_tolerance import rounded_weights_bound
-from tests.test_fp8_cache import check_decode, decode_case, gpu, rng_of, run_decode
+from tests.test_fp8_cache import DTYPES, check_decode, check_write, decode_case, fill, gpu, make_cache, rng_of, run_decode
 from tests.test_fp8_prefill import chunk_case, run_chunk
 
 
@@ -155,3 +155,26 @@ def test_decode_over_more_than_1024_partitions(dtype, d):
     assert np.abs(got[:, 0].double().cpu().numpy() - want).max() <= 0.1
     whole = run_decode(cache, q, tables, ctx, hq, hkv, d, bs, partition_size=33024)
     check_decode(whole, held, q, tables, ctx, d, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("count,hkv,d", [(8192, 8, 64), (6600, 5, 128), (9400, 7, 64), (4100, 16, 64)])
+def test_write_of_several_heads_a_wave(dtype, count, hkv, d):
+    """Long writes give a work-group more (head, cache) pairs than it has waves, and a last group of fewer heads;
+    the first block is entered in its middle and holds rows that are rounded again."""
+    rng = rng_of(95)
+    bs = 16
+    assert -(-count // 16) * hkv >= 2048
+    nb = count // bs + 20
+    cache = make_cache(nb, bs, hkv, d, dtype)
+    held = fill(cache, rng)
+    blocks = rng.permutation(nb)
+    pos = np.arange(9, 9 + count)
+    slots = blocks[pos // bs] * bs + pos % bs
+    slots[100] = -1
+    slots[count // 2] = slots[3]                      # among rows of another block: the last token is the one written
+    k, v = (torch.from_numpy(rng.standard_normal((count, hkv, d)) * np.exp2(rng.integers(-4, 8, (count, 1, 1)))
+                             ).to("cuda", DTYPES[dtype]) for _ in range(2))
+    cache.write_kv_slots(0, torch.from_numpy(slots.astype(np.int32)).cuda(), k, v)
+    check_write(cache, held, k, v, slots)
