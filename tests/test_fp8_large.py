@@ -178,3 +178,21 @@ def test_write_of_several_heads_a_wave(dtype, count, hkv, d):
                              ).to("cuda", DTYPES[dtype]) for _ in range(2))
     cache.write_kv_slots(0, torch.from_numpy(slots.astype(np.int32)).cuda(), k, v)
     check_write(cache, held, k, v, slots)
+
+
+@gpu
+def test_calls_repeat_bit_for_bit():
+    """Split contexts, split keys and log-probabilities with ties: no order of arrival shows in the results."""
+    from tinyvllm_amd.sampling import token_logprobs
+    rng = rng_of(96)
+    cache, held, q, tables, ctx = decode_case(rng, [4000, 33, 2900], 8, 2, 128, 16, "bfloat16")
+    rows = torch.from_numpy(rng.integers(0, 40, (20, 70000)).astype(np.float32)).cuda()
+    tokens = torch.arange(20, dtype=torch.int32, device="cuda")
+    chunk_cache, _, cq, table = chunk_case(rng, 21, 3000, 8, 2, 128, 16, "float16")
+
+    def once():
+        return (run_decode(cache, q, tables, ctx, 8, 2, 128, 16, partition_size=128), run_chunk(chunk_cache, cq, table, 3000),
+                *token_logprobs(rows, tokens, 20))
+    first = once()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, once()))
