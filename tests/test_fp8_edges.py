@@ -156,3 +156,30 @@ def test_a_replaced_cache_can_be_released(kind):
     assert jit.graph_for(new, 2, 2) is kept
     kept.run(1)
     torch.cuda.synchronize()
+
+
+def test_rows_are_checked_without_making_tensors():
+    """``write_kv``'s checks run on every call: they look at sizes and strides and create nothing."""
+    import types
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from tinyvllm_amd.kv_cache import KVCache
+    made = []
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, kinds, args=(), kwargs=None):
+            made.append(func)
+            return func(*args, **(kwargs or {}))
+
+    def cache(hkv, d):
+        return types.SimpleNamespace(n_kv_heads=hkv, head_dim=d, dtype=torch.float32, k_cache=[wide])
+    wide = torch.zeros(6, 4, 32)
+    for x, stride in ((wide[:, 1:2], 128), (wide[:1, 1:2], 32), (wide[:0, :2], 64), (wide, 128), (wide[::2], 256),
+                      (wide[2:3], 128), (wide[:, :1, :1], 128), (wide.transpose(0, 1)[:, :1], 32)):
+        hkv, d = x.shape[1:]
+        with Record():
+            assert KVCache._rows(cache(hkv, d), x, "k") == (x, stride)
+    for x in (wide[:1, ::2], wide[:, ::2], wide[:1, :, :16], wide[:, :, ::2], wide[:1, :1, ::2]):
+        hkv, d = x.shape[1:]
+        with pytest.raises(ValueError, match="contiguous"):
+            KVCache._rows(cache(hkv, d), x, "k")
+    assert made == []

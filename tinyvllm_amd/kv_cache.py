@@ -57,10 +57,11 @@ class KVCache:
             raise ValueError(f"{name} dtype {x.dtype} differs from cache dtype {self.dtype}")
         if x.device != self.k_cache[0].device:
             raise ValueError(f"{name} must be on {self.k_cache[0].device}")
-        if x.shape[0] and not x[0].is_contiguous():
+        stride = x.stride()         # a dimension of size 1 may have any
+        if x.shape[0] and ((stride[2] != 1 and self.head_dim > 1) or
+                           (stride[1] != self.head_dim and self.n_kv_heads > 1)):
             raise ValueError(f"{name}: heads and head_dim must be contiguous")
-        stride = x.stride(0) if x.shape[0] > 1 else self.n_kv_heads * self.head_dim
-        return x, stride
+        return x, stride[0] if x.shape[0] > 1 else self.n_kv_heads * self.head_dim
 
     # -- reference API -------------------------------------------------------
     def write_kv(self, layer_idx, block_id, start_offset, k, v):
