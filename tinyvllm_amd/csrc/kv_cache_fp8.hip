@@ -282,7 +282,11 @@ __global__ void __launch_bounds__(256) kv_gather_fp8_kernel(const KVGatherFp8Par
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const f32x4 a = limited<T>(fp8_to_f32x4(w[i][0]) * f[i]), b = limited<T>(fp8_to_f32x4(w[i][1]) * f[i]);
+      f32x4 a = fp8_to_f32x4(w[i][0]) * f[i], b = fp8_to_f32x4(w[i][1]) * f[i];
+      if (f[i] > kSafeScale<T>) {
+        a = limited<T>(a);
+        b = limited<T>(b);
+      }
       T* out = reinterpret_cast<T*>(i ? p.v_out : p.k_out) + idx * 8;
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<f32x4*>(out) = a;
