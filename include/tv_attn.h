@@ -300,7 +300,9 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
  * size the cache may have, any number of blocks and of query heads per KV head;
  * fp16 / bf16 queries (TV_EUNSUPPORTED otherwise), 16-byte aligned rows.  A row
  * that attends a key in a block outside [0, num_blocks), or a NaN in K or V, is
- * NaN in that head; other rows are not touched by it.  workspace: of
+ * NaN in that head; other rows are not touched by it.  K and V enter as values of
+ * dtype: with TV_F16 limited to +-65504 and below 2^-14 rounded to steps of 2^-24,
+ * where tv_paged_decode_fp8 applies the scales in fp32.  workspace: of
  * tv_flash_prefill_paged_fp8_workspace_bytes bytes (0 for grids that fill the
  * device without it; depends on the current device), 16-byte aligned, lets the
  * keys of few rows be split between work-groups; NULL runs them unsplit.

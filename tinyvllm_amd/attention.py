@@ -336,7 +336,9 @@ def paged_decode_attention_fp8(queries, k_cache, v_cache, k_scale, v_scale, bloc
     """``paged_decode_attention`` over an 8-bit cache (one layer's tensors of ``kv_cache.FP8KVCache``; no
     reference counterpart).  queries may be float32, float16 or bfloat16 whatever dtype the cache was
     written from; head_dim 64, 128 or 256, any number of query heads per KV head.  A context of no tokens
-    gives zeros.  ``partition_size`` is a multiple of 32."""
+    gives zeros.  ``partition_size`` is a multiple of 32.  Scales are powers of two of at least 2^-100, as the
+    cache's writes keep them; others are not checked for and give no defined result.  Values of 2^89 and more
+    in magnitude may overflow the fp32 sums of the sequences that attend them."""
     plan = PagedDecodeFP8Plan(queries, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, n_heads,
                               n_kv_heads, head_dim, block_size, max_context_len, partition_size=partition_size,
                               out_dtype=out_dtype)
@@ -348,7 +350,10 @@ def flash_prefill_paged_fp8(queries, k_cache, v_cache, k_scale, v_scale, block_t
     """``flash_prefill_paged`` over an 8-bit cache (one layer's tensors of ``kv_cache.FP8KVCache``; no
     reference counterpart): the chunk's rows attend the cached keys and the chunk's own, all as the
     cache holds them.  fp16 / bf16 queries [1, n, Hq, D] or [n, Hq, D], head_dim 64, 128 or 256, any
-    block size.  Returns [1, n, Hq, D]."""
+    block size.  Returns [1, n, Hq, D].  K, V and the softmax weights enter the products in the queries' dtype:
+    exact for K and V but for the dtype's range (fp16: magnitudes are limited to 65504 and, below 2^-14, rounded
+    to steps of 2^-24, where ``paged_decode_attention_fp8`` has fp32's range).  Scales and large values as
+    there."""
     nb, hkv, bs, d2, index = check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
     _require(index >= 0, "tensors must live on a HIP device")
     check_devices(index, queries, block_table)

@@ -2,17 +2,19 @@
 // layout: tv_fp8.h): query row i at position start_pos + i attends keys j <=
 // start_pos + i (causal) or all start_pos + q_len keys.
 //
-// Bound: the matrix cores, 4 D operations per (row, query head, key), and beside
-// them the vector unit (an exponential per score).  An 8-bit key or value costs a
+// Bound: the matrix cores, 4 D operations per (row, query head, key), and the
+// vector unit (an exponential per score), which two to four waves a SIMD overlap in
+// part only.  An 8-bit key or value costs a
 // conversion more than a 16-bit one, so it is made once per work-group, on the
 // way from registers to LDS, and the work-group's rows are as many as the shape
 // has: the query heads of a KV head are packed into one row index, row r = query
 // r / G of head r % G, so that a chunk of few rows still fills its tiles and all
 // G heads share one conversion.  MI355X, 32 / 8 heads of 128, bf16, 2048 rows after
-// 6144 cached ones: 252 us, 954 TFLOP/s; of these the products and the exponentials
-// alone take 200 and the staging alone 105 (copies of the kernel with the other part
-// taken out): both use LDS, and more of either's overlap was not to be had by
-// offsetting the key groups against each other.
+// 6144 cached ones: 255 us, 942 TFLOP/s, matrix cores busy 38% of the cycles and the
+// vector unit 41%; the products and the exponentials alone take 200 and the staging
+// alone 105 (copies of the kernel with the other part taken out): both use LDS, and
+// more of either's overlap was not to be had by offsetting the key groups against
+// each other.
 //
 // A work-group of 4 waves owns BM = 64 RB rows of one KV head, RB blocks of 16 a
 // wave, and walks tiles of BN keys: S^T = K Q^T with the key rows as operand A;
@@ -25,7 +27,12 @@
 // (values are limited to T's largest number; below fp16's normal numbers they are
 // rounded as fp16 inputs that small are).  Scores, maxima, sums, accumulators are
 // fp32; a weight is rounded to T for the second product, as in the 16-bit prefill
-// kernels, and the row sum is that of the rounded weights.
+// kernels, and the row sum is that of the rounded weights.  That rounding is the
+// largest error beside the output's own: against 64 bits 2.3e-3 in bf16 and 2.7e-4
+// in fp16, with weights of two parts 1.7e-3 and 2.1e-4, the output's rounding alone.
+// Two parts (as the decode kernel has, where bytes leave the time for them) cost a
+// quarter: 322 against 257 us for the rows above, 36.7 against 28.4 for 512 fp16
+// rows of 64-wide heads after 3584.
 // A NaN in a key or value and a block id outside the cache show in the rows that
 // attend that key and in no others: the key's score becomes NaN, which the mask
 // replaces for rows that do not see it, and a NaN value is zero in LDS, since a
@@ -484,10 +491,11 @@ template <typename T> void launch_dims(const PrefillFp8Params& p, int head_dim, 
 
 // 128-row work-groups of two key groups (8 waves) where they give nearly every CU
 // one, else 64 rows and four key groups (16 waves).  A CU holds one of either.
-// MI355X, bf16, 32 / 8 heads of 128, us: 1024 rows after 4000 cached ones (256
-// tiles of 128) 92 / 107 (64 rows), with one group of 4 waves 132; 512 after 2000 43
-// / 34; 2048 after 6144 250, with one group 256; 32 / 4 heads of 64, 512 after 3584
-// 38 / 34, with two groups of 64 rows 40.
+// MI355X, bf16, us, 128 rows / 64 rows: 32 / 8 heads of 128, 1024 rows after 4000
+// cached ones (256 tiles of 128) 94 / 109, with 128 rows in one group of 4 waves 134;
+// 512 after 2000 50 / 33; 2048 after 6144 255 / 322, in one group 252; 32 / 4 heads of
+// 64, 512 after 3584 46 / 28, with two groups of 64 rows 37.  Heads of 256 have 64
+// rows and one group: 512 after 3584 (32 / 8) 125, 2048 after 6144 690 (697 TFLOP/s).
 bool wide_rows(long long rows, int num_kv_heads, int head_dim, int cus) {
   return head_dim != 256 && (rows + 127) / 128 * num_kv_heads * 8 >= 7LL * cus;
 }

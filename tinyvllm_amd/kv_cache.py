@@ -127,8 +127,9 @@ class FP8KVCache:
     (float32); an element stands for number * scale.  ``dtype`` is the model's: rows are written from it
     and read back in it.  A block's scale fits the rows written so far: writing its row 0 starts it
     anew (rows that the call does not write become zero), and a later row that needs a larger scale has
-    the rows before it rounded again.  NaN and infinite elements are stored as NaN.  head_dim 64, 128
-    or 256, block_size at most 1024.
+    the rows before it rounded again.  (A ``KVCache`` takes a block's rows in any order; here row 0 comes
+    first.)  NaN and infinite elements are stored as NaN; values read back are limited to ``dtype``'s largest
+    finite number.  head_dim 64, 128 or 256, block_size at most 1024.
     """
 
     def __init__(self, num_layers, num_blocks, block_size, n_kv_heads, head_dim, dtype, device="cuda"):
