@@ -154,8 +154,10 @@ typedef struct tv_llama_model {
 /*
  * Paged K/V caches: host arrays of n_layers device pointers [num_blocks, block_size, Hkv, D] of the model
  * dtype (k_scales and v_scales NULL), or 8-bit caches (tv_attn.h): e4m3 numbers [num_blocks, Hkv,
- * block_size, D] with scales [num_blocks, Hkv].  Over an 8-bit cache head_dim is 64, 128 or 256, a decode
- * step's partition_size a multiple of 32, and a sequence of context 0 attends to nothing.
+ * block_size, D] with scales [num_blocks, Hkv].  Over an 8-bit cache head_dim is 64, 128 or 256, block_size
+ * at most 1024, a decode step's partition_size a multiple of 32, and a chunk of fp32 rows that attends the
+ * prefix at most 65535 tokens (anything else is refused before the first launch); a sequence of context 0
+ * attends to nothing.
  */
 typedef struct tv_llama_cache {
   void* const* k_caches;

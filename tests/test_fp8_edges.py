@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from tests.test_fp8_cache import DTYPES, gpu, make_cache, rng_of
+from tests.test_fp8_cache import DTYPES, check_decode, decode_case, gpu, make_cache, rng_of, run_decode
 from tests.test_fp8_llama import build
 from tests.test_fp8_prefill import check_chunk, chunk_case, run_chunk
 
@@ -183,3 +183,24 @@ def test_rows_are_checked_without_making_tensors():
         with pytest.raises(ValueError, match="contiguous"):
             KVCache._rows(cache(hkv, d), x, "k")
     assert made == []
+
+
+@gpu
+@pytest.mark.parametrize("spread", [2.0 ** -80, 2.0 ** 75])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_attention_over_values_of_any_defined_size(dtype, spread):
+    """V of 2^-80 to 2^84 (the sums are defined below 2^89): results scale with it."""
+    rng = rng_of(81)
+    hq, hkv, d, bs = 8, 2, 64, 16
+    cache, held, q, tables, ctx = decode_case(rng, [700, 33, 64], hq, hkv, d, bs, dtype)
+    cache.v_scale[0].mul_(spread)
+    for part in (None, 64):
+        got = run_decode(cache, q, tables, ctx, hq, hkv, d, bs, partition_size=part, out_dtype=torch.float32)
+        check_decode(got.double() / spread, held, q, tables, ctx, d, dtype, "float32")
+    if dtype == "float32":
+        return                                        # chunks are of 16-bit queries
+    for n, start in ((40, 90), (9, 2100)):            # unsplit and split keys
+        cache, held, q, table = chunk_case(rng, n, start, hq, hkv, d, bs, dtype)
+        cache.v_scale[0].mul_(spread)
+        got = run_chunk(cache, q, table, start, out_dtype=torch.float32)
+        check_chunk(got.double() / spread, held, q, table, start, dtype, out_dtype="float32")
