@@ -1,4 +1,4 @@
-"""ctypes binding of libtvattn.so (declarations: include/tv_attn.h, include/tv_llama.h).
+"""ctypes binding of libtvattn.so (declarations: include/tv_attn.h, tv_draft.h, tv_llama.h).
 
 The library is required: importing the ops without it raises immediately, and
 there is no CPU or PyTorch fallback for any op.
@@ -15,7 +15,7 @@ LIB_PATH = Path(os.environ.get("TV_ATTN_LIB", _PKG / "libtvattn.so"))
 TV_F32, TV_F16, TV_BF16 = 0, 1, 2
 TV_OK, TV_EINVAL, TV_EUNSUPPORTED, TV_EHIP = 0, 1, 2, 3
 
-# name -> (restype, argtypes); mirrors include/tv_attn.h, tv_llama.h and tv_bench.h
+# name -> (restype, argtypes); mirrors include/tv_attn.h, tv_draft.h, tv_llama.h and tv_bench.h
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
@@ -47,6 +47,17 @@ SIGNATURES = {
     "tv_flash_prefill_paged_fp8_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
     "tv_flash_prefill_paged_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _L, _L, _I, _F, _I,
                                         _I, _P, _S, _P]),
+    # include/tv_draft.h
+    "tv_draft_tree_layout": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "tv_rope_and_cache": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _L, _L,
+                               _I, _P, _P]),
+    "tv_paged_tree_workspace_bytes": (_S, [_I, _I, _I, _I, _I, _I, _I]),
+    "tv_paged_tree_partition_size": (_I, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "tv_paged_tree": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _F, _I, _I,
+                           _I, _P, _S, _P]),
+    "tv_verify_draft_tree_workspace_bytes": (_S, [_I, _I, _I, _I]),
+    "tv_verify_draft_tree": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _I, _P, _S, _P]),
+    "tv_keep_draft_rows": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     # include/tv_llama.h
     "tv_linear_k_split": (_I, [_I, _I, _I]),
     "tv_linear_kernel": (_I, [_I, _I, _I, _I, _I, _I]),
@@ -68,7 +79,7 @@ SIGNATURES = {
     # include/tv_bench.h
     "tv_stream_read": (_I, [_P, _L, _I, _I, _I, _I, _P, _P]),
 }
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 _lib = None
 

@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .draft_tree import MAX_NODES, check_block_tables, check_tree_tensors
 from .kv_cache import check_devices, check_fp8_cache
 
 _lib.load()
@@ -379,6 +380,83 @@ def flash_prefill_paged_fp8(queries, k_cache, v_cache, k_scale, v_scale, block_t
               _lib.dtype_code(queries.dtype), _lib.dtype_code(out_dtype), ws.data_ptr() if ws is not None else None,
               ws_bytes)
     return out
+
+
+class PagedTreePlan:
+    """Attention of drafted tokens, a tree of them for every sequence, over the paged cache (no reference
+    counterpart), checked once and pointer-stable: ``run()`` is one C call without an allocation, which a HIP graph
+    can capture.
+
+    queries [B, T, Hq, D], rotated, any strides between sequences and nodes; k_cache / v_cache [NB, bs, Hkv, D] of
+    their dtype, the nodes' own K/V at positions context + i; block_tables [B, columns], context_lens [B] (tokens before
+    the tree) and tree_lens [B] int32; tree_mask [B, T, ceil(T / 64)] int64 as ``draft_tree.draft_tree_layout`` makes
+    it, or [T, ceil(T / 64)] for one shape of tree.  Node i attends all context tokens and the nodes t < tree_lens
+    whose bit its mask has (any mask; its own bit is not implied).  Nodes at tree_lens and beyond, and nodes that see
+    nothing, get zeros.  A block id outside the cache, a NaN in a key, a score of +inf, or a NaN or infinity in a value
+    spoils the nodes that see it and no others; a score of -inf has weight 0.  head_dim 64, 128 or 256, T at most 256, any block size.
+    ``max_context_len`` (context and tree) trims the table; ``partition_size``, a multiple of 64, is the number of keys a
+    work-group takes.  The tensors are read on every ``run()`` and must keep their storage.
+    """
+
+    def __init__(self, queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask,
+                 n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, partition_size=None, out_dtype=None):
+        index = k_cache.get_device()
+        _require(index >= 0, f"tensors must live on a HIP device (got {k_cache.device})")
+        check_devices(index, queries, v_cache, tree_mask)
+        _require(queries.dim() == 4, f"queries must be [B, T, Hq, D], got {tuple(queries.shape)}")
+        b, t, hq, d = queries.shape
+        _require(hq == n_heads and d == head_dim, "queries shape does not match n_heads/head_dim")
+        _require(1 <= t <= MAX_NODES, f"T must be 1 to {MAX_NODES}, got {t}")
+        qs = queries.stride()
+        _require(qs[3] == 1 and (qs[2] == d or hq == 1), "queries: heads and head_dim must be contiguous")
+        _require(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.is_contiguous() and
+                 v_cache.is_contiguous(), "k_cache / v_cache must be dense [NB, bs, Hkv, D] tensors of one shape")
+        nb, bs, hkv, d2 = k_cache.shape
+        _require((bs, hkv, d2) == (block_size, n_kv_heads, head_dim),
+                 f"cache shape {tuple(k_cache.shape)} does not match block_size/n_kv_heads/head_dim")
+        _require(n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
+        _require(queries.dtype == k_cache.dtype == v_cache.dtype, "queries and caches must share a dtype")
+        check_block_tables(index, b, block_tables)
+        check_tree_tensors(index, b, t, context_lens=context_lens, tree_lens=tree_lens)
+        words = (t + 63) // 64
+        _require(tree_mask.dtype == torch.int64 and tuple(tree_mask.shape) in ((b, t, words), (t, words)) and
+                 tree_mask.is_contiguous(), f"tree_mask must be contiguous int64 [{b}, {t}, {words}] or [{t}, {words}]")
+        mb = block_tables.shape[1]
+        used = mb if max_context_len is None else min((int(max_context_len) + block_size - 1) // block_size, mb)
+        _require(used > 0, "no block table columns to attend over")
+        code = _lib.dtype_code(queries.dtype)
+        if partition_size is None:
+            partition_size = _lib.device_size("tv_paged_tree_partition_size", index, max(b, 1), t, n_heads, n_kv_heads,
+                                              head_dim, used, block_size, code)
+            _require(partition_size > 0, f"head_dim {head_dim} or this table width is not supported")
+        self.partition_size = int(partition_size)
+        self.index = index
+        out_dtype = queries.dtype if out_dtype is None else out_dtype
+        self.out = torch.empty((b, t, n_heads, head_dim), dtype=out_dtype, device=queries.device)
+        self.ws_bytes = _lib.device_size("tv_paged_tree_workspace_bytes", index, b, t, n_heads, head_dim, used,
+                                         block_size, self.partition_size)
+        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=queries.device) if self.ws_bytes else None
+        self._inputs = (queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask)
+        self.args = (self.out.data_ptr(), queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                     block_tables.data_ptr(), context_lens.data_ptr(), tree_lens.data_ptr(), tree_mask.data_ptr(),
+                     1 if tree_mask.dim() == 2 else 0, b, t, n_heads, n_kv_heads, head_dim, block_size, nb, mb, used,
+                     qs[0] if b > 1 else t * hq * d, qs[1] if t > 1 else hq * d, 1.0 / math.sqrt(head_dim), code,
+                     _lib.dtype_code(out_dtype), self.partition_size, self.ws.data_ptr() if self.ws is not None else None,
+                     self.ws_bytes)
+
+    def run(self):
+        _lib.call("PagedTreePlan.run", self.index, _lib.load().tv_paged_tree, *self.args)
+        return self.out
+
+
+def paged_tree_attention(queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask,
+                         n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, partition_size=None,
+                         out_dtype=None):
+    """Attention of drafted tokens over the paged cache and each other; see ``PagedTreePlan``.  Returns
+    [B, T, Hq, D] in ``out_dtype`` (default: the query dtype)."""
+    return PagedTreePlan(queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask, n_heads,
+                         n_kv_heads, head_dim, block_size, max_context_len, partition_size=partition_size,
+                         out_dtype=out_dtype).run()
 
 
 class PrefillPlan:

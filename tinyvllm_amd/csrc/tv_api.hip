@@ -132,7 +132,7 @@ int decode_scratch(void** ptr) {
 
 extern "C" {
 
-int tv_abi_version(void) { return 10; }
+int tv_abi_version(void) { return 11; }
 
 const char* tv_last_error(void) { return tv::last_error(); }
 

@@ -6,10 +6,13 @@ sits at ((blk*bs + t)*Hkv + h)*D + d, the layout paged_decode_attention reads.
 All writes and reads go through libtvattn.so kernels.
 """
 
+import ctypes
+
 import numpy as np
 import torch
 
 from . import _lib
+from .draft_tree import check_block_tables, check_tree_tensors
 
 _lib.load()
 
@@ -117,6 +120,17 @@ class KVCache:
         """
         return reshape_and_cache(self.k_cache[layer_idx], self.v_cache[layer_idx], k, v,
                                  slot_mapping, err_count=err_count)
+
+    def write_rope_slots(self, layer_idx, slot_mapping, positions, rope, q, k, v, *, pairs="adjacent", out=None,
+                         err_count=None):
+        """``write_kv_slots`` of keys that are rotated on the way; returns the rotated queries.  See
+        ``rope_and_cache``."""
+        return rope_and_cache(self.k_cache[layer_idx], self.v_cache[layer_idx], q, k, v, slot_mapping, positions, rope,
+                              pairs=pairs, out=out, err_count=err_count)
+
+    def keep_draft_path(self, path, counts, context_lens, block_tables):
+        """Moves an accepted path's K/V to where the sequences go on, in all layers; see ``keep_draft_rows``."""
+        keep_draft_rows(self.k_cache, self.v_cache, path, counts, context_lens, block_tables)
 
 
 class FP8KVCache:
@@ -289,3 +303,106 @@ def reshape_and_cache(k_cache, v_cache, k, v, slot_mapping, err_count=None):
         _lib.dtype_code(k_cache.dtype), err_count.data_ptr() if err_count is not None else None,
         _lib.stream_ptr(dev))
     _lib.check(rc, "reshape_and_cache")
+
+
+def _token_stride(x, heads, d, name):
+    """Elements between the tokens of x [N, heads, d]; raises unless a token's heads are dense."""
+    if x.dim() != 3 or tuple(x.shape[1:]) != (heads, d):
+        raise ValueError(f"{name} must be [N, {heads}, {d}], got {list(x.shape)}")
+    stride = x.stride()                 # a dimension of size 1 may have any
+    if (stride[2] != 1 and d > 1) or (stride[1] != d and heads > 1):
+        raise ValueError(f"{name}: heads and head_dim must be contiguous")
+    if x.shape[0] > 1 and stride[0] < heads * d:
+        raise ValueError(f"{name}: tokens overlap")
+    return stride[0] if x.shape[0] > 1 else heads * d
+
+
+def rope_and_cache(k_cache, v_cache, q, k, v, slot_mapping, positions, rope, *, pairs="adjacent", out=None,
+                   err_count=None):
+    """Rotates queries and keys to their positions and writes keys and values into the cache, in one launch
+    (no reference counterpart as one call: apply_rope, llama.py:34-55, then the writes of llama.py:188-209).
+
+    q [N, Hq, D], k / v [N, Hkv, D] of the cache's dtype, rows possibly strided (views of one projection);
+    slot_mapping and positions [N] int32 (or [B, T] with B * T = N); rope [P, R / 2, 2] float32, cos and sin of
+    each pair by position (``Llama.rope``).  The first R elements of a head are rotated, pairs (2i, 2i + 1), or with
+    ``pairs="halves"`` (i, i + R / 2); the others stay as they are.  Returns the rotated queries [N, Hq, D], in
+    ``out`` where it is given (which may be q).
+
+    A negative slot is padding: its K/V are not written.  A slot past the cache is not written and counted
+    in ``err_count`` (int32/uint32 device scalar); nor is a token whose position the table does not hold,
+    whose queries become NaN.  The slots of a call differ from each other.
+    """
+    index = k_cache.get_device()
+    if index < 0:
+        raise ValueError(f"the cache must be on a HIP device (got {k_cache.device})")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache / v_cache must be dense [NB, bs, Hkv, D] tensors of one shape")
+    nb, bs, hkv, d = k_cache.shape
+    if q.dim() != 3:
+        raise ValueError(f"q must be [N, Hq, {d}], got {list(q.shape)}")
+    n, hq = q.shape[:2]
+    strides = [_token_stride(x, h, d, name) for x, h, name in ((q, hq, "q"), (k, hkv, "k"), (v, hkv, "v"))]
+    if k.shape[0] != n or v.shape[0] != n:
+        raise ValueError("q, k and v must hold the same number of tokens")
+    dtype = k_cache.dtype
+    if not (v_cache.dtype == q.dtype == k.dtype == v.dtype == dtype):
+        raise ValueError("q, k, v and the caches must share a dtype")
+    for x, name in ((slot_mapping, "slot_mapping"), (positions, "positions")):
+        if x.dtype != torch.int32 or x.numel() != n or not x.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 with one entry per token")
+    if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous():
+        raise ValueError("rope must be contiguous float32 [positions, pairs, 2]")
+    if not 1 <= 2 * rope.shape[1] <= d or rope.shape[0] < 1:
+        raise ValueError(f"rope of {rope.shape[1]} pairs does not fit head_dim {d}")
+    if pairs not in ("adjacent", "halves"):
+        raise ValueError(f"pairs must be 'adjacent' or 'halves', got {pairs!r}")
+    check_devices(index, v_cache, q, k, v, slot_mapping, positions, rope)
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=dtype, device=q.device)
+    elif out.dtype != dtype or tuple(out.shape) != (n, hq, d) or out.get_device() != index:
+        raise ValueError("out must be like q")
+    out_stride = _token_stride(out, hq, d, "out")
+    if err_count is not None and (err_count.get_device() != index or
+                                  err_count.dtype not in (torch.int32, torch.uint32)):
+        raise ValueError("err_count must be an int32/uint32 tensor on the cache's device")
+    _lib.call("rope_and_cache", index, _lib.load().tv_rope_and_cache,
+              out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              slot_mapping.data_ptr(), positions.data_ptr(), rope.data_ptr(), rope.shape[0], 2 * rope.shape[1],
+              1 if pairs == "halves" else 0, n, hq, hkv, d, bs, nb, out_stride, *strides, _lib.dtype_code(dtype),
+              err_count.data_ptr() if err_count is not None else None)
+    return out
+
+
+def keep_draft_rows(k_caches, v_caches, path, counts, context_lens, block_tables):
+    """Moves the K/V of a verified tree's accepted nodes to where their sequences go on, in every layer's cache
+    [NB, bs, Hkv, D]: position context + path[j] -> context + j for j < count, in one launch per 64 layers (no
+    reference counterpart).
+
+    path [B, T], counts and context_lens [B] int32 (``sampling.verify_draft_tree``; the context before the
+    tree), block_tables [B, columns] int32.  ``path`` rises from node to node.  Entries outside j .. T - 1 and
+    positions that the table does not reach, or whose block is outside the cache, are not moved.  Other rows stay as
+    they are.
+    """
+    if len(k_caches) != len(v_caches) or not k_caches:
+        raise ValueError("k_caches and v_caches must hold one tensor per layer each")
+    first = k_caches[0]
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"the caches must be on a HIP device (got {first.device})")
+    if first.dim() != 4:
+        raise ValueError("caches must be dense [NB, bs, Hkv, D] tensors")
+    for c in (*k_caches, *v_caches):
+        if c.shape != first.shape or c.dtype != first.dtype or not c.is_contiguous():
+            raise ValueError("caches must be dense tensors of one shape and dtype")
+    check_devices(index, *k_caches, *v_caches)
+    if path.dim() != 2 or path.shape[1] < 1:
+        raise ValueError(f"path must be [B, T], got {list(path.shape)}")
+    b, t = path.shape
+    check_tree_tensors(index, b, t, path=path, counts=counts, context_lens=context_lens)
+    check_block_tables(index, b, block_tables)
+    nb, bs, hkv, d = first.shape
+    n = len(k_caches)
+    arrays = [(ctypes.c_void_p * n)(*[c.data_ptr() for c in cs]) for cs in (k_caches, v_caches)]
+    _lib.call("keep_draft_rows", index, _lib.load().tv_keep_draft_rows, *arrays, n, path.data_ptr(), counts.data_ptr(),
+              context_lens.data_ptr(), block_tables.data_ptr(), b, t, block_tables.shape[1], hkv, d, bs, nb,
+              _lib.dtype_code(first.dtype))
