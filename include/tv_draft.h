@@ -78,21 +78,22 @@ int tv_rope_and_cache(void* q_out, void* k_cache, void* v_cache, const void* q, 
  * ceil(nodes/64)], or with mask_shared != 0 one [nodes, ceil(nodes/64)] for all.
  * out [num_seqs, nodes, num_heads, head_dim] of dtype or TV_F32 (out_dtype).
  * head_dim 64, 128 or 256; any block size; any number of query heads per KV head.
- * partition_size: keys of a work-group, a positive multiple of 64; longer sequences are
- * split and their parts joined through `workspace` (16-byte aligned, of
- * tv_paged_tree_workspace_bytes bytes, one per launch that may overlap).
+ * work_groups: 0 gives every (sequence, KV head, tile of rows) a work-group.  n > 0 deals
+ * the keys of all of them evenly to n work-groups by the lengths on the device, and joins what
+ * that cuts through `workspace` (16-byte aligned, of tv_paged_tree_workspace_bytes bytes,
+ * one per launch that may overlap); results then depend on the batch in their last digits.
  */
-size_t tv_paged_tree_workspace_bytes(int num_seqs, int nodes, int num_heads, int head_dim, int max_blocks,
-                                     int block_size, int partition_size);
-/* Partition size for the current device; 0: bad arguments. */
-int tv_paged_tree_partition_size(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim,
-                                 int max_blocks, int block_size, int dtype);
+size_t tv_paged_tree_workspace_bytes(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim, int dtype,
+                                     int work_groups);
+/* work_groups for the current device; negative: bad arguments. */
+int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim, int max_blocks,
+                              int block_size, int dtype);
 int tv_paged_tree(void* out, const void* queries, const void* k_cache, const void* v_cache,
                   const int32_t* block_tables, const int32_t* context_lens, const int32_t* tree_lens,
                   const uint64_t* mask, int mask_shared, int num_seqs, int nodes, int num_heads, int num_kv_heads,
                   int head_dim, int block_size, int num_blocks, int block_table_stride, int max_blocks,
                   int64_t q_seq_stride, int64_t q_node_stride, float scale, int dtype, int out_dtype,
-                  int partition_size, void* workspace, size_t workspace_bytes, void* stream);
+                  int work_groups, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The path through a tree that the model's logits accept.

@@ -16,7 +16,7 @@ from tests.test_draft_tree import DTYPES, cuda, gpu, random_tables, random_tree,
 def test_entry_point_validates_on_the_host():
     from tinyvllm_amd import _lib
     lib, p = _lib.load(), ctypes.c_void_p(256)
-    base = [p] * 8 + [0, 4, 8, 8, 2, 64, 16, 20, 8, 8, 4096, 512, 0.1, 1, 1, 128, None, 0, None]
+    base = [p] * 8 + [0, 4, 8, 8, 2, 64, 16, 20, 8, 8, 4096, 512, 0.1, 1, 1, 0, None, 0, None]
 
     def call(**kw):
         a = list(base)
@@ -38,14 +38,15 @@ def test_entry_point_validates_on_the_host():
     assert call(_14=1 << 10, _15=1 << 11, _16=1 << 21, _17=1 << 21) == _lib.TV_EINVAL and b"too large" in lib.tv_last_error()
     assert call(_18=4097) == _lib.TV_EINVAL and call(_19=504) == _lib.TV_EINVAL and b"strides" in lib.tv_last_error()
     assert call(_21=3) == _lib.TV_EINVAL and call(_22=2) == _lib.TV_EINVAL and b"dtype" in lib.tv_last_error()
-    for size in (0, -64, 96):
-        assert call(_23=size) == _lib.TV_EINVAL and b"multiple of 64" in lib.tv_last_error()
+    for n in (-1, (1 << 16) + 1):
+        assert call(_23=n) == _lib.TV_EINVAL and b"work_groups" in lib.tv_last_error()
     assert call(_23=64) == _lib.TV_EINVAL and b"workspace" in lib.tv_last_error()
     assert call(_23=64, _24=ctypes.c_void_p(264), _25=1 << 30) == _lib.TV_EINVAL and b"16-byte" in lib.tv_last_error()
-    assert call(_9=65535, _10=256, _23=64, _24=p, _25=1 << 60) == _lib.TV_EINVAL and b"grid" in lib.tv_last_error()
-    assert lib.tv_paged_tree_workspace_bytes(4, 8, 8, 64, 8, 16, 128) == 0
-    assert lib.tv_paged_tree_workspace_bytes(4, 8, 8, 64, 8, 16, 64) == 2 * 4 * 8 * 8 * 66 * 4
-    assert lib.tv_paged_tree_partition_size(4, 8, 7, 2, 64, 8, 16, 1) == 0
+    assert call(_9=65535, _10=256, _11=256, _19=16384) == _lib.TV_EINVAL and b"grid" in lib.tv_last_error()
+    assert lib.tv_paged_tree_workspace_bytes(4, 8, 8, 2, 64, 1, 0) == 0
+    need = lib.tv_paged_tree_workspace_bytes(4, 8, 8, 2, 64, 1, 64)
+    assert need > 0 and call(_23=64, _24=p, _25=need - 1) == _lib.TV_EINVAL and b"workspace" in lib.tv_last_error()
+    assert lib.tv_paged_tree_work_groups(4, 8, 7, 2, 64, 8, 16, 1) < 0
 
 
 def test_python_refuses_tensors_on_the_cpu():
@@ -139,18 +140,19 @@ def test_any_mask(dtype, d):
     rng = rng_of(d)
     case = Case(rng, dtype, 4, 2, d, 16, [70, 70, 41, 3], [0, 129, 0, 64], 70, trees=False)
     case.check(case.run())
-    case.check(case.run(partition_size=64))
+    case.check(case.run(work_groups=11))
     case.check(case.run(out_dtype=torch.float32), out_dtype="float32")
 
 
 @gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
-@pytest.mark.parametrize("size", [64, 128, 192, 512, 4096])
-def test_partitions(dtype, size):
-    """Sequences of no, one and many parts in one launch; parts that hold only keys some nodes do not see."""
-    rng = rng_of(size)
+@pytest.mark.parametrize("size", [1, 2, 7, 8, 33, 64, 500])
+def test_work_groups(dtype, size):
+    """Sequences of no, one and many parts in one launch; work-groups with many units, with a part of one and with
+    nothing; parts that hold only keys some nodes do not see."""
+    rng = rng_of(size + 100)
     case = Case(rng, dtype, 8, 2, 128, 16, [40, 40, 40, 0, 7], [0, 64, 500, 300, 1100], 40)
-    case.check(case.run(partition_size=size))
+    case.check(case.run(work_groups=size))
 
 
 @gpu
@@ -159,7 +161,7 @@ def test_long_context(dtype):
     rng = rng_of(77)
     case = Case(rng, dtype, 8, 2, 64, 16, [12, 9], [20011, 3000], 12)
     case.check(case.run())
-    case.check(case.run(partition_size=20224))
+    case.check(case.run(work_groups=0))
 
 
 @gpu
@@ -169,7 +171,7 @@ def test_large_scores(dtype):
     rng = rng_of(78)
     case = Case(rng, dtype, 4, 2, 128, 16, [20, 20], [700, 50], 20, scale=40.0)
     case.check(case.run())
-    case.check(case.run(partition_size=128))
+    case.check(case.run(work_groups=10))
 
 
 @gpu
@@ -206,14 +208,14 @@ def test_one_token_is_paged_decode():
 
 @gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
-@pytest.mark.parametrize("size", [None, 64])
+@pytest.mark.parametrize("size", [0, 9])
 def test_tables_that_end_before_the_sequence(dtype, size):
     """Positions past the table, or past max_context_len's columns, do not exist."""
     rng = rng_of(81)
     case = Case(rng, dtype, 4, 2, 64, 16, [20, 20, 20], [30, 200, 85], 20)
     case.table = np.ascontiguousarray(case.table[:, :6])
-    case.check(case.run(partition_size=size))
-    case.check(case.run(partition_size=size, max_context_len=50), width=64)
+    case.check(case.run(work_groups=size))
+    case.check(case.run(work_groups=size, max_context_len=50), width=64)
 
 
 @gpu
@@ -227,14 +229,14 @@ def test_lengths_out_of_range_are_clamped():
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("where", ["k", "v"])
-@pytest.mark.parametrize("size", [None, 64])
+@pytest.mark.parametrize("size", [0, 9])
 def test_values_that_are_not_finite(dtype, value, where, size):
     """Behind the tree and in other sequences' rows they reach nothing; in a drafted token's row the nodes that see
     it, in a context row every node.  An infinite key element times a query element of the other sign is a score of
     -inf, whose weight is 0 by the definition: those rows stay finite."""
     rng = rng_of(83)
     case = Case(rng, dtype, 8, 2, 64, 16, [11, 20], [70, 10], 20)
-    clean = case.run(partition_size=size)
+    clean = case.run(work_groups=size)
     cache = case.k if where == "k" else case.v
 
     def row(b, pos):
@@ -242,9 +244,9 @@ def test_values_that_are_not_finite(dtype, value, where, size):
 
     row(0, 70 + 11)[:] = value                        # past the tree, in its tile
     row(0, 70 + 19)[:] = value
-    assert torch.equal(case.run(partition_size=size), clean)
+    assert torch.equal(case.run(work_groups=size), clean)
     row(0, 70 + 3)[1, 5] = value                      # node 3, KV head 1
-    got = case.run(partition_size=size)
+    got = case.run(work_groups=size)
     sees = torch.from_numpy(case.seen[0][:, 3].copy()).cuda() & (torch.arange(20, device="cuda") < 11)
     assert torch.equal(got[1], clean[1]) and torch.equal(got[0][:, :4], clean[0][:, :4])
     assert torch.equal(got[0][~sees], clean[0][~sees])
@@ -254,21 +256,21 @@ def test_values_that_are_not_finite(dtype, value, where, size):
 
     assert torch.equal(got[0][sees][:, 4:].isnan().any(2), spoilt(case.q[0][sees][:, 4:, 5]))
     row(0, 40)[0, 9] = value                          # context, KV head 0
-    got = case.run(partition_size=size)
+    got = case.run(work_groups=size)
     assert torch.equal((~got[0, :11, :4].isfinite()).any(2), spoilt(case.q[0, :11, :4, 9])) and torch.equal(got[1], clean[1])
 
 
 @gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
-@pytest.mark.parametrize("size", [None, 64])
+@pytest.mark.parametrize("size", [0, 9])
 def test_block_ids_outside_the_cache(dtype, size):
     """NaN in the nodes that see the block, and nowhere else."""
     rng = rng_of(84)
     case = Case(rng, dtype, 4, 2, 128, 16, [20, 20, 20], [70, 60, 5], 20)
-    clean = case.run(partition_size=size)
+    clean = case.run(work_groups=size)
     case.table[0, 1] = case.pool                      # context
     case.table[1, 4] = -1                             # positions 64 .. 79: nodes 4 .. 19
-    got = case.run(partition_size=size)
+    got = case.run(work_groups=size)
     assert got[0].isnan().all() and torch.equal(got[2], clean[2])
     sees = torch.from_numpy(case.seen[1][:, 4:].any(1)).cuda()
     assert got[1][sees].isnan().all() and torch.equal(got[1][~sees], clean[1][~sees])
@@ -293,15 +295,17 @@ def test_queries_of_padding_are_not_looked_at():
 def test_results_repeat_and_do_not_depend_on_the_batch():
     rng = rng_of(86)
     case = Case(rng, "bfloat16", 8, 2, 128, 16, [16] * 5, [900, 40, 333, 0, 1200], 16)
-    a = case.run(partition_size=256)
-    for _ in range(3):
-        assert torch.equal(case.run(partition_size=256), a)
+    for size in (0, 24):
+        a = case.run(work_groups=size)
+        for _ in range(3):
+            assert torch.equal(case.run(work_groups=size), a)
+    a = case.run(work_groups=0)
     one = Case.__new__(Case)
     one.__dict__ = dict(case.__dict__)
     for name in ("lens", "ctx", "table", "mask"):
         setattr(one, name, getattr(case, name)[2:3])
     one.q = case.q[2:3]
-    assert torch.equal(one.run(partition_size=256), a[2:3])
+    assert torch.equal(one.run(work_groups=0), a[2:3])
 
 
 @gpu
@@ -311,7 +315,7 @@ def test_plans_in_graphs_follow_their_inputs():
     rng = rng_of(87)
     case = Case(rng, "float16", 8, 2, 64, 16, [20] * 4, [600] * 4, 20)
     bufs = list(case.args())
-    plans = [PagedTreePlan(*bufs, partition_size=size) for size in (128, 1024)]
+    plans = [PagedTreePlan(*bufs, work_groups=size) for size in (20, 0)]
     for p in plans:
         p.run()
     torch.cuda.synchronize()
@@ -338,14 +342,14 @@ def test_plans_in_graphs_follow_their_inputs():
 def test_two_streams_at_once():
     rng = rng_of(88)
     cases = [Case(rng, "bfloat16", 8, 2, 128, 16, [30, 12], [900, 2000], 30) for _ in range(2)]
-    want = [c.run(partition_size=256) for c in cases]
+    want = [c.run(work_groups=40) for c in cases]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in cases]
     got = [[], []]
     for _ in range(5):
         for i, c in enumerate(cases):
             with torch.cuda.stream(streams[i]):
-                got[i].append(c.run(partition_size=256))
+                got[i].append(c.run(work_groups=40))
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
@@ -378,7 +382,7 @@ def test_python_refusals_on_the_gpu():
         args[at] = bad
         with pytest.raises(ValueError, match=what):
             paged_tree_attention(*args)
-    for kw, what in (({"partition_size": 32}, "multiple of 64"), ({"max_context_len": 0}, "columns"),
+    for kw, what in (({"work_groups": -1}, "work_groups"), ({"max_context_len": 0}, "columns"),
                      ({"out_dtype": torch.bfloat16}, "dtype")):
         with pytest.raises(ValueError, match=what):
             paged_tree_attention(*good, **kw)
@@ -398,5 +402,5 @@ def test_random_trees(case):
     block = int(rng.choice([1, 3, 8, 16, 16, 32, 64, 100]))
     c = Case(rng, str(rng.choice(sorted(DTYPES))), hq, hkv, d, block, rng.integers(0, nodes + 1, b),
              rng.integers(0, int(rng.choice([2, 80, 700])), b), nodes, trees=bool(rng.integers(2)))
-    size = rng.choice([0, 64, 256])
-    c.check(c.run(partition_size=int(size) or None))
+    size = rng.choice([-1, 0, 3, 37])
+    c.check(c.run(work_groups=None if size < 0 else int(size)))

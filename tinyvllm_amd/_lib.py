@@ -52,7 +52,7 @@ SIGNATURES = {
     "tv_rope_and_cache": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _L, _L,
                                _I, _P, _P]),
     "tv_paged_tree_workspace_bytes": (_S, [_I, _I, _I, _I, _I, _I, _I]),
-    "tv_paged_tree_partition_size": (_I, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "tv_paged_tree_work_groups": (_I, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "tv_paged_tree": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _F, _I, _I,
                            _I, _P, _S, _P]),
     "tv_verify_draft_tree_workspace_bytes": (_S, [_I, _I, _I, _I]),

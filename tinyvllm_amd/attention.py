@@ -394,12 +394,13 @@ class PagedTreePlan:
     whose bit its mask has (any mask; its own bit is not implied).  Nodes at tree_lens and beyond, and nodes that see
     nothing, get zeros.  A block id outside the cache, a NaN in a key, a score of +inf, or a NaN or infinity in a value
     spoils the nodes that see it and no others; a score of -inf has weight 0.  head_dim 64, 128 or 256, T at most 256, any block size.
-    ``max_context_len`` (context and tree) trims the table; ``partition_size``, a multiple of 64, is the number of keys a
-    work-group takes.  The tensors are read on every ``run()`` and must keep their storage.
+    ``max_context_len`` (context and tree) trims the table.  ``work_groups``: 0 gives every (sequence, KV head, tile of
+    rows) a work-group; n > 0 deals all their keys evenly to n work-groups and joins what that cuts, and results then depend
+    on the batch in their last digits.  The tensors are read on every ``run()`` and must keep their storage.
     """
 
     def __init__(self, queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask,
-                 n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, partition_size=None, out_dtype=None):
+                 n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, work_groups=None, out_dtype=None):
         index = k_cache.get_device()
         _require(index >= 0, f"tensors must live on a HIP device (got {k_cache.device})")
         check_devices(index, queries, v_cache, tree_mask)
@@ -425,23 +426,23 @@ class PagedTreePlan:
         used = mb if max_context_len is None else min((int(max_context_len) + block_size - 1) // block_size, mb)
         _require(used > 0, "no block table columns to attend over")
         code = _lib.dtype_code(queries.dtype)
-        if partition_size is None:
-            partition_size = _lib.device_size("tv_paged_tree_partition_size", index, max(b, 1), t, n_heads, n_kv_heads,
-                                              head_dim, used, block_size, code)
-            _require(partition_size > 0, f"head_dim {head_dim} or this table width is not supported")
-        self.partition_size = int(partition_size)
+        if work_groups is None:
+            work_groups = _lib.device_size("tv_paged_tree_work_groups", index, max(b, 1), t, n_heads, n_kv_heads, head_dim,
+                                           used, block_size, code)
+            _require(work_groups >= 0, f"head_dim {head_dim} or this table width is not supported")
+        self.work_groups = int(work_groups)
         self.index = index
         out_dtype = queries.dtype if out_dtype is None else out_dtype
         self.out = torch.empty((b, t, n_heads, head_dim), dtype=out_dtype, device=queries.device)
-        self.ws_bytes = _lib.device_size("tv_paged_tree_workspace_bytes", index, b, t, n_heads, head_dim, used,
-                                         block_size, self.partition_size)
+        self.ws_bytes = _lib.device_size("tv_paged_tree_workspace_bytes", index, b, t, n_heads, n_kv_heads,
+                                         head_dim, code, self.work_groups)
         self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=queries.device) if self.ws_bytes else None
         self._inputs = (queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask)
         self.args = (self.out.data_ptr(), queries.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                      block_tables.data_ptr(), context_lens.data_ptr(), tree_lens.data_ptr(), tree_mask.data_ptr(),
                      1 if tree_mask.dim() == 2 else 0, b, t, n_heads, n_kv_heads, head_dim, block_size, nb, mb, used,
                      qs[0] if b > 1 else t * hq * d, qs[1] if t > 1 else hq * d, 1.0 / math.sqrt(head_dim), code,
-                     _lib.dtype_code(out_dtype), self.partition_size, self.ws.data_ptr() if self.ws is not None else None,
+                     _lib.dtype_code(out_dtype), self.work_groups, self.ws.data_ptr() if self.ws is not None else None,
                      self.ws_bytes)
 
     def run(self):
@@ -450,12 +451,12 @@ class PagedTreePlan:
 
 
 def paged_tree_attention(queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask,
-                         n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, partition_size=None,
+                         n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, work_groups=None,
                          out_dtype=None):
     """Attention of drafted tokens over the paged cache and each other; see ``PagedTreePlan``.  Returns
     [B, T, Hq, D] in ``out_dtype`` (default: the query dtype)."""
     return PagedTreePlan(queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask, n_heads,
-                         n_kv_heads, head_dim, block_size, max_context_len, partition_size=partition_size,
+                         n_kv_heads, head_dim, block_size, max_context_len, work_groups=work_groups,
                          out_dtype=out_dtype).run()
 
 

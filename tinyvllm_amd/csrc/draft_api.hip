@@ -3,7 +3,6 @@
 #include <algorithm>
 
 #include "../../include/tv_draft.h"
-#include "tv_device_cache.h"
 #include "tv_draft.h"
 #include "tv_error.h"
 
@@ -21,23 +20,18 @@ bool aligned(const void* p, int n) { return (uintptr_t)p % n == 0; }
 int elem_size(int dtype) { return dtype == TV_F32 ? 4 : 2; }
 int log2_or_minus1(int x) { return (x & (x - 1)) ? -1 : __builtin_ctz(x); }
 
-// Compute units of the current device, asked for once per device.
-int device_cus() {
-  static std::atomic<int> known[tv::kMaxDevices];
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
-  if (dev < tv::kMaxDevices && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
-  if (dev < tv::kMaxDevices) known[dev].store(cus, std::memory_order_relaxed);
-  return cus;
-}
-
 // The arguments that every call over trees shares; blocks: whether it has a block table.
 int check_trees(const char* who, int num_seqs, int nodes) {
   if (num_seqs < 0 || num_seqs > 65535) return fail(TV_EINVAL, "%s: num_seqs %d outside 0..65535", who, num_seqs);
   if (nodes < 1 || nodes > TV_DRAFT_MAX_NODES)
     return fail(TV_EINVAL, "%s: nodes %d outside 1..%d", who, nodes, TV_DRAFT_MAX_NODES);
   return TV_OK;
+}
+
+tv::TreeShapeInfo tree_info(long long rows, int head_dim, int dtype) {
+  return dtype == TV_F32   ? tv::tree_info_f32(rows, head_dim)
+         : dtype == TV_F16 ? tv::tree_info_f16(rows, head_dim)
+                           : tv::tree_info_bf16(rows, head_dim);
 }
 
 int check_blocks(const char* who, int bt_stride, int block_size, int num_blocks) {
@@ -143,34 +137,39 @@ int tv_rope_and_cache(void* q_out, void* k_cache, void* v_cache, const void* q, 
   return check_launch(who);
 }
 
-size_t tv_paged_tree_workspace_bytes(int num_seqs, int nodes, int num_heads, int head_dim, int max_blocks,
-                                     int block_size, int partition_size) {
-  if (num_seqs <= 0 || nodes <= 0 || num_heads <= 0 || head_dim <= 0 || max_blocks <= 0 || block_size <= 0 ||
-      partition_size <= 0)
+size_t tv_paged_tree_workspace_bytes(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim, int dtype,
+                                     int work_groups) {
+  if (num_seqs <= 0 || nodes <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      !valid_head_dim(head_dim) || !valid_dtype(dtype) || work_groups <= 0)
     return 0;
-  const long long width = (long long)max_blocks * block_size;
-  const long long parts = (width + partition_size - 1) / partition_size;
-  if (parts <= 1) return 0;
-  return (size_t)parts * num_seqs * nodes * num_heads * (head_dim + 2) * sizeof(float);
+  const int rows = tree_info((long long)nodes * (num_heads / num_kv_heads), head_dim, dtype).tile_rows;
+  const size_t groups = std::max(1, work_groups / num_kv_heads);
+  return 2 * groups * num_kv_heads * rows * (head_dim + 2) * sizeof(float) + ((size_t)num_seqs + 1) * sizeof(long long);
 }
 
-int tv_paged_tree_partition_size(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim,
-                                 int max_blocks, int block_size, int dtype) {
-  const char* who = "tv_paged_tree_partition_size";
+int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim, int max_blocks,
+                              int block_size, int dtype) {
+  const char* who = "tv_paged_tree_work_groups";
   if (num_seqs <= 0 || nodes <= 0 || nodes > TV_DRAFT_MAX_NODES || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads != 0 || max_blocks <= 0 || block_size <= 0 ||
       (long long)max_blocks * block_size > (1LL << 30) || !valid_dtype(dtype))
-    return fail(TV_EINVAL, "%s: bad arguments", who), 0;
+    return fail(TV_EINVAL, "%s: bad arguments", who), -1;
   if (!valid_head_dim(head_dim))
-    return fail(TV_EUNSUPPORTED, "%s: head_dim %d not supported (64/128/256)", who, head_dim), 0;
-  const int cus = device_cus();
-  if (cus < 1) return fail(TV_EHIP, "%s: no device", who), 0;
-  const long long width = (long long)max_blocks * block_size;
-  const int whole = (int)((width + 63) / 64 * 64);
-  const long long units = (long long)num_seqs * num_kv_heads * (((long long)nodes * (num_heads / num_kv_heads) + 63) / 64);
-  const long long parts = std::max(1LL, std::min((2LL * cus + units - 1) / units, width / 256));
-  const long long p = std::max(256LL, ((width + parts - 1) / parts + 63) / 64 * 64);
-  return (int)std::min<long long>(p, whole);
+    return fail(TV_EUNSUPPORTED, "%s: head_dim %d not supported (64/128/256)", who, head_dim), -1;
+  const long long rows = (long long)nodes * (num_heads / num_kv_heads);
+  const tv::TreeShapeInfo shape = tree_info(rows, head_dim, dtype);
+  const long long slots = shape.resident();
+  const long long units = (rows + shape.tile_rows - 1) / shape.tile_rows * num_kv_heads * num_seqs;
+  const long long tiles = ((long long)max_blocks * block_size + shape.tile_keys - 1) / shape.tile_keys;
+  // In tiles that a work-group takes one after the other: undealt, its rounds of whole units; dealt, its share and
+  // what dealing and joining cost (8 us).  Long units are dealt in any case: their lengths are rarely equal, and few of them end a
+  // launch on a few CUs.  MI355X, us, undealt / dealt, 32 / 8 heads of 128 in fp16: 16 x 8 nodes over 100..500 tokens 15 / 18,
+  // over 500..2000 45 / 26; 64 x 8 over 500..1000 41 / 50; 64 x 16 over 512..4096 133 / 127; 256 x 4 over 500..2000
+  // 245 / 248, over 512..4096 444 / 432; 32 / 4 heads of 64: 64 x 8 over 200..1000 17 / 22, 1 x 32 over 1000 23 / 15,
+  // 1 x 64 over 8000 134 / 23; in fp32 4 x 8 over 17..250 17 / 11.
+  const long long cost = dtype == TV_F32 ? 6 : head_dim == 64 ? 12 : 8;
+  const long long undealt = (units + slots - 1) / slots * tiles, dealt = units * tiles / slots + cost;
+  return dealt < undealt || tiles >= 6 * cost ? (int)slots : 0;
 }
 
 int tv_paged_tree(void* out, const void* queries, const void* k_cache, const void* v_cache,
@@ -178,7 +177,7 @@ int tv_paged_tree(void* out, const void* queries, const void* k_cache, const voi
                   const uint64_t* mask, int mask_shared, int num_seqs, int nodes, int num_heads, int num_kv_heads,
                   int head_dim, int block_size, int num_blocks, int block_table_stride, int max_blocks,
                   int64_t q_seq_stride, int64_t q_node_stride, float scale, int dtype, int out_dtype,
-                  int partition_size, void* workspace, size_t workspace_bytes, void* stream) {
+                  int work_groups, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "tv_paged_tree";
   int rc = check_trees(who, num_seqs, nodes);
   if (rc == TV_OK) rc = check_blocks(who, block_table_stride, block_size, num_blocks);
@@ -193,8 +192,10 @@ int tv_paged_tree(void* out, const void* queries, const void* k_cache, const voi
     return fail(TV_EINVAL, "%s: bad block table (stride=%d, max_blocks=%d)", who, block_table_stride, max_blocks);
   const long long width = (long long)max_blocks * block_size;
   if (width > (1LL << 30)) return fail(TV_EINVAL, "%s: context width too large", who);
-  if (partition_size <= 0 || partition_size % 64 != 0)
-    return fail(TV_EINVAL, "%s: partition_size must be a positive multiple of 64 (got %d)", who, partition_size);
+  if (work_groups < 0 || work_groups > 1 << 16)
+    return fail(TV_EINVAL, "%s: work_groups %d outside 0..%d", who, work_groups, 1 << 16);
+  if ((long long)block_size * num_kv_heads * head_dim * elem_size(dtype) > 0x7fffffffLL)
+    return fail(TV_EUNSUPPORTED, "%s: blocks of 2 GiB and more", who);
   const int vec = 16 / elem_size(dtype);
   if (q_node_stride < (int64_t)num_heads * head_dim || q_node_stride % vec || q_seq_stride % vec ||
       (num_seqs > 1 && q_seq_stride < 0))
@@ -205,15 +206,14 @@ int tv_paged_tree(void* out, const void* queries, const void* k_cache, const voi
   if (!aligned(out, 16) || !aligned(queries, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(mask, 8) ||
       !aligned(block_tables, 4) || !aligned(context_lens, 4) || !aligned(tree_lens, 4))
     return fail(TV_EINVAL, "%s: queries, caches and out must be 16-byte aligned, the mask 8-byte aligned", who);
-  const long long max_parts = (width + partition_size - 1) / partition_size;
-  const size_t need =
-      tv_paged_tree_workspace_bytes(num_seqs, nodes, num_heads, head_dim, max_blocks, block_size, partition_size);
-  if (max_parts > 1 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+  const size_t need = tv_paged_tree_workspace_bytes(num_seqs, nodes, num_heads, num_kv_heads, head_dim, dtype, work_groups);
+  if (work_groups && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(TV_EINVAL, "%s: workspace of %zu bytes, 16-byte aligned, required (got %zu)", who, need, workspace_bytes);
   const long long rows = (long long)nodes * (num_heads / num_kv_heads);
-  // 1024 threads each at most in one dimension of fewer than 2^32
-  if (num_kv_heads > 65535 || rows > (1 << 20) ||
-      (rows + 15) / 16 * num_kv_heads > (1LL << 22) / num_seqs / max_parts)
+  const long long units = (rows + 63) / 64 * num_kv_heads * num_seqs;
+  // at most 512 threads each in one dimension of fewer than 2^32; a work-group counts its tiles in 32 bits
+  if (num_kv_heads > 65535 || rows > 1 << 22 || units >= 1 << 23 ||
+      (work_groups && (width / 16 + 1) * units / work_groups > 0x3fffffff))
     return fail(TV_EINVAL, "%s: grid too large", who);
   tv::TreeParams p{};
   p.out = out;
@@ -239,12 +239,9 @@ int tv_paged_tree(void* out, const void* queries, const void* k_cache, const voi
   p.width = (int)width;
   p.scale = scale;
   p.out_dtype = out_dtype;
-  p.partition = partition_size;
-  p.max_parts = (int)max_parts;
-  if (max_parts > 1) {
-    p.part_o = reinterpret_cast<float*>(workspace);
-    p.part_ml = p.part_o + (size_t)max_parts * num_seqs * nodes * num_heads * head_dim;
-  }
+  p.work_groups = work_groups;
+  p.least_tiles = dtype == TV_F32 ? 1 : 2;   // 4 x 8 nodes over 500..1000 tokens (32 / 8 heads of 128, fp16), us: 1 16.3, 2 15.0, 4 16.9
+  p.part_o = reinterpret_cast<float*>(workspace);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == TV_F32) tv::launch_tree_f32(p, head_dim, s);
   else if (dtype == TV_F16) tv::launch_tree_f16(p, head_dim, s);

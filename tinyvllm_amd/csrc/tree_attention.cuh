@@ -16,10 +16,13 @@
 // NaN, which the mask replaces for the rows that do not see the key.
 #pragma once
 
+#include "tv_device_cache.h"
 #include "tv_draft.h"
 #include "tv_fp8.h"
+#include "tv_tile_dma.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tv {
 
@@ -47,190 +50,319 @@ __device__ __forceinline__ float tree_max4(f32x4 x) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[0], x[1]), __builtin_elementwise_maximum(x[2], x[3]));
 }
 
-// Keys per tile.
-template <typename T, int D> constexpr int kTreeKeys = sizeof(T) == 4 ? (D == 256 ? 16 : 32) : (D == 256 ? 32 : 64);
+// The chunk permutation of a tile's row r (16-byte chunks, by exclusive or): without it all rows of a column
+// lie in the same banks.
+template <int CPR> __device__ __forceinline__ int tree_perm(int r) {
+  if constexpr (CPR == 8) return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  else return ((r & 7) << 1) | ((r >> 3) & 1);
+}
 
-// UB: the block size is 16 or a larger power of two: the rows that a wave stages at
-// once lie in one block, whose id and address are then scalar.
-template <typename T, int D, int RB, bool UB>
-__global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(const TreeParams p) {
+// 16 bytes per lane from a lane's own address into LDS at lds_base + 16 * lane.
+__device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_base), "v"(p) : "memory", "m0");
+}
+
+// A row tile of a sequence: its lengths, and the tiles of its keys.
+struct TreeUnit { int b, rt, ctx, len, keys, tiles; };
+
+// RG groups of four waves, 16 RB rows a wave.  BN keys a tile, NS tiles in LDS: one that is read and NS - 1 on the way.
+// UB: the block size is 16 or a larger power of two: the rows of a load lie in one
+// block, whose id and address are then scalar, and whose range ends at the last key.
+template <typename T, int D, int RB, int RG, int BN, int NS, int EU, bool NT, bool UB>
+__global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(const TreeParams p) {
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int BM = 64 * RB;
-  constexpr int BN = kTreeKeys<T, D>;
+  constexpr int THREADS = kTreeThreads * RG;
+  constexpr int WAVES = 4 * RG;
+  constexpr int BM = 64 * RB * RG;
   constexpr int KB = BN / 16;
   constexpr int DB = D / 16;
   constexpr int VEC = 16 / (int)sizeof(T);
-  constexpr int CPR = D / VEC;                 // 16-byte vectors of a row
-  constexpr int P = F32 ? D + 4 : D + 16;      // LDS row pitch (elements)
-  constexpr int SKT = BN * P;
-  constexpr int NV = BN * CPR / kTreeThreads;  // vectors per thread and tile, each of K and V
-  constexpr int RPP = kTreeThreads / CPR;      // tile rows of one pass over the threads
-  static_assert(NV * kTreeThreads == BN * CPR && NV >= 1, "tile shape");
-  __shared__ __attribute__((aligned(16))) T smem[2][2 * SKT];
+  constexpr int CPR = D / VEC;                 // 16-byte chunks of a row
+  constexpr int ROW = D * (int)sizeof(T);      // bytes of a row
+  constexpr int TILE = BN * ROW;
+  constexpr int STAGE = 2 * TILE;              // K tile, then V tile
+  constexpr int NV = BN * CPR / THREADS;       // loads of a wave for a tile, each of K and V
+  constexpr int RPI = 64 / CPR;                // rows of a load
+  constexpr int RPP = WAVES * RPI;             // rows of all waves' loads
+  static_assert(NV * THREADS == BN * CPR && NV >= 1 && NV * NS <= 64, "tile shape");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE];
+  __shared__ long long wave_tiles[WAVES];
+  __shared__ int start_seq, start_tile;        // the work-group's first tile
 
+  const uint32_t smem_at = sgpr((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem);
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int g = lane >> 4, col = lane & 15;
-  int unit = blockIdx.x;
-  const int rt = unit % p.row_tiles;
-  unit /= p.row_tiles;
-  const int kh = unit % p.num_kv_heads;
-  unit /= p.num_kv_heads;
-  const int b = unit % p.num_seqs;
-  const int part = unit / p.num_seqs;
-
   const int G = p.group;
-  const int ctx = min(max(p.context_lens[b], 0), p.width);
-  const int len = min(max(p.tree_lens[b], 0), p.nodes);
-  const int keys = min(ctx + len, p.width);
-  const int parts = max(1, (keys + p.partition - 1) / p.partition);
-  if (part >= parts) return;
   const int rows = p.nodes * G;
-  const int row0 = rt * BM + wave * RB * 16;
-  const int t0 = part * (p.partition / BN);
-  // a tile without a live node has nothing to attend, and writes its zeros
-  const int t1 = rt * BM < len * G ? min(t0 + p.partition / BN, (keys + BN - 1) / BN) : t0;
+
+  // The walk's state is the same in all lanes; saying so keeps it in scalar registers.
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto unit_of = [&](int b) {
+    TreeUnit u;
+    u.b = uniform(b);
+    u.rt = 0;
+    u.ctx = uniform(min(max(uniform_load(p.context_lens + u.b), 0), p.width));
+    u.len = uniform(min(max(uniform_load(p.tree_lens + u.b), 0), p.nodes));
+    u.keys = uniform(min(u.ctx + u.len, p.width));
+    u.tiles = uniform((u.keys + BN - 1) / BN);
+    return u;
+  };
+
+  // ---- this work-group's tiles: `left` of them from tile `tile` of unit cu on, of one KV head ----
+  TreeUnit cu;
+  int tile = 0, left = 0, kh;
+  int wg = blockIdx.x;
+  if (p.work_groups) {
+    // the heads of a group read the same keys' neighbouring slices of the cache's rows at about the same time
+    const int group = wg / p.num_kv_heads;
+    kh = wg - group * p.num_kv_heads;
+    // prefix sums of the sequences' tiles: a thread has `per` consecutive sequences
+    const int per = (p.num_seqs + THREADS - 1) / THREADS;
+    auto tiles_of = [&](int b) -> int {
+      if (b >= p.num_seqs) return 0;
+      const int ctx = min(max(p.context_lens[b], 0), p.width), len = min(max(p.tree_lens[b], 0), p.nodes);
+      return (min(ctx + len, p.width) + BN - 1) / BN * ((len * G + BM - 1) / BM);
+    };
+    long long mine = 0;
+    for (int k = 0; k < per; ++k) mine += tiles_of(tid * per + k);
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int lo = __builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)(uint32_t)(unsigned long long)upto);
+      const int hi = __builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)((unsigned long long)upto >> 32));
+      if (lane >= d) upto += (long long)((unsigned long long)(uint32_t)hi << 32 | (uint32_t)lo);
+    }
+    if (lane == 63) wave_tiles[wave] = upto;
+    if (tid == 0) start_seq = -1;
+    __syncthreads();
+    long long total = 0, before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) before += wave_tiles[w];
+      total += wave_tiles[w];
+    }
+    const long long share = max((total + p.groups - 1) / p.groups, (long long)p.least_tiles);
+    const long long from = share * group, to = min(from + share, total);
+    for (int k = 0; k < per; ++k) {
+      const int b = tid * per + k;
+      const long long n = tiles_of(b);
+      if (wg == 0 && b < p.num_seqs) p.first_tiles[b] = before;
+      if (from >= before && from < before + n) {
+        start_seq = b;
+        start_tile = (int)(from - before);
+      }
+      before += n;
+    }
+    if (wg == 0 && tid == 0) p.first_tiles[p.num_seqs] = share;
+    __syncthreads();
+    const int b0 = __builtin_amdgcn_readfirstlane(start_seq);
+    if (b0 < 0) return;                        // no tiles are left for it
+    left = __builtin_amdgcn_readfirstlane((int)(to - from));
+    tile = __builtin_amdgcn_readfirstlane(start_tile);
+    cu = unit_of(b0);
+    cu.rt = uniform(tile / cu.tiles);
+    tile = uniform(tile - cu.rt * cu.tiles);
+  } else {
+    const int rt = wg % p.row_tiles;
+    wg /= p.row_tiles;
+    kh = wg % p.num_kv_heads;
+    cu = unit_of(wg / p.num_kv_heads);
+    cu.rt = rt;
+    left = rt * BM < cu.len * G ? cu.tiles : 0;          // nothing to attend: zeros
+  }
+  // The next row tile, or the first of the next sequence that has a node.
+  auto advance = [&](TreeUnit& u) {
+    u.rt = uniform(u.rt + 1);
+    if (u.rt * BM < u.len * G) return;
+    do u = unit_of(u.b + 1);
+    while (uniform(u.b + 1 < p.num_seqs && u.len == 0));
+  };
 
   int qrow[RB], node[RB];
   constexpr int QF = F32 ? D / 16 : D / 32;
   u32x4 qf[RB][QF];
+  f32x4 oacc[RB][DB];
+  f32x4 sums[RB];                              // 16-bit: every lane's row sum; fp32: of the lane's own keys, in [0]
+  float m[RB];
+  auto begin_unit = [&]() {
 #pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    qrow[r] = row0 + r * 16 + col;
-    node[r] = qrow[r] / G;
-    const T* qg = reinterpret_cast<const T*>(p.q) + (size_t)b * p.q_seq_stride + (size_t)node[r] * p.q_node_stride +
-                  (size_t)(kh * G + qrow[r] - node[r] * G) * D;
-    // fp32: k index of step 4 f + e, lane g: 16 f + 4 g + e, on both operands
+    for (int r = 0; r < RB; ++r) {
+      qrow[r] = cu.rt * BM + (wave * RB + r) * 16 + col;
+      node[r] = qrow[r] / G;
+      const T* qg = reinterpret_cast<const T*>(p.q) + (size_t)cu.b * p.q_seq_stride + (size_t)node[r] * p.q_node_stride +
+                    (size_t)(kh * G + qrow[r] - node[r] * G) * D;
+      // fp32: k index of step 4 f + e, lane g: 16 f + 4 g + e, on both operands
 #pragma unroll
-    for (int f = 0; f < QF; ++f)
-      qf[r][f] = node[r] < len ? *reinterpret_cast<const u32x4*>(qg + (F32 ? 16 * f + 4 * g : 32 * f + 8 * g))
-                               : u32x4{0, 0, 0, 0};
-  }
+      for (int f = 0; f < QF; ++f)
+        qf[r][f] = node[r] < cu.len ? *reinterpret_cast<const u32x4*>(qg + (F32 ? 16 * f + 4 * g : 32 * f + 8 * g))
+                                    : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int db = 0; db < DB; ++db) oacc[r][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+      sums[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[r] = kNegInf;
+    }
+  };
 
-  // staging: this thread's vectors are chunk ch of tile rows sr + RPP i
-  const int sr = tid / CPR, ch = tid % CPR;
-  const int wr = wave * (64 / CPR);            // first of the wave's rows
+  // loading: load i of a wave fills tile rows wr + RPP i .. + RPI - 1, a lane chunk lane % CPR of row lane / CPR of them
+  const int wr = wave * RPI;
+  const int lr = lane / CPR;
   const int bs = p.block_size;
-  const size_t rs = (size_t)p.num_kv_heads * D;
-  const int* table = p.block_tables + (size_t)b * p.bt_stride;
-  const T* kc = reinterpret_cast<const T*>(p.k_cache) + (size_t)kh * D;
-  const T* vc = reinterpret_cast<const T*>(p.v_cache) + (size_t)kh * D;
-  auto key_of = [&](int t, int i) { return min(t * BN + (UB ? wr : sr) + RPP * i, keys - 1); };
-  struct Ids { int id[NV]; };
-  struct Stage { u32x4 k[NV], v[NV]; int ok[NV]; };
-  auto ids_of = [&](int t, Ids& x) {
+  const long long row_bytes = (long long)p.num_kv_heads * ROW;
+  const uint32_t block_bytes = (uint32_t)(bs * row_bytes);
+  const u64 kc = reinterpret_cast<u64>(p.k_cache) + (u64)kh * ROW, vc = reinterpret_cast<u64>(p.v_cache) + (u64)kh * ROW;
+  uint32_t voff[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    voff[i] = (UB ? (uint32_t)(lr * row_bytes) : 0u) + (((lane % CPR) ^ tree_perm<CPR>(wr + RPP * i + lr)) * 16);
+  // The next tile to request: tile lt of unit lu, with `to_load` to come; its block ids are looked up a tile ahead.
+  TreeUnit lu = cu;
+  int lt = tile, to_load = left;
+  struct Ids { int id[NV]; } ids;
+  auto look_up = [&]() {
+    if (to_load <= 0) return;
+    const int* table = p.block_tables + (size_t)lu.b * p.bt_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int key = key_of(t, i);
-      x.id[i] = UB ? uniform_load(table + (key >> p.bs_log2)) : table[key / bs];
+      const int key = min(lt * BN + wr + RPP * i + (UB ? 0 : lr), lu.keys - 1);
+      ids.id[i] = UB ? uniform_load(table + (key >> p.bs_log2)) : table[key / bs];
     }
   };
-  auto gload = [&](int t, const Ids& x, Stage& s) {
+  // Requests it into a stage and moves on; returns bit i for a load whose block is outside the cache.  Where no tile is
+  // left the requests are empty, so that their number is the same every time.
+  auto issue = [&](int stage) -> uint32_t {
+    uint32_t bad = 0;
+    uint32_t range[NV];                        // bytes of a load; rows past the last key arrive as zeros
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int id = UB ? __builtin_amdgcn_readfirstlane(x.id[i]) : x.id[i];
-      s.ok[i] = (unsigned)id < (unsigned)p.num_blocks ? -1 : 0;
-      const size_t block = (size_t)(id & s.ok[i]) * bs;
-      if constexpr (UB) {
-        // a wave's rows start at a multiple of their number: those past the last key are the block's own
-        const int first = (t * BN + wr + RPP * i) & (bs - 1);
-        const size_t at = (block + first) * rs;
-        const size_t lane_at = (size_t)(sr - wr) * rs + ch * VEC;
-        s.k[i] = *reinterpret_cast<const u32x4*>(kc + at + lane_at);
-        s.v[i] = *reinterpret_cast<const u32x4*>(vc + at + lane_at);
-      } else {
-        const int key = key_of(t, i);
-        const size_t at = (block + key % bs) * rs + ch * VEC;
-        s.k[i] = *reinterpret_cast<const u32x4*>(kc + at);
-        s.v[i] = *reinterpret_cast<const u32x4*>(vc + at);
-      }
-    }
-  };
-  auto lstore = [&](const Stage& s, int buf, int t) {
-    T* sk = smem[buf] + sr * P + ch * VEC;
-    bool plain = (t + 1) * BN <= ctx;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) plain = plain && s.ok[i];
-    if (__builtin_amdgcn_ballot_w64(!plain) == 0) {
+    for (int i = 0; i < NV; ++i) range[i] = (uint32_t)((RPI - 1) * row_bytes + ROW);
+    if (UB && !(to_load > 0 && (lt + 1) * BN <= lu.keys)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        *reinterpret_cast<u32x4*>(sk + RPP * i * P) = s.k[i];
-        *reinterpret_cast<u32x4*>(sk + RPP * i * P + SKT) = s.v[i];
+        const int count = to_load > 0 ? min(RPI, lu.keys - (lt * BN + wr + RPP * i)) : 0;
+        range[i] = count > 0 ? (uint32_t)((count - 1) * row_bytes + ROW) : 0u;
       }
-      return;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      u32x4 k = s.k[i], v = s.v[i];
-      const bool in = t * BN + sr + RPP * i < keys;
-      if (!in || !s.ok[i]) k = v = u32x4{0, 0, 0, 0};
-      bool poison = in && !s.ok[i];
+      const uint32_t at = sgpr(smem_at + stage * STAGE + (wr + RPP * i) * ROW);
+      if constexpr (UB) {
+        const uint32_t id = sgpr(ids.id[i]);
+        const bool ok = id < (uint32_t)p.num_blocks;
+        const u64 off = (u64)(ok ? id : 0) * block_bytes + (uint32_t)((lt * BN + wr + RPP * i) & (bs - 1)) * (uint32_t)row_bytes;
+        const u64 ka = kc + off, va = vc + off;
+        const uint32_t n = sgpr(ok ? range[i] : 0u);
+        const u32x4 kr = u32x4{sgpr((uint32_t)ka), sgpr((uint32_t)(ka >> 32)), n, 0x00020000u};
+        const u32x4 vr = u32x4{sgpr((uint32_t)va), sgpr((uint32_t)(va >> 32)), n, 0x00020000u};
+        if constexpr (NT) {
+          load_lds16_nt(kr, at, voff[i]);
+          load_lds16_nt(vr, sgpr(at + TILE), voff[i]);
+        } else {
+          load_lds16(kr, at, voff[i]);
+          load_lds16(vr, sgpr(at + TILE), voff[i]);
+        }
+        bad |= ok ? 0u : 1u << i;
+      } else {
+        const bool ok = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
+        const int key = min(lt * BN + wr + RPP * i + lr, lu.keys - 1);
+        const long long off = ((long long)(ok ? ids.id[i] : 0) * bs + key % bs) * row_bytes + voff[i];
+        load_lds16_at(reinterpret_cast<const void*>(kc + off), at);
+        load_lds16_at(reinterpret_cast<const void*>(vc + off), sgpr(at + TILE));
+        bad |= ok ? 0u : 1u << i;
+      }
+    }
+    if (--to_load > 0 && ++lt == lu.tiles) {
+      lt = 0;
+      advance(lu);
+    }
+    return bad;
+  };
+  // A wave's own loads of a tile that not all rows see in the same way.
+  auto amend = [&](int t, uint32_t bad, int stage) {   // of unit cu
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32x4* kp = reinterpret_cast<u32x4*>(smem + stage * STAGE + (wr + RPP * i) * ROW + lane * 16);
+      u32x4* vp = kp + TILE / 16;
+      u32x4 k = *kp, v = *vp;
+      const bool in = t * BN + wr + RPP * i + lr < cu.keys;
+      const bool lost = bad >> i & 1;
+      if (!in || lost) k = v = u32x4{0, 0, 0, 0};
+      bool poison = in && lost;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t bad = not_finite<T>(v[j]);
-        poison = poison || bad != 0;
-        v[j] &= ~bad;
+        const uint32_t w = not_finite<T>(v[j]);
+        poison = poison || w != 0;
+        v[j] &= ~w;
       }
       if (poison) k[0] = kTreeNan<T>;
-      *reinterpret_cast<u32x4*>(sk + RPP * i * P) = k;
-      *reinterpret_cast<u32x4*>(sk + RPP * i * P + SKT) = v;
+      *kp = k;
+      *vp = v;
     }
   };
 
   // Bits of the keys k0 .. k0 + 63 that a live node sees.
   auto seen_from = [&](int n, int k0) -> u64 {
-    const u64* words = p.mask + (size_t)b * p.mask_seq_stride + (size_t)n * p.words;
-    const int left = keys - k0;
+    const u64* words = p.mask + (size_t)cu.b * p.mask_seq_stride + (size_t)n * p.words;
+    const int left = cu.keys - k0;
     u64 bits;
-    if (k0 >= ctx) {
-      const int w = (k0 - ctx) >> 6, s = (k0 - ctx) & 63;
+    if (k0 >= cu.ctx) {
+      const int w = (k0 - cu.ctx) >> 6, s = (k0 - cu.ctx) & 63;
       bits = w < p.words ? words[w] >> s : 0;
       if (s && w + 1 < p.words) bits |= words[w + 1] << (64 - s);
     } else {
-      const int s = ctx - k0;                  // context keys of the tile
+      const int s = cu.ctx - k0;                  // context keys of the tile
       bits = s >= 64 ? ~0ull : ((1ull << s) - 1) | words[0] << s;
     }
     return left >= 64 ? bits : left > 0 ? bits & ((1ull << left) - 1) : 0;
   };
 
-  f32x4 oacc[RB][DB];
-  f32x4 sums[RB];                              // 16-bit: every lane's row sum; fp32: of the lane's own keys, in [0]
-  float m[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-#pragma unroll
-    for (int db = 0; db < DB; ++db) oacc[r][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    sums[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[r] = kNegInf;
-  }
   const float c = p.scale * kLog2e;
 
-  auto compute = [&](int buf, int t) {
-    const T* sk = smem[buf];
-    const T* sv = sk + SKT;
+  auto compute = [&](int stage, int t) {
+    const unsigned char* sk = smem + stage * STAGE;
+    const unsigned char* sv = sk + TILE;
     const int k0 = t * BN;
     f32x4 st[RB][KB];
+    // reads first, then products, so that one wait covers many reads
+    constexpr int FG = QF * KB > 16 ? 16 / KB : QF;      // reads of at most 16 fragments at once
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int f0 = 0; f0 < QF; f0 += FG) {
+      u32x4 kf[FG][KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) st[r][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int f = 0; f < FG; ++f)
 #pragma unroll
-    for (int f = 0; f < QF; ++f)
+        for (int kb = 0; kb < KB; ++kb)
+          kf[f][kb] = *reinterpret_cast<const u32x4*>(sk + (kb * 16 + col) * ROW + ((4 * (f0 + f) + g) ^ tree_perm<CPR>(col)) * 16);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + (kb * 16 + col) * P + (F32 ? 16 * f + 4 * g : 32 * f + 8 * g));
+      for (int f = 0; f < FG; ++f)
 #pragma unroll
-        for (int r = 0; r < RB; ++r) {
-          if constexpr (F32) {
+        for (int e = 0; e < (F32 ? 4 : 1); ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              st[r][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(u32_as_f32(kf[e]), u32_as_f32(qf[r][f][e]), st[r][kb], 0, 0, 0);
-          } else {
-            st[r][kb] = mfma16x16x32<T>(kf, qf[r][f], st[r][kb]);
-          }
-        }
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+              const f32x4 acc = f0 + f + e ? st[r][kb] : f32x4{0.f, 0.f, 0.f, 0.f};
+              if constexpr (F32)
+                st[r][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(u32_as_f32(kf[f][kb][e]), u32_as_f32(qf[r][f0 + f][e]), acc, 0, 0, 0);
+              else
+                st[r][kb] = mfma16x16x32<T>(kf[f][kb], qf[r][f0 + f], acc);
+            }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // V^T operands of the first 32 keys: from LDS while the softmax runs
+    u32x4 vf[F32 ? 1 : 2][F32 ? 1 : DB];
+    auto values = [&](int x) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const int r = x * 32 + 4 * g + (col >> 2);      // and 16 rows on, whose permutation is the same
+        const unsigned char* at = sv + r * ROW + ((db * 2 + ((col & 3) >> 1)) ^ tree_perm<CPR>(r)) * 16 + (col & 1) * 8;
+        const u32x2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(at));
+        const u32x2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(at + 16 * ROW));
+        vf[x & 1][db] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
+    };
+    if constexpr (!F32) values(0);
     float base[RB], mt[RB];
     bool need = false;
 #pragma unroll
@@ -241,10 +373,10 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(const Tree
 #pragma unroll
         for (int i = 0; i < 4; ++i) st[r][kb][i] = fmaf(st[r][kb][i], c, -base[r]);
     }
-    if (k0 + BN > ctx) {
+    if (k0 + BN > cu.ctx) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        const u64 bits = node[r] < len ? seen_from(node[r], k0) >> (4 * g) : 0;
+        const u64 bits = node[r] < cu.len ? seen_from(node[r], k0) >> (4 * g) : 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -290,7 +422,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(const Tree
         for (int i = 0; i < 4; ++i)            // keys 4 g + i of the block
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            const float v = sv[(kb * 16 + 4 * g + i) * P + db * 16 + col];
+            const int r = kb * 16 + 4 * g + i;
+            const float v = *reinterpret_cast<const float*>(sv + r * ROW + ((db * 4 + (col >> 2)) ^ tree_perm<CPR>(r)) * 16 + (col & 3) * 4);
 #pragma unroll
             for (int r = 0; r < RB; ++r)
               oacc[r][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, st[r][kb][i], oacc[r][db], 0, 0, 0);
@@ -300,6 +433,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(const Tree
       const u32x4 ones = u32x4{kOnes2<T>, kOnes2<T>, kOnes2<T>, kOnes2<T>};
 #pragma unroll
       for (int x = 0; x < BN / 32; ++x) {
+        if (x + 1 < BN / 32) values(x + 1);
         u32x4 pf[RB];
         // reduction index 8g + j: key 4g + j of block 2 x (j < 4), 4g + j - 4 of block 2 x + 1
 #pragma unroll
@@ -307,147 +441,219 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(const Tree
           pf[r] = u32x4{pack2<T>(st[r][2 * x][0], st[r][2 * x][1]), pack2<T>(st[r][2 * x][2], st[r][2 * x][3]),
                         pack2<T>(st[r][2 * x + 1][0], st[r][2 * x + 1][1]), pack2<T>(st[r][2 * x + 1][2], st[r][2 * x + 1][3])};
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const T* a = sv + (x * 32 + 4 * g + (col >> 2)) * P + db * 16 + 4 * (col & 3);
-          const u32x2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(a));
-          const u32x2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(a + 16 * P));
-          const u32x4 vf = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int r = 0; r < RB; ++r) oacc[r][db] = mfma16x16x32<T>(vf, pf[r], oacc[r][db]);
-        }
+          for (int r = 0; r < RB; ++r) oacc[r][db] = mfma16x16x32<T>(vf[x & 1][db], pf[r], oacc[r][db]);
 #pragma unroll
         for (int r = 0; r < RB; ++r) sums[r] = mfma16x16x32<T>(ones, pf[r], sums[r]);
       }
     }
   };
 
-  if (t0 < t1) {
-    Ids ids;
-    Stage s;
-    ids_of(t0, ids);
-    gload(t0, ids, s);
-    ids_of(t0 + 1, ids);
-    lstore(s, 0, t0);
-    gload(t0 + 1, ids, s);
-    ids_of(t0 + 2, ids);
-    lds_barrier();
-    for (int t = t0; t < t1; ++t) {
-      compute((t - t0) & 1, t);
-      if (t + 1 < t1) {
-        lstore(s, ((t - t0) & 1) ^ 1, t + 1);
-        gload(t + 2, ids, s);
-        ids_of(t + 3, ids);
+  // A unit's rows go out, or, where other work-groups have tiles of it, its part of them.
+  auto end_unit = [&](int first, int past, int slot) {
+    const bool whole = first == 0 && past == cu.tiles;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const float l = F32 ? sum_over_g(sums[r][0]) : sums[r][0];
+      const bool live = node[r] < cu.len;
+      if (!(live || (!p.work_groups && qrow[r] < rows))) continue;
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;     // a row that sees nothing is zero
+      if (whole) {
+        const size_t at = (((size_t)cu.b * p.nodes + node[r]) * p.num_kv_heads * G + (size_t)kh * G + qrow[r] - node[r] * G) * D + 4 * g;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const f32x4 x = live ? oacc[r][db] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+          if (F32 || p.out_dtype == kF32)
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at + db * 16) = x;
+          else if constexpr (!F32)
+            *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at + db * 16) =
+                u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+        }
+      } else {
+        const size_t at = (size_t)slot * BM + (wave * RB + r) * 16 + col;
+        if (g == 0) {
+          p.part_ml[2 * at] = m[r];
+          p.part_ml[2 * at + 1] = l;           // zero: no keys of this row
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          *reinterpret_cast<f32x4*>(p.part_o + (at - col) * D + db * 256 + col * 16 + 4 * g) = oacc[r][db] * inv;
       }
-      lds_barrier();
     }
-  }
+  };
 
+  begin_unit();
+  if (left <= 0) {
+    end_unit(0, cu.tiles, 0);
+    return;
+  }
+  look_up();
+  u64 bad = 0;                                 // NV bits a tile, the next one's lowest
 #pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    if (qrow[r] >= rows) continue;
-    const bool live = node[r] < len;
-    const float l = F32 ? sum_over_g(sums[r][0]) : sums[r][0];
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;       // a row that sees nothing is zero
-    if (parts == 1) {
-      const size_t at = (((size_t)b * p.nodes + node[r]) * p.num_kv_heads * G + (size_t)kh * G + qrow[r] - node[r] * G) * D + 4 * g;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const f32x4 x = live ? oacc[r][db] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
-        if (F32 || p.out_dtype == kF32)
-          *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at + db * 16) = x;
-        else if constexpr (!F32)
-          *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at + db * 16) =
-              u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-      }
-    } else if (live) {
-      const size_t slot = (((size_t)part * p.num_seqs + b) * p.num_kv_heads + kh) * rows + qrow[r];
-      if (g == 0) {
-        p.part_ml[2 * slot] = m[r];
-        p.part_ml[2 * slot + 1] = l;           // zero: no keys of this row, and no output row
-      }
-      if (l != 0.0f) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(p.part_o + slot * D + db * 16 + 4 * g) = oacc[r][db] * inv;
-      }
+  for (int k = 0; k < NS - 1; ++k) {
+    bad |= (u64)issue(k) << (NV * k);
+    look_up();
+  }
+  int first = tile, slot = 2 * wg;
+  int stage = 0;
+  while (true) {
+    wait_vmcnt<2 * NV * (NS - 2)>();
+    const uint32_t lost = (uint32_t)bad & ((1u << NV) - 1);
+    if (__builtin_amdgcn_ballot_w64((tile + 1) * BN > cu.ctx || lost != 0) != 0) {
+      __asm__ volatile("" ::: "memory");
+      amend(tile, lost, stage);
+    }
+    lds_barrier();                             // the tile is there; the one before has been read
+    bad = bad >> NV | (u64)issue(stage == 0 ? NS - 1 : stage - 1) << (NV * (NS - 2));
+    look_up();
+    compute(stage, tile);
+    stage = stage + 1 == NS ? 0 : stage + 1;
+    ++tile;
+    --left;
+    if (tile == cu.tiles || left == 0) {
+      end_unit(first, tile, slot);
+      if (left == 0) break;
+      advance(cu);
+      begin_unit();
+      first = tile = 0;
+      slot |= 1;
     }
   }
+  wait_vmcnt<0>();                             // (empty requests write zeros)
 }
 
-// Joins the parts of a split sequence's rows: out = sum w_s o_s / sum w_s, w_s = l_s 2^(m_s - max m).
+// Joins the parts of a unit's rows that several work-groups have: out = sum w_s o_s / sum w_s, w_s = l_s 2^(m_s - max m).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
   constexpr int TPR = D / 4;                   // threads of a row
   const int b = blockIdx.z, kh = blockIdx.y;
   const int G = p.group;
-  const int rows = p.nodes * G;
-  const int ctx = min(max(p.context_lens[b], 0), p.width);
   const int len = min(max(p.tree_lens[b], 0), p.nodes);
-  const int keys = min(ctx + len, p.width);
-  const int parts = (keys + p.partition - 1) / p.partition;
-  if (parts <= 1) return;                      // written already
   const int row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  if (row >= rows) return;
+  if (row >= p.nodes * G) return;
   const int d = (threadIdx.x % TPR) * 4;
   const int node = row / G;
+  const size_t out_at = (((size_t)b * p.nodes + node) * p.num_kv_heads * G + (size_t)kh * G + row - node * G) * D + d;
+  auto store = [&](f32x4 x) {
+    if (sizeof(T) == 4 || p.out_dtype == kF32)
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + out_at) = x;
+    else if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + out_at) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+  };
+  if (node >= len) return store(f32x4{0.f, 0.f, 0.f, 0.f});      // padding
+  const int ctx = min(max(p.context_lens[b], 0), p.width);
+  const int tiles = (min(ctx + len, p.width) + p.tile_keys - 1) / p.tile_keys;
+  const int rt = row / p.tile_rows;
+  const long long share = p.first_tiles[p.num_seqs], from = p.first_tiles[b] + (long long)rt * tiles;
+  const int g0 = (int)(from / share), g1 = (int)((from + tiles - 1) / share);
+  if (g0 == g1) return;                        // written already
+  const int parts = g1 - g0 + 1;
+  // a part that begins where its work-group does is that one's first, others its second.  Within 16 rows the values
+  // lie as the kernel's accumulators do, [D / 16][16 rows][16]
+  auto place = [&](int s) -> size_t {
+    const int g = g0 + s;
+    const size_t slot = 2 * ((size_t)g * p.num_kv_heads + kh) + (s == 0 && from > share * g ? 1 : 0);
+    return slot * p.tile_rows + row - rt * p.tile_rows;
+  };
   f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (node < len) {
-    const size_t step = (size_t)p.num_seqs * p.num_kv_heads * rows;
-    const size_t slot0 = ((size_t)b * p.num_kv_heads + kh) * rows + row;
-    constexpr int U = 8;                       // parts on the way at once
-    float M = kNegInf;
-    for (int s0 = 0; s0 < parts; s0 += U) {
-      float mv[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) mv[u] = p.part_ml[2 * (slot0 + min(s0 + u, parts - 1) * step)];
-#pragma unroll
-      for (int u = 0; u < U; ++u) M = fmaxf(M, mv[u]);
-    }
-    float den = 0.0f;
+  float den = 0.0f, M = kNegInf;
+  // U parts on the way at once; past the last one they are read again and weigh nothing
+  auto join = [&](auto count) {
+    constexpr int U = decltype(count)::value;
     for (int s0 = 0; s0 < parts; s0 += U) {
       float mv[U], lv[U];
       f32x4 o[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const size_t slot = slot0 + min(s0 + u, parts - 1) * step;
-        mv[u] = p.part_ml[2 * slot];
-        lv[u] = p.part_ml[2 * slot + 1];
-        o[u] = *reinterpret_cast<const f32x4*>(p.part_o + slot * D + d);
+        const size_t at = place(min(s0 + u, parts - 1));
+        mv[u] = p.part_ml[2 * at];
+        lv[u] = p.part_ml[2 * at + 1];
+        o[u] = *reinterpret_cast<const f32x4*>(p.part_o + at / 16 * 16 * D + d / 16 * 256 + at % 16 * 16 + d % 16);
       }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, mv[u]);
+      const float f = M == kNegInf ? 1.0f : fast_exp2(M - top);      // (without a maximum: nothing, or NaN)
+      x *= f;
+      den *= f;
+      M = top;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (s0 + u >= parts || lv[u] == 0.0f) continue;  // no keys of this row: its part was not written
-        const float w = lv[u] * (M == kNegInf ? 1.0f : fast_exp2(mv[u] - M));   // without a maximum: only NaN
+        if (s0 + u >= parts || lv[u] == 0.0f) continue;  // no keys of this row
+        const float w = lv[u] * (mv[u] == kNegInf ? 1.0f : fast_exp2(mv[u] - M));
         den += w;
         x += o[u] * w;
       }
     }
-    x *= den != 0.0f ? 1.0f / den : 0.0f;
-  }
-  const size_t at = (((size_t)b * p.nodes + node) * p.num_kv_heads * G + (size_t)kh * G + row - node * G) * D + d;
-  if (sizeof(T) == 4 || p.out_dtype == kF32)
-    *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at) = x;
-  else if constexpr (sizeof(T) == 2)
-    *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+  };
+  if (parts <= 2) join(std::integral_constant<int, 2>());
+  else join(std::integral_constant<int, 8>());
+  x *= den != 0.0f ? 1.0f / den : 0.0f;
+  store(x);
 }
 
-template <typename T, int D, int RB> void tree_launch_of(TreeParams p, hipStream_t s) {
-  const int rows = p.nodes * p.group;
-  p.row_tiles = (rows + 64 * RB - 1) / (64 * RB);
-  const dim3 grid((unsigned)((long long)p.row_tiles * p.num_kv_heads * p.num_seqs * p.max_parts));
-  if (p.bs_log2 >= 4) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, true>), grid, dim3(kTreeThreads), 0, s, p);
-  else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, false>), grid, dim3(kTreeThreads), 0, s, p);
-  if (p.max_parts > 1) {
-    constexpr int per = 256 / (D / 4);
-    hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((rows + per - 1) / per, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
+// What a (type, head size, number of rows) runs as.
+template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool NT_> struct TreeShape {
+  static constexpr int RB = RB_, RG = RG_, BN = BN_, NS = NS_, EU = EU_;
+  static constexpr bool NT = NT_;
+  static constexpr int kRows = 64 * RB * RG, kThreads = kTreeThreads * RG;
+
+  static void launch(TreeParams p, hipStream_t s) {
+    const int rows = p.nodes * p.group;
+    p.tile_rows = kRows;
+    p.tile_keys = BN;
+    p.row_tiles = (rows + kRows - 1) / kRows;
+    if (p.work_groups) {
+      p.groups = std::max(1, p.work_groups / p.num_kv_heads);
+      p.work_groups = p.groups * p.num_kv_heads;
+      p.part_ml = p.part_o + (size_t)2 * p.work_groups * kRows * D;
+      p.first_tiles = reinterpret_cast<long long*>(p.part_ml + (size_t)4 * p.work_groups * kRows);
+    }
+    const dim3 grid(p.work_groups ? p.work_groups : (unsigned)((long long)p.row_tiles * p.num_kv_heads * p.num_seqs));
+    if (p.bs_log2 >= 4)
+      hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, true>), grid, dim3(kThreads), 0, s, p);
+    else
+      hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, false>), grid, dim3(kThreads), 0, s, p);
+    if (p.work_groups) {
+      constexpr int per = 256 / (D / 4);
+      hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((rows + per - 1) / per, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
+    }
   }
+  static long long resident() {
+    static std::atomic<long long> slots[kMaxDevices];
+    return resident_work_groups(slots, tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, true>, kThreads);
+  }
+};
+
+// Calls f with the shape for so many rows (nodes times query heads of a KV head).
+template <typename T, int D, typename F> auto tree_shape(long long rows, F f) {
+  if constexpr (sizeof(T) == 4) {
+    constexpr int BN = D == 256 ? 16 : 32;
+    return rows <= 64 ? f(TreeShape<T, D, 1, 1, BN, 2, 2, true>()) : f(TreeShape<T, D, 1, 1, BN, 2, 2, false>());
+  } else if constexpr (D == 256) {
+    return rows <= 64 ? f(TreeShape<T, D, 1, 1, 32, 2, 2, true>()) : f(TreeShape<T, D, 1, 1, 32, 2, 2, false>());
+  } else {
+    constexpr int BN = D == 64 ? 64 : 32, EU = D == 64 ? 3 : 2;
+    if (rows <= 64) return f(TreeShape<T, D, 1, 1, 64, 2, (D == 64 ? 4 : 2), true>());
+    return rows <= 128 ? f(TreeShape<T, D, 2, 1, BN, 2, EU, true>()) : f(TreeShape<T, D, 2, 1, BN, 2, EU, false>());
+  }
+}
+template <typename T, typename F> auto tree_shape(long long rows, int head_dim, F f) {
+  if (head_dim == 64) return tree_shape<T, 64>(rows, f);
+  if (head_dim == 128) return tree_shape<T, 128>(rows, f);
+  return tree_shape<T, 256>(rows, f);
 }
 
 }  // namespace
 
 template <typename T> void tree_launch(const TreeParams& p, int head_dim, hipStream_t s) {
-  if (head_dim == 64) tree_launch_of<T, 64, 1>(p, s);
-  else if (head_dim == 128) tree_launch_of<T, 128, 1>(p, s);
-  else tree_launch_of<T, 256, 1>(p, s);
+  tree_shape<T>((long long)p.nodes * p.group, head_dim, [&](auto shape) { shape.launch(p, s); });
+}
+template <typename T> TreeShapeInfo tree_info(long long rows, int head_dim) {
+  return tree_shape<T>(rows, head_dim, [](auto shape) {
+    return TreeShapeInfo{decltype(shape)::kRows, decltype(shape)::BN, [] { return decltype(shape)::resident(); }};
+  });
 }
 
 }  // namespace tv

@@ -55,10 +55,15 @@ struct TreeParams {
   int width;                 // max_blocks * block_size
   float scale;
   int out_dtype;
-  int partition, max_parts;
   int row_tiles;
-  float* part_o;             // [max_parts, B, Hkv, nodes * group, D] normalised parts
-  float* part_ml;            // [max_parts, B, Hkv, nodes * group, 2] (max in log2 units, sum)
+  // 0: a work-group per row tile of a (sequence, KV head).  Else the key tiles of all sequences' row tiles, one after the
+  // other, are dealt evenly to groups, at least least_tiles each; a group is a work-group for every KV head.  A second
+  // kernel joins what is cut.
+  int work_groups, groups, least_tiles;
+  int tile_rows, tile_keys;
+  float* part_o;             // [work_groups, 2, tile_rows, D] normalised parts: of a work-group's first unit, of a later one
+  float* part_ml;            // [work_groups, 2, tile_rows, 2] (max in log2 units, sum)
+  long long* first_tiles;    // [B + 1] tiles of the sequences before; then the tiles of a group
 };
 
 struct VerifyParams {
@@ -90,9 +95,17 @@ struct KeepParams {
 
 void launch_draft_layout(const DraftLayoutParams& p, hipStream_t s);
 void launch_rope_cache(const RopeCacheParams& p, int dtype, bool halves, bool wide, hipStream_t s);
+// The tile of so many rows: its rows, its keys, and the work-groups that are resident at once.
+struct TreeShapeInfo {
+  int tile_rows, tile_keys;
+  long long (*resident)();
+};
 void launch_tree_f32(const TreeParams& p, int head_dim, hipStream_t s);
 void launch_tree_f16(const TreeParams& p, int head_dim, hipStream_t s);
 void launch_tree_bf16(const TreeParams& p, int head_dim, hipStream_t s);
+TreeShapeInfo tree_info_f32(long long rows, int head_dim);
+TreeShapeInfo tree_info_f16(long long rows, int head_dim);
+TreeShapeInfo tree_info_bf16(long long rows, int head_dim);
 size_t verify_workspace_bytes(int num_seqs, int nodes, int vocab, int dtype);
 void launch_verify(VerifyParams p, int dtype, hipStream_t s);
 void launch_keep(const KeepParams& p, int layers, int vec_bytes, hipStream_t s);
