@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .draft_tree import MAX_NODES, check_block_tables, check_tree_tensors
+from .draft_tree import MAX_NODES, check_block_tables, check_int32
 from .kv_cache import check_devices, check_fp8_cache
 
 _lib.load()
@@ -402,27 +402,31 @@ class PagedTreePlan:
     def __init__(self, queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask,
                  n_heads, n_kv_heads, head_dim, block_size, max_context_len=None, *, work_groups=None, out_dtype=None):
         index = k_cache.get_device()
-        _require(index >= 0, f"tensors must live on a HIP device (got {k_cache.device})")
+        if index < 0:
+            raise ValueError(f"tensors must live on a HIP device (got {k_cache.device})")
         check_devices(index, queries, v_cache, tree_mask)
-        _require(queries.dim() == 4, f"queries must be [B, T, Hq, D], got {tuple(queries.shape)}")
+        if queries.dim() != 4:
+            raise ValueError(f"queries must be [B, T, Hq, D], got {tuple(queries.shape)}")
         b, t, hq, d = queries.shape
         _require(hq == n_heads and d == head_dim, "queries shape does not match n_heads/head_dim")
-        _require(1 <= t <= MAX_NODES, f"T must be 1 to {MAX_NODES}, got {t}")
+        if not 1 <= t <= MAX_NODES:
+            raise ValueError(f"T must be 1 to {MAX_NODES}, got {t}")
         qs = queries.stride()
         _require(qs[3] == 1 and (qs[2] == d or hq == 1), "queries: heads and head_dim must be contiguous")
-        _require(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.is_contiguous() and
-                 v_cache.is_contiguous(), "k_cache / v_cache must be dense [NB, bs, Hkv, D] tensors of one shape")
-        nb, bs, hkv, d2 = k_cache.shape
-        _require((bs, hkv, d2) == (block_size, n_kv_heads, head_dim),
-                 f"cache shape {tuple(k_cache.shape)} does not match block_size/n_kv_heads/head_dim")
+        shape = k_cache.shape
+        _require(len(shape) == 4 and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous(),
+                 "k_cache / v_cache must be dense [NB, bs, Hkv, D] tensors of one shape")
+        if shape[1:] != (block_size, n_kv_heads, head_dim):
+            raise ValueError(f"cache shape {tuple(shape)} does not match block_size/n_kv_heads/head_dim")
+        nb = shape[0]
         _require(n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
-        _require(queries.dtype == k_cache.dtype == v_cache.dtype, "queries and caches must share a dtype")
-        check_block_tables(index, b, block_tables)
-        check_tree_tensors(index, b, t, context_lens=context_lens, tree_lens=tree_lens)
+        _require(queries.dtype is k_cache.dtype and v_cache.dtype is k_cache.dtype, "queries and caches must share a dtype")
+        mb = check_block_tables(index, b, block_tables)
+        check_int32(index, (b,), ("context_lens", context_lens), ("tree_lens", tree_lens))
         words = (t + 63) // 64
-        _require(tree_mask.dtype == torch.int64 and tuple(tree_mask.shape) in ((b, t, words), (t, words)) and
-                 tree_mask.is_contiguous(), f"tree_mask must be contiguous int64 [{b}, {t}, {words}] or [{t}, {words}]")
-        mb = block_tables.shape[1]
+        if tree_mask.dtype is not torch.int64 or tree_mask.shape not in ((b, t, words), (t, words)) or \
+                not tree_mask.is_contiguous():
+            raise ValueError(f"tree_mask must be contiguous int64 [{b}, {t}, {words}] or [{t}, {words}]")
         used = mb if max_context_len is None else min((int(max_context_len) + block_size - 1) // block_size, mb)
         _require(used > 0, "no block table columns to attend over")
         code = _lib.dtype_code(queries.dtype)

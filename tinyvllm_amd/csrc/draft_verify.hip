@@ -14,7 +14,7 @@
 // probability 2^17 d.
 //
 // A walk over a path is serial and reads its rows only; reading the rows of all
-// nodes first is parallel.  The second is taken for trees of few logits.
+// nodes first is parallel (all_rows).
 #include "tv_draft.h"
 
 #include <algorithm>
@@ -23,13 +23,12 @@ namespace tv {
 
 namespace {
 
-constexpr int kWalkThreads = 1024;
+constexpr int kWalkThreads = 512;
 constexpr int kStatThreads = 256;
 constexpr int kStatVecs = 8;             // 16-byte vectors a thread of the stats kernel: 32 KiB of a row
 constexpr int kDrawThreads = 256;
 constexpr int kDrawPer = 8;              // elements a thread of the draw kernels
 constexpr int kDrawChunk = kDrawThreads * kDrawPer;
-constexpr int NC = kDraftMaxNodes / 64;
 constexpr double kUnsure = 0x1p-13;
 
 // What is known of a row, or of a part of it: the first maximum, and sum e relative to it.
@@ -43,6 +42,7 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
   if (x == 0.0f) return 0x80000000u;     // -0 equals +0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float from_order_bits(uint32_t o) { return u32_as_f32(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ u64 shfl_xor64(u64 x, int mask) {
   const uint32_t lo = __builtin_bit_cast(uint32_t, shfl_xor(u32_as_f32((uint32_t)x), mask));
   const uint32_t hi = __builtin_bit_cast(uint32_t, shfl_xor(u32_as_f32((uint32_t)(x >> 32)), mask));
@@ -120,9 +120,13 @@ template <typename T> __device__ __forceinline__ float sum_of(const u32x4& w, fl
 }
 
 // One thread's share of x[0 .. n): 16-byte vectors tid, tid + threads, .. from the first 16-byte boundary on, and of the
-// elements before and behind them one each.
+// elements before and behind them one each.  Its maximum, the index of the first of that value, and sum e.
+struct ThreadStat {
+  float m, s;
+  int idx;
+};
 template <typename T>
-__device__ __forceinline__ RowStat thread_stat(const T* x, int n, int tid, int threads, float c, bool sampled) {
+__device__ __forceinline__ ThreadStat thread_stat(const T* x, int n, int tid, int threads, float c, bool sampled) {
   constexpr int EPV = 16 / (int)sizeof(T);
   constexpr int U = kStatVecs;
   const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
@@ -130,10 +134,14 @@ __device__ __forceinline__ RowStat thread_stat(const T* x, int n, int tid, int t
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   float m = kNegInf, s = 0.0f;
   int at = 0;                            // the vector, or -1 - element, that the maximum was met in first
-  if (tid < head) {
-    m = to_float<T>(x[tid]);
+  u32x4 held = u32x4{0, 0, 0, 0};        // that vector
+  const int tail = head + vecs * EPV + tid;
+  const float first = tid < head ? to_float<T>(x[tid]) : kNegInf;
+  const float last = tail < n ? to_float<T>(x[tail]) : kNegInf;
+  if (first != kNegInf) {
+    m = first;
     at = -1 - tid;
-    s = m > kNegInf ? 1.0f : 0.0f;
+    s = 1.0f;
   }
   for (int v0 = tid; v0 < vecs; v0 += threads * U) {
     u32x4 w[U];
@@ -142,10 +150,12 @@ __device__ __forceinline__ RowStat thread_stat(const T* x, int n, int tid, int t
     const float old = m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (v0 + u * threads >= vecs) break;
       const float was = m;
-      m = max_of<T>(w[u], m);
-      at = m != was ? v0 + u * threads : at;   // (a NaN differs from itself: at is not looked at then)
+      m = max_of<T>(w[u], m);            // (past the end the last vector again: it raises nothing)
+      const bool up = m != was;          // a NaN differs from itself: at is not looked at then
+      at = up ? min(v0 + u * threads, vecs - 1) : at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) held[i] = up ? w[u][i] : held[i];
     }
     if (sampled && m > kNegInf) {
       if (m > old) s *= old > kNegInf ? weight(old, m, c) : 0.0f;
@@ -154,42 +164,48 @@ __device__ __forceinline__ RowStat thread_stat(const T* x, int n, int tid, int t
         if (v0 + u * threads < vecs) s += sum_of<T>(w[u], m, c);
     }
   }
-  const int tail = head + vecs * EPV + tid;
-  if (tail < n) {
-    const float v = to_float<T>(x[tail]);
-    const float was = m;
-    m = __builtin_elementwise_maximum(m, v);
-    if (m > was) {
-      at = -1 - tail;
-      s *= was > kNegInf ? weight(was, m, c) : 0.0f;
-    }
-    if (m > kNegInf) s += weight(v, m, c);
+  const float was = m;
+  m = __builtin_elementwise_maximum(m, last);
+  if (m > was) {
+    at = -1 - tail;
+    s *= was > kNegInf ? weight(was, m, c) : 0.0f;
   }
-  RowStat r{0, m, s};
-  if (m != m) {
-    r.key = ~0ull;
-  } else if (m > kNegInf) {
-    int idx = -1 - at;
-    if (at >= 0) {
-      idx = head + at * EPV;
+  if (last > kNegInf && m > kNegInf) s += weight(last, m, c);
+  int idx = -1 - at;
+  if (at >= 0) {
 #pragma unroll
-      for (int e = EPV - 1; e >= 0; --e)
-        if (to_float<T>(x[head + at * EPV + e]) == m) idx = head + at * EPV + e;
+    for (int e = EPV - 1; e >= 0; --e) {
+      float v;
+      if constexpr (sizeof(T) == 4) {
+        v = u32_as_f32(held[e]);
+      } else {
+        float lo, hi;
+        unpack2<T>(held[e / 2], lo, hi);
+        v = e % 2 ? hi : lo;
+      }
+      if (v == m) idx = head + at * EPV + e;
     }
-    r.key = (u64)order_bits(m) << 32 | (uint32_t)~idx;
   }
-  return r;
+  return ThreadStat{m, s, idx};
 }
 
 // The wave's shares as one, in every lane.
-__device__ __forceinline__ RowStat wave_stat(RowStat r, float c, bool sampled) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) r.key = max(r.key, shfl_xor64(r.key, d));
-  if (sampled) {
-    const float top = group_max<64>(r.m);      // (of a NaN nothing is used)
-    r.s = group_sum<64>(r.m > kNegInf ? r.s * weight(r.m, top, c) : 0.0f);
-    r.m = top;
+__device__ __forceinline__ RowStat wave_stat(const ThreadStat& t, float c, bool sampled) {
+  RowStat r{0, group_max<64>(t.m), 0.0f};                    // (of a NaN nothing is used)
+  if (__builtin_amdgcn_ballot_w64(t.m != t.m)) {
+    r.key = ~0ull;
+    return r;
   }
+  if (r.m == kNegInf) return r;
+  // nearly always one lane has it; of several the lowest index
+  u64 with = __builtin_amdgcn_ballot_w64(t.m == r.m);
+  int idx = 0x7fffffff;
+  while (with) {
+    idx = min(idx, __builtin_amdgcn_readlane(t.idx, __builtin_ctzll(with)));
+    with &= with - 1;
+  }
+  r.key = (u64)order_bits(r.m) << 32 | (uint32_t)~idx;
+  if (sampled) r.s = group_sum<64>(t.m > kNegInf ? t.s * weight(t.m, r.m, c) : 0.0f);
   return r;
 }
 
@@ -198,19 +214,26 @@ __device__ __forceinline__ float temperature_of(const VerifyParams& p, int b) {
   return t >= 0x1p-126f ? t : 0.0f;
 }
 
+// What the walk leaves for the draw after a sequence's last node.
+struct DrawJob {
+  double mass;                           // E: the children's e
+  int node;                              // -1: no draw
+  float top;                             // m
+  int children;
+  int token[kDraftMaxNodes];             // theirs, each once
+};
+
 struct VerifyWorkspace {
-  int* node;                             // [B] the node to draw after, or -1
-  float* top;                            // [B] its maximum
+  DrawJob* jobs;                         // [B]
   double* sums;                          // [B, draw chunks]
   RowStat* stats;                        // [B * nodes, stat parts]
 };
 
 __host__ __device__ inline VerifyWorkspace workspace_of(const VerifyParams& p) {
   VerifyWorkspace w;
-  w.sums = reinterpret_cast<double*>(p.workspace);
-  w.stats = reinterpret_cast<RowStat*>(w.sums + (((size_t)p.num_seqs * p.draw_chunks + 1) & ~(size_t)1));
-  w.node = reinterpret_cast<int*>(w.stats + (size_t)p.num_seqs * p.nodes * p.stat_parts);
-  w.top = reinterpret_cast<float*>(w.node + p.num_seqs);
+  w.jobs = reinterpret_cast<DrawJob*>(p.workspace);
+  w.sums = reinterpret_cast<double*>(w.jobs + p.num_seqs);
+  w.stats = reinterpret_cast<RowStat*>(w.sums + (size_t)p.num_seqs * p.draw_chunks);
   return w;
 }
 
@@ -242,58 +265,77 @@ template <typename T> __global__ void __launch_bounds__(kStatThreads) verify_sta
   workspace_of(p).stats[(size_t)row * p.stat_parts + part] = r;
 }
 
-// A work-group per sequence.  STATS: the rows' parts are there.
-template <typename T, bool STATS>
+// A work-group per sequence.  STATS: the rows' parts are there.  NC: nodes of a lane.
+template <typename T, bool STATS, int NC>
 __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(const VerifyParams p) {
   constexpr int kThreads = STATS ? 64 : kWalkThreads;
   constexpr int kWaves = kThreads / 64;
   __shared__ int tokens[kDraftMaxNodes], parents[kDraftMaxNodes];
+  __shared__ float logits[kDraftMaxNodes];                   // of a node's token after its parent
+  __shared__ float uniforms[kDraftMaxNodes];
   __shared__ RowStat red[kWaves];
+  __shared__ u64 keys[STATS ? kDraftMaxNodes : 1];            // the nodes' joined parts
+  __shared__ double totals[STATS ? kDraftMaxNodes : 1];
   __shared__ double red_d[kWaves];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int len = min(max(p.tree_lens[b], 0), p.nodes);
   const int vocab = p.vocab;
   const VerifyWorkspace ws = workspace_of(p);
-  for (int i = tid; i < p.nodes; i += kThreads) {
-    tokens[i] = p.tokens[(size_t)b * p.nodes + i];
-    parents[i] = p.parents[(size_t)b * p.nodes + i];
-  }
   const float temp = temperature_of(p, b);
   const bool sampled = temp > 0.0f;
   const float c = sampled ? kLog2e / temp : 0.0f;
+  const double c64 = sampled ? 1.4426950408889634074 / (double)temp : 0.0;
   int* path = p.path + (size_t)b * p.nodes;
+  const T* row0 = reinterpret_cast<const T*>(p.logits) + (size_t)b * p.nodes * p.row_stride;
+  const RowStat* stats = ws.stats + (size_t)b * p.nodes * p.stat_parts;
+  // what the walk may come to is fetched beforehand: its steps then wait for rows (or nothing) only
+  for (int i = tid; i < p.nodes; i += kThreads) {
+    const int tok = p.tokens[(size_t)b * p.nodes + i], up = p.parents[(size_t)b * p.nodes + i];
+    const bool is = up >= 0 && up < i && i < len && (unsigned)tok < (unsigned)vocab;
+    if (sampled) uniforms[i] = p.uniforms[(size_t)b * p.nodes + i];
+    tokens[i] = tok;
+    parents[i] = is ? up : -1;                               // a node that cannot be taken has no parent
+    if (sampled && is) logits[i] = to_float<T>(row0[(size_t)up * p.row_stride + tok]);
+  }
+  if constexpr (STATS) {
+    for (int i = tid; i < len; i += kThreads) {
+      const RowStat* parts = stats + (size_t)i * p.stat_parts;
+      u64 key = 0;
+      for (int k = 0; k < p.stat_parts; ++k) key = max(key, parts[k].key);
+      const float top = from_order_bits((uint32_t)(key >> 32));
+      double S = 0.0;
+      if (sampled && key != 0 && key != ~0ull)
+        for (int k = 0; k < p.stat_parts; ++k)
+          if (parts[k].m > kNegInf) S += (double)parts[k].s * weight(parts[k].m, top, c);
+      keys[i] = key;
+      totals[i] = S;
+    }
+  }
   __syncthreads();
 
   int count = 0, cur = len > 0 ? 0 : -1, next = -1, draw = -1;
   float M = 0.0f;
+  double mass = 0.0;
   while (cur >= 0) {
     if (tid == 0) path[count] = cur;
     ++count;
-    const size_t row = (size_t)b * p.nodes + cur;
-    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.row_stride;
+    const T* x = row0 + (size_t)cur * p.row_stride;
 
     u64 key = 0;
     double S = 0.0;
     if constexpr (STATS) {
-      const RowStat* parts = ws.stats + row * p.stat_parts;
-      for (int i = lane; i < p.stat_parts; i += 64) key = max(key, parts[i].key);
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) key = max(key, shfl_xor64(key, d));
-      M = key == 0 || key == ~0ull ? 0.0f : to_float<T>(x[(int)~(uint32_t)key]);
-      if (sampled) {
-        for (int i = lane; i < p.stat_parts; i += 64)
-          if (parts[i].m > kNegInf) S += (double)parts[i].s * weight(parts[i].m, M, c);
-        S = wave_sum(S);
-      }
+      key = keys[cur];
+      S = totals[cur];
+      M = from_order_bits((uint32_t)(key >> 32));
     } else {
       const RowStat r = wave_stat(thread_stat<T>(x, vocab, tid, kThreads, c, sampled), c, sampled);
       if (lane == 0) red[wave] = r;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) key = max(key, red[w].key);
-      M = key == 0 || key == ~0ull ? 0.0f : to_float<T>(x[(int)~(uint32_t)key]);
-      if (sampled) {
+      M = from_order_bits((uint32_t)(key >> 32));
+      if (sampled && key != ~0ull) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
           if (red[w].m > kNegInf) S += (double)red[w].s * weight(red[w].m, M, c);
@@ -303,13 +345,12 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
     const int best = (int)~(uint32_t)key;
     if (key == 0 || key == ~0ull || (sampled && M == __builtin_inff())) break;      // next stays -1
 
-    // the children, of equal tokens the first: every wave finds the same
+    // the children: every wave finds the same
     int child[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int i = lane + 64 * n;
-      const bool is = i > cur && i < len && parents[i] == cur && (unsigned)tokens[i] < (unsigned)vocab;
-      child[n] = is ? tokens[i] : -1;
+      child[n] = i < p.nodes && parents[i] == cur ? tokens[i] : -1;
     }
     int go = -1;
     if (!sampled) {
@@ -318,17 +359,33 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
         const u64 hit = __builtin_amdgcn_ballot_w64(child[n] == best);
         if (hit && go < 0) go = 64 * n + __builtin_ctzll(hit);
       }
+      if (go < 0) {
+        next = best;
+        break;
+      }
     } else {
-      const double u = p.uniforms[row];
-      const double c64 = 1.4426950408889634074 / (double)temp;
+      const double u = uniforms[cur];
       double e[NC];
 #pragma unroll
-      for (int n = 0; n < NC; ++n) e[n] = child[n] >= 0 ? weight64(to_float<T>(x[child[n]]), M, c64) : 0.0;
+      for (int n = 0; n < NC; ++n) e[n] = child[n] >= 0 ? weight64(logits[lane + 64 * n], M, c64) : 0.0;
+      // of equal tokens the first counts
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        u64 left = __builtin_amdgcn_ballot_w64(child[n] >= 0);
+        while (left) {
+          const int l = __builtin_ctzll(left);
+          left &= left - 1;
+          const int tok = __builtin_amdgcn_readlane(child[n], l);
+#pragma unroll
+          for (int k = n; k < NC; ++k)
+            if (child[k] == tok && (k > n || lane > l)) child[k] = -1;
+          left &= __builtin_amdgcn_ballot_w64(child[n] >= 0);
+        }
+      }
       // sure: whether u is away from every bound that was met
-      auto choose = [&](double total, double margin, bool& sure, double& mass, int& last) {
+      auto choose = [&](double total, double margin, bool& sure) {
         int found = -1;
         mass = 0.0;
-        last = -1;
         sure = true;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
@@ -336,14 +393,7 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
           while (left && found < 0) {
             const int l = __builtin_ctzll(left);
             left &= left - 1;
-            const int tok = __builtin_amdgcn_readlane(child[n], l);
-            bool before = false;
-#pragma unroll
-            for (int k = 0; k < NC; ++k) before |= child[k] == tok && (k < n || (k == n && lane < l));
-            if (__builtin_amdgcn_ballot_w64(before)) continue;
-            const double mine = lane_value(e[n], l);
-            mass += mine;
-            if (mine > 0.0) last = 64 * n + l;
+            mass += lane_value(e[n], l);
             sure = sure && fabs(u * total - mass) >= margin * total;
             if (u * total < mass) found = 64 * n + l;
           }
@@ -351,9 +401,7 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
         return found;
       };
       bool sure;
-      double mass;
-      int last;
-      go = choose(S, kUnsure, sure, mass, last);
+      go = choose(S, kUnsure, sure);
       if (!sure) {
         double part = 0.0;
         for (int i = tid; i < vocab; i += kThreads) part += weight64(to_float<T>(x[i]), M, c64);
@@ -363,16 +411,28 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
         S = 0.0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) S += red_d[w];
-        go = choose(S, 0.0, sure, mass, last);
-        // nearly all of S is the children's: whether there is anything else to draw
-        if (go < 0 && S - mass <= 0x1p-40 * S) go = last;
+        go = choose(S, 0.0, sure);
         __syncthreads();                 // red_d: read by all
       }
-      if (go < 0) draw = cur;
-    }
-    if (go < 0) {
-      if (!sampled) next = best;
-      break;
+      if (go < 0) {
+        draw = cur;
+        if (wave == 0) {
+          DrawJob& job = ws.jobs[b];
+          int before = 0;
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            const u64 is = __builtin_amdgcn_ballot_w64(child[n] >= 0);
+            if (child[n] >= 0) job.token[before + __popcll(is & ((1ull << lane) - 1))] = child[n];
+            before += __popcll(is);
+          }
+          if (lane == 0) {
+            job.mass = mass;
+            job.top = M;
+            job.children = before;
+          }
+        }
+        break;
+      }
     }
     cur = go;
   }
@@ -380,62 +440,59 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
   if (tid == 0) {
     p.counts[b] = count;
     p.next_tokens[b] = next;
-    if (p.temperatures) {
-      ws.node[b] = draw;
-      ws.top[b] = M;
-    }
+    if (p.temperatures) ws.jobs[b].node = draw;
   }
 }
 
-// Tokens of the children of a node, and whether one lies in a range.
-struct DrawChildren {
+// A draw's row, and this lane's children; all loads at once.
+template <typename T> struct DrawRow {
+  static constexpr int NC = kDraftMaxNodes / 64;
+  const T* x;
+  int node, children, vocab;
   int token[NC];
-  template <typename F> __device__ __forceinline__ DrawChildren(const VerifyParams& p, int b, int node, F keep) {
-    const int len = min(max(p.tree_lens[b], 0), p.nodes);
-    const int lane = threadIdx.x & 63;
+  float top;
+  double c64;
+  __device__ __forceinline__ DrawRow(const VerifyParams& p, const DrawJob& job, int b) {
+    node = job.node;
+    children = job.children;
+    top = job.top;
+    vocab = p.vocab;
+    c64 = 1.4426950408889634074 / (double)p.temperatures[b];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) token[n] = job.token[(threadIdx.x & 63) + 64 * n];      // (past the children: of no meaning)
+    x = reinterpret_cast<const T*>(p.logits) + ((size_t)b * p.nodes + max(node, 0)) * p.row_stride;
+  }
+  // The thread's kDrawPer consecutive elements of a chunk as e, children's and those past the row as 0.
+  __device__ __forceinline__ void elements(int chunk, double (&e)[kDrawPer]) const {
+    const int first = chunk * kDrawChunk + threadIdx.x * kDrawPer, lane = threadIdx.x & 63;
+    float v[kDrawPer];
+#pragma unroll
+    for (int k = 0; k < kDrawPer; ++k) v[k] = to_float<T>(x[min(first + k, vocab - 1)]);
+#pragma unroll
+    for (int k = 0; k < kDrawPer; ++k) e[k] = first + k < vocab ? weight64(v[k], top, c64) : 0.0;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      const int i = lane + 64 * n;
-      token[n] = -1;
-      if (i > node && i < len && p.parents[(size_t)b * p.nodes + i] == node) token[n] = keep(p.tokens[(size_t)b * p.nodes + i]);
+      const int at = token[n] - chunk * kDrawChunk;
+      u64 in = __builtin_amdgcn_ballot_w64(lane + 64 * n < children && (unsigned)at < (unsigned)kDrawChunk);
+      while (in) {
+        const int off = __builtin_amdgcn_readlane(at, __builtin_ctzll(in)) - (int)threadIdx.x * kDrawPer;
+        in &= in - 1;
+#pragma unroll
+        for (int k = 0; k < kDrawPer; ++k)
+          if (off == k) e[k] = 0.0;
+      }
     }
   }
 };
-
-// A thread's kDrawPer consecutive elements of a chunk as e, children's and those past the row as 0.
-template <typename T>
-__device__ __forceinline__ void draw_elements(const VerifyParams& p, int b, int node, float M, double c64, int chunk,
-                                              double (&e)[kDrawPer]) {
-  const T* x = reinterpret_cast<const T*>(p.logits) + ((size_t)b * p.nodes + node) * p.row_stride;
-  const int first = chunk * kDrawChunk + threadIdx.x * kDrawPer;
-  float v[kDrawPer];
-#pragma unroll
-  for (int k = 0; k < kDrawPer; ++k) v[k] = to_float<T>(x[min(first + k, p.vocab - 1)]);
-  const DrawChildren children(p, b, node, [](int t) { return t; });
-#pragma unroll
-  for (int k = 0; k < kDrawPer; ++k) e[k] = first + k < p.vocab ? weight64(v[k], M, c64) : 0.0;
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const int at = children.token[n] - chunk * kDrawChunk;
-    u64 in = __builtin_amdgcn_ballot_w64(children.token[n] >= 0 && (unsigned)at < (unsigned)kDrawChunk);
-    while (in) {
-      const int off = __builtin_amdgcn_readlane(at, __builtin_ctzll(in)) - (int)threadIdx.x * kDrawPer;
-      in &= in - 1;
-#pragma unroll
-      for (int k = 0; k < kDrawPer; ++k)
-        if (off == k) e[k] = 0.0;
-    }
-  }
-}
 
 template <typename T> __global__ void __launch_bounds__(kDrawThreads) verify_rest_kernel(const VerifyParams p) {
   __shared__ double red[kDrawThreads / 64];
   const int chunk = blockIdx.x, b = blockIdx.y;
   const VerifyWorkspace ws = workspace_of(p);
-  const int node = ws.node[b];
-  if (node < 0) return;
+  const DrawRow<T> row(p, ws.jobs[b], b);
+  if (row.node < 0) return;
   double e[kDrawPer];
-  draw_elements<T>(p, b, node, ws.top[b], 1.4426950408889634074 / (double)temperature_of(p, b), chunk, e);
+  row.elements(chunk, e);
   double sum = 0.0;
 #pragma unroll
   for (int k = 0; k < kDrawPer; ++k) sum += e[k];
@@ -457,38 +514,17 @@ template <typename T> __global__ void __launch_bounds__(kDrawThreads) verify_dra
   const int b = blockIdx.x, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const VerifyWorkspace ws = workspace_of(p);
-  const int node = ws.node[b];
-  if (node < 0) return;
-  const float M = ws.top[b];
-  const double c64 = 1.4426950408889634074 / (double)temperature_of(p, b);
-  const T* x = reinterpret_cast<const T*>(p.logits) + ((size_t)b * p.nodes + node) * p.row_stride;
+  const DrawRow<T> row(p, ws.jobs[b], b);
+  if (row.node < 0) return;
   const double* sums = ws.sums + (size_t)b * p.draw_chunks;
-
-  // the children's mass, of equal tokens once: every wave finds the same
-  const int vocab = p.vocab;
-  const DrawChildren children(p, b, node, [vocab](int t) { return (unsigned)t < (unsigned)vocab ? t : -1; });
-  double mass = 0.0;
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const double e = children.token[n] >= 0 ? weight64(to_float<T>(x[children.token[n]]), M, c64) : 0.0;
-    u64 left = __builtin_amdgcn_ballot_w64(children.token[n] >= 0);
-    while (left) {
-      const int l = __builtin_ctzll(left);
-      left &= left - 1;
-      const int tok = __builtin_amdgcn_readlane(children.token[n], l);
-      bool before = false;
-#pragma unroll
-      for (int k = 0; k < NC; ++k) before |= children.token[k] == tok && (k < n || (k == n && lane < l));
-      if (!__builtin_amdgcn_ballot_w64(before)) mass += lane_value(e, l);
-    }
-  }
+  const double mass = ws.jobs[b].mass;
+  const double u = p.uniforms[(size_t)b * p.nodes + row.node];
   // the rest's chunks: every wave sums and searches them for itself
   const int per = (p.draw_chunks + 63) / 64;
   double mine = 0.0;
   for (int k = 0; k < per; ++k) mine += lane * per + k < p.draw_chunks ? sums[lane * per + k] : 0.0;
   const double upto = wave_prefix(mine, lane);
   const double rest = lane_value(upto, 63);
-  const double u = p.uniforms[(size_t)b * p.nodes + node];
   const double target = u * (mass + rest) - mass;
   u64 past = __builtin_amdgcn_ballot_w64(upto > target && mine > 0.0);
   if (!past) {                                            // u of 1: the last token
@@ -509,7 +545,7 @@ template <typename T> __global__ void __launch_bounds__(kDrawThreads) verify_dra
     before += s;
   }
   double e[kDrawPer];
-  draw_elements<T>(p, b, node, M, c64, chunk, e);
+  row.elements(chunk, e);
   double own = 0.0;
 #pragma unroll
   for (int k = 0; k < kDrawPer; ++k) own += e[k];
@@ -538,15 +574,18 @@ template <typename T> __global__ void __launch_bounds__(kDrawThreads) verify_dra
   if (any >= 0) atomicMin(&lowest, first + any);
   __syncthreads();
   // none where the target lies below the chunk's first token by a rounding
-  if (tid == 0) p.next_tokens[b] = found >= 0 ? found : lowest;
+  if (tid == 0) p.next_tokens[b] = found >= 0 ? found : lowest == 0x7fffffff ? -1 : lowest;
 }
 
 int stat_size(int dtype) { return kStatThreads * kStatVecs * 16 / (dtype == kF32 ? 4 : 2); }
 
-// Whether the rows of all nodes are read first.
+// Whether the rows of all nodes are read first: at 5.2 GB/ms, against seven steps of a walk, each 0.9 us and 36 ns for a KiB of
+// its row (paths are about so long; their lengths are known on the device only).  MI355X, us, all rows / walk, trees with
+// paths of up to 7 nodes: greedy, 32000 fp32 logits: 16 x 32 nodes 19 / 26, 64 x 16 27.5 / 29, 64 x 32 48 / 29; 128256 bf16:
+// 8 x 64 27 / 48, 64 x 16 50 / 72; sampled, 2 x 32 of 128256 bf16 31 / 74.
 bool all_rows(int num_seqs, int nodes, int vocab, int dtype) {
-  const long long rows = (long long)num_seqs * nodes;
-  return rows <= 1 << 20 && rows * vocab * (dtype == kF32 ? 4 : 2) <= 64LL << 20;
+  const long long rows = (long long)num_seqs * nodes, row = (long long)vocab * (dtype == kF32 ? 4 : 2);
+  return rows <= 1 << 20 && rows * row / 5.2e6 + 4.0 <= 7.0 * (0.9 + row / 1024.0 * 0.036);
 }
 
 void plan(VerifyParams& p, int dtype) {
@@ -555,13 +594,17 @@ void plan(VerifyParams& p, int dtype) {
   p.stat_parts = all_rows(p.num_seqs, p.nodes, p.vocab, dtype) ? (p.vocab + p.stat_size - 1) / p.stat_size : 0;
 }
 
+template <typename T, int NC> void launch_walk(const VerifyParams& p, hipStream_t s) {
+  if (p.stat_parts) hipLaunchKernelGGL((verify_walk_kernel<T, true, NC>), dim3(p.num_seqs), dim3(64), 0, s, p);
+  else hipLaunchKernelGGL((verify_walk_kernel<T, false, NC>), dim3(p.num_seqs), dim3(kWalkThreads), 0, s, p);
+}
+
 template <typename T> void launch_of(const VerifyParams& p, hipStream_t s) {
-  if (p.stat_parts) {
+  if (p.stat_parts)
     hipLaunchKernelGGL(verify_stats_kernel<T>, dim3(p.num_seqs * p.nodes, p.stat_parts), dim3(kStatThreads), 0, s, p);
-    hipLaunchKernelGGL((verify_walk_kernel<T, true>), dim3(p.num_seqs), dim3(64), 0, s, p);
-  } else {
-    hipLaunchKernelGGL((verify_walk_kernel<T, false>), dim3(p.num_seqs), dim3(kWalkThreads), 0, s, p);
-  }
+  if (p.nodes <= 64) launch_walk<T, 1>(p, s);
+  else if (p.nodes <= 128) launch_walk<T, 2>(p, s);
+  else launch_walk<T, 4>(p, s);
   if (p.temperatures) {
     hipLaunchKernelGGL(verify_rest_kernel<T>, dim3(p.draw_chunks, p.num_seqs), dim3(kDrawThreads), 0, s, p);
     hipLaunchKernelGGL(verify_draw_kernel<T>, dim3(p.num_seqs), dim3(kDrawThreads), 0, s, p);
@@ -576,7 +619,7 @@ size_t verify_workspace_bytes(int num_seqs, int nodes, int vocab, int dtype) {
   p.nodes = nodes;
   p.vocab = vocab;
   plan(p, dtype);
-  return reinterpret_cast<uintptr_t>(workspace_of(p).top + num_seqs);
+  return reinterpret_cast<uintptr_t>(workspace_of(p).stats + (size_t)num_seqs * nodes * p.stat_parts);
 }
 
 void launch_verify(VerifyParams p, int dtype, hipStream_t s) {

@@ -34,25 +34,24 @@ class DraftTreeLayout(NamedTuple):
     slots: torch.Tensor       # [B, T] int32
 
 
-def check_tree_tensors(index, b, t, **tensors):
-    """Raises ValueError unless each tensor is dense int32 on device ``index``: [B, T] by the names parents,
-    tokens and path, [B] by the others."""
-    for name, x in tensors.items():
-        shape = (b, t) if name in ("parents", "tokens", "path") else (b,)
-        if x.dtype != torch.int32 or tuple(x.shape) != shape or not x.is_contiguous():
+def check_int32(index, shape, *named):
+    """Raises ValueError unless each (name, tensor) is dense int32 of ``shape`` on device ``index``."""
+    for name, x in named:
+        if x.dtype is not torch.int32 or x.shape != shape or not x.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {x.dtype} {list(x.shape)}")
         if x.get_device() != index:
             raise ValueError("all tensors must be on one HIP device")
 
 
 def check_block_tables(index, b, block_tables):
-    """Raises ValueError unless block_tables is dense int32 [B, columns] on device ``index``."""
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != b or \
-            block_tables.shape[1] < 1 or not block_tables.is_contiguous():
-        raise ValueError(f"block_tables must be contiguous int32 [{b}, columns], got {block_tables.dtype} "
-                         f"{list(block_tables.shape)}")
+    """Raises ValueError unless block_tables is dense int32 [B, columns] on device ``index``; the columns."""
+    shape = block_tables.shape
+    if block_tables.dtype is not torch.int32 or len(shape) != 2 or shape[0] != b or shape[1] < 1 or \
+            not block_tables.is_contiguous():
+        raise ValueError(f"block_tables must be contiguous int32 [{b}, columns], got {block_tables.dtype} {list(shape)}")
     if block_tables.get_device() != index:
         raise ValueError("all tensors must be on one HIP device")
+    return shape[1]
 
 
 def draft_tree_layout(parents, tree_lens, context_lens, block_tables, block_size, num_blocks):
@@ -68,17 +67,16 @@ def draft_tree_layout(parents, tree_lens, context_lens, block_tables, block_size
     index = parents.get_device()
     if index < 0:
         raise ValueError(f"tensors must live on a HIP device (got {parents.device})")
-    if parents.dim() != 2 or not 1 <= parents.shape[1] <= MAX_NODES:
-        raise ValueError(f"parents must be [B, T] with T of 1 to {MAX_NODES}, got {list(parents.shape)}")
-    b, t = parents.shape
-    check_tree_tensors(index, b, t, parents=parents, tree_lens=tree_lens, context_lens=context_lens)
-    check_block_tables(index, b, block_tables)
-    dev = parents.device
-    mask = torch.empty((b, t, (t + 63) // 64), dtype=torch.int64, device=dev)
-    positions = torch.empty((b, t), dtype=torch.int32, device=dev)
-    slots = torch.empty((b, t), dtype=torch.int32, device=dev)
+    shape = parents.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_NODES:
+        raise ValueError(f"parents must be [B, T] with T of 1 to {MAX_NODES}, got {list(shape)}")
+    b, t = shape
+    check_int32(index, shape, ("parents", parents))
+    check_int32(index, shape[:1], ("tree_lens", tree_lens), ("context_lens", context_lens))
+    columns = check_block_tables(index, b, block_tables)
+    mask = parents.new_empty((b, t, (t + 63) // 64), dtype=torch.int64)
+    positions, slots = torch.empty_like(parents), torch.empty_like(parents)
     _lib.call("draft_tree_layout", index, _lib.load().tv_draft_tree_layout,
               mask.data_ptr(), positions.data_ptr(), slots.data_ptr(), parents.data_ptr(), tree_lens.data_ptr(),
-              context_lens.data_ptr(), block_tables.data_ptr(), b, t, block_tables.shape[1], int(block_size),
-              int(num_blocks))
+              context_lens.data_ptr(), block_tables.data_ptr(), b, t, columns, int(block_size), int(num_blocks))
     return DraftTreeLayout(mask, positions, slots)

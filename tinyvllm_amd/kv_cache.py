@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .draft_tree import check_block_tables, check_tree_tensors
+from .draft_tree import check_block_tables, check_int32
 
 _lib.load()
 
@@ -305,16 +305,19 @@ def reshape_and_cache(k_cache, v_cache, k, v, slot_mapping, err_count=None):
     _lib.check(rc, "reshape_and_cache")
 
 
-def _token_stride(x, heads, d, name):
-    """Elements between the tokens of x [N, heads, d]; raises unless a token's heads are dense."""
-    if x.dim() != 3 or tuple(x.shape[1:]) != (heads, d):
-        raise ValueError(f"{name} must be [N, {heads}, {d}], got {list(x.shape)}")
-    stride = x.stride()                 # a dimension of size 1 may have any
-    if (stride[2] != 1 and d > 1) or (stride[1] != d and heads > 1):
+def _token_stride(x, shape, name):
+    """Elements between the tokens of x, which has to be of ``shape`` [N, heads, d] with dense heads."""
+    if x.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(x.shape)}")
+    n, heads, d = shape
+    s0, s1, s2 = x.stride()             # a dimension of size 1 may have any
+    if (s2 != 1 and d > 1) or (s1 != d and heads > 1):
         raise ValueError(f"{name}: heads and head_dim must be contiguous")
-    if x.shape[0] > 1 and stride[0] < heads * d:
+    if n <= 1:
+        return heads * d
+    if s0 < heads * d:
         raise ValueError(f"{name}: tokens overlap")
-    return stride[0] if x.shape[0] > 1 else heads * d
+    return s0
 
 
 def rope_and_cache(k_cache, v_cache, q, k, v, slot_mapping, positions, rope, *, pairs="adjacent", out=None,
@@ -335,41 +338,47 @@ def rope_and_cache(k_cache, v_cache, q, k, v, slot_mapping, positions, rope, *, 
     index = k_cache.get_device()
     if index < 0:
         raise ValueError(f"the cache must be on a HIP device (got {k_cache.device})")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache / v_cache must be dense [NB, bs, Hkv, D] tensors of one shape")
-    nb, bs, hkv, d = k_cache.shape
+    nb, bs, hkv, d = shape
     if q.dim() != 3:
         raise ValueError(f"q must be [N, Hq, {d}], got {list(q.shape)}")
-    n, hq = q.shape[:2]
-    strides = [_token_stride(x, h, d, name) for x, h, name in ((q, hq, "q"), (k, hkv, "k"), (v, hkv, "v"))]
-    if k.shape[0] != n or v.shape[0] != n:
+    n, hq, _ = q.shape
+    if len(k) != n or len(v) != n:
         raise ValueError("q, k and v must hold the same number of tokens")
+    q_stride = _token_stride(q, (n, hq, d), "q")
+    k_stride, v_stride = _token_stride(k, (n, hkv, d), "k"), _token_stride(v, (n, hkv, d), "v")
     dtype = k_cache.dtype
-    if not (v_cache.dtype == q.dtype == k.dtype == v.dtype == dtype):
+    if not (v_cache.dtype is dtype and q.dtype is dtype and k.dtype is dtype and v.dtype is dtype):
         raise ValueError("q, k, v and the caches must share a dtype")
-    for x, name in ((slot_mapping, "slot_mapping"), (positions, "positions")):
-        if x.dtype != torch.int32 or x.numel() != n or not x.is_contiguous():
-            raise ValueError(f"{name} must be contiguous int32 with one entry per token")
-    if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous():
+    if slot_mapping.dtype is not torch.int32 or slot_mapping.numel() != n or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int32 with one entry per token")
+    if positions.dtype is not torch.int32 or positions.numel() != n or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 with one entry per token")
+    if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous():
         raise ValueError("rope must be contiguous float32 [positions, pairs, 2]")
-    if not 1 <= 2 * rope.shape[1] <= d or rope.shape[0] < 1:
-        raise ValueError(f"rope of {rope.shape[1]} pairs does not fit head_dim {d}")
+    rope_len, half, _ = rope.shape
+    if not 1 <= 2 * half <= d or rope_len < 1:
+        raise ValueError(f"rope of {half} pairs does not fit head_dim {d}")
     if pairs not in ("adjacent", "halves"):
         raise ValueError(f"pairs must be 'adjacent' or 'halves', got {pairs!r}")
     check_devices(index, v_cache, q, k, v, slot_mapping, positions, rope)
     if out is None:
-        out = torch.empty((n, hq, d), dtype=dtype, device=q.device)
-    elif out.dtype != dtype or tuple(out.shape) != (n, hq, d) or out.get_device() != index:
-        raise ValueError("out must be like q")
-    out_stride = _token_stride(out, hq, d, "out")
+        out = q.new_empty((n, hq, d))
+        out_stride = hq * d
+    else:
+        if out.dtype is not dtype or out.shape != q.shape or out.get_device() != index:
+            raise ValueError("out must be like q")
+        out_stride = _token_stride(out, (n, hq, d), "out")
     if err_count is not None and (err_count.get_device() != index or
                                   err_count.dtype not in (torch.int32, torch.uint32)):
         raise ValueError("err_count must be an int32/uint32 tensor on the cache's device")
     _lib.call("rope_and_cache", index, _lib.load().tv_rope_and_cache,
               out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-              slot_mapping.data_ptr(), positions.data_ptr(), rope.data_ptr(), rope.shape[0], 2 * rope.shape[1],
-              1 if pairs == "halves" else 0, n, hq, hkv, d, bs, nb, out_stride, *strides, _lib.dtype_code(dtype),
-              err_count.data_ptr() if err_count is not None else None)
+              slot_mapping.data_ptr(), positions.data_ptr(), rope.data_ptr(), rope_len, 2 * half,
+              1 if pairs == "halves" else 0, n, hq, hkv, d, bs, nb, out_stride, q_stride, k_stride, v_stride,
+              _lib.dtype_code(dtype), err_count.data_ptr() if err_count is not None else None)
     return out
 
 
@@ -383,26 +392,28 @@ def keep_draft_rows(k_caches, v_caches, path, counts, context_lens, block_tables
     positions that the table does not reach, or whose block is outside the cache, are not moved.  Other rows stay as
     they are.
     """
-    if len(k_caches) != len(v_caches) or not k_caches:
+    n = len(k_caches)
+    if n == 0 or len(v_caches) != n:
         raise ValueError("k_caches and v_caches must hold one tensor per layer each")
     first = k_caches[0]
-    index = first.get_device()
+    shape, dtype, index = first.shape, first.dtype, first.get_device()
     if index < 0:
         raise ValueError(f"the caches must be on a HIP device (got {first.device})")
-    if first.dim() != 4:
+    if len(shape) != 4:
         raise ValueError("caches must be dense [NB, bs, Hkv, D] tensors")
     for c in (*k_caches, *v_caches):
-        if c.shape != first.shape or c.dtype != first.dtype or not c.is_contiguous():
+        if c.shape != shape or c.dtype is not dtype or not c.is_contiguous():
             raise ValueError("caches must be dense tensors of one shape and dtype")
-    check_devices(index, *k_caches, *v_caches)
-    if path.dim() != 2 or path.shape[1] < 1:
-        raise ValueError(f"path must be [B, T], got {list(path.shape)}")
-    b, t = path.shape
-    check_tree_tensors(index, b, t, path=path, counts=counts, context_lens=context_lens)
-    check_block_tables(index, b, block_tables)
-    nb, bs, hkv, d = first.shape
-    n = len(k_caches)
-    arrays = [(ctypes.c_void_p * n)(*[c.data_ptr() for c in cs]) for cs in (k_caches, v_caches)]
-    _lib.call("keep_draft_rows", index, _lib.load().tv_keep_draft_rows, *arrays, n, path.data_ptr(), counts.data_ptr(),
-              context_lens.data_ptr(), block_tables.data_ptr(), b, t, block_tables.shape[1], hkv, d, bs, nb,
-              _lib.dtype_code(first.dtype))
+        if c.get_device() != index:
+            raise ValueError("all tensors must be on the cache's device")
+    tree = path.shape
+    if len(tree) != 2 or tree[1] < 1:
+        raise ValueError(f"path must be [B, T], got {list(tree)}")
+    check_int32(index, tree, ("path", path))
+    check_int32(index, tree[:1], ("counts", counts), ("context_lens", context_lens))
+    columns = check_block_tables(index, tree[0], block_tables)
+    nb, bs, hkv, d = shape
+    array = ctypes.c_void_p * n
+    _lib.call("keep_draft_rows", index, _lib.load().tv_keep_draft_rows, array(*[c.data_ptr() for c in k_caches]),
+              array(*[c.data_ptr() for c in v_caches]), n, path.data_ptr(), counts.data_ptr(), context_lens.data_ptr(),
+              block_tables.data_ptr(), *tree, columns, hkv, d, bs, nb, _lib.dtype_code(dtype))

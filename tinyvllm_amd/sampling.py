@@ -10,7 +10,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .draft_tree import MAX_NODES, check_tree_tensors
+from .draft_tree import MAX_NODES, check_int32
 
 _lib.load()
 
@@ -97,7 +97,8 @@ def verify_draft_tree(logits, tokens, parents, tree_lens, *, temperatures=None, 
         raise ValueError(f"logits must be [B, T, V] with T of 1 to {MAX_NODES}, got {list(logits.shape)}")
     b, t, v = logits.shape
     code = _lib.dtype_code(logits.dtype)
-    check_tree_tensors(index, b, t, tokens=tokens, parents=parents, tree_lens=tree_lens)
+    check_int32(index, (b, t), ("tokens", tokens), ("parents", parents))
+    check_int32(index, (b,), ("tree_lens", tree_lens))
     if logits.stride(2) != 1 and v > 1:
         raise ValueError("the vocabulary must be contiguous")
     try:
@@ -110,12 +111,9 @@ def verify_draft_tree(logits, tokens, parents, tree_lens, *, temperatures=None, 
         for x, name, shape in ((temperatures, "temperatures", (b,)), (uniforms, "uniforms", (b, t))):
             if x.dtype != torch.float32 or tuple(x.shape) != shape or not x.is_contiguous() or x.get_device() != index:
                 raise ValueError(f"{name} must be contiguous float32 {list(shape)} on the logits' device")
-    dev = logits.device
-    path = torch.empty((b, t), dtype=torch.int32, device=dev)
-    counts = torch.empty((b,), dtype=torch.int32, device=dev)
-    following = torch.empty_like(counts)
+    path, counts, following = torch.empty_like(tokens), torch.empty_like(tree_lens), torch.empty_like(tree_lens)
     need = _lib.device_size("tv_verify_draft_tree_workspace_bytes", index, b, t, v, code)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     _lib.call("verify_draft_tree", index, _lib.load().tv_verify_draft_tree,
               path.data_ptr(), counts.data_ptr(), following.data_ptr(), logits.data_ptr(), tokens.data_ptr(),
               parents.data_ptr(), tree_lens.data_ptr(), temperatures.data_ptr() if temperatures is not None else None,
