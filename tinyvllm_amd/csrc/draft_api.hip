@@ -144,7 +144,7 @@ size_t tv_paged_tree_workspace_bytes(int num_seqs, int nodes, int num_heads, int
     return 0;
   const int rows = tree_info((long long)nodes * (num_heads / num_kv_heads), head_dim, dtype).tile_rows;
   const size_t groups = std::max(1, work_groups / num_kv_heads);
-  return 2 * groups * num_kv_heads * rows * (head_dim + 2) * sizeof(float) + ((size_t)num_seqs + 1) * sizeof(long long);
+  return 2 * groups * num_kv_heads * rows * (head_dim + 2) * sizeof(float) + ((size_t)num_seqs + 1) * sizeof(int);
 }
 
 int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv_heads, int head_dim, int max_blocks,
@@ -169,7 +169,8 @@ int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv
   // 1 x 64 over 8000 134 / 23; in fp32 4 x 8 over 17..250 17 / 11.
   const long long cost = dtype == TV_F32 ? 6 : head_dim == 64 ? 12 : 8;
   const long long undealt = (units + slots - 1) / slots * tiles, dealt = units * tiles / slots + cost;
-  return dealt < undealt || tiles >= 6 * cost ? (int)slots : 0;
+  const bool counted = ((long long)max_blocks * block_size / 16 + 1) * ((rows + 63) / 64) * num_seqs <= 0x7fffffff;
+  return counted && (dealt < undealt || tiles >= 6 * cost) ? (int)slots : 0;
 }
 
 int tv_paged_tree(void* out, const void* queries, const void* k_cache, const void* v_cache,
@@ -211,9 +212,9 @@ int tv_paged_tree(void* out, const void* queries, const void* k_cache, const voi
     return fail(TV_EINVAL, "%s: workspace of %zu bytes, 16-byte aligned, required (got %zu)", who, need, workspace_bytes);
   const long long rows = (long long)nodes * (num_heads / num_kv_heads);
   const long long units = (rows + 63) / 64 * num_kv_heads * num_seqs;
-  // at most 512 threads each in one dimension of fewer than 2^32; a work-group counts its tiles in 32 bits
+  // 256 threads each in one dimension of fewer than 2^32; tiles are counted in 32 bits
   if (num_kv_heads > 65535 || rows > 1 << 22 || units >= 1 << 23 ||
-      (work_groups && (width / 16 + 1) * units / work_groups > 0x3fffffff))
+      (work_groups && (width / 16 + 1) * (units / num_kv_heads) > 0x7fffffff))
     return fail(TV_EINVAL, "%s: grid too large", who);
   tv::TreeParams p{};
   p.out = out;

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
   constexpr int RPP = WAVES * RPI;             // rows of all waves' loads
   static_assert(NV * THREADS == BN * CPR && NV >= 1 && NV * NS <= 64, "tile shape");
   __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE];
-  __shared__ long long wave_tiles[WAVES];
+  __shared__ int wave_tiles[WAVES];
   __shared__ int start_seq, start_tile;        // the work-group's first tile
 
   const uint32_t smem_at = sgpr((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem);
@@ -118,40 +118,40 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
     // the heads of a group read the same keys' neighbouring slices of the cache's rows at about the same time
     const int group = wg / p.num_kv_heads;
     kh = wg - group * p.num_kv_heads;
-    // prefix sums of the sequences' tiles: a thread has `per` consecutive sequences
+    // prefix sums of the sequences' tiles (fewer than 2^31): a thread has `per` consecutive sequences
     const int per = (p.num_seqs + THREADS - 1) / THREADS;
     auto tiles_of = [&](int b) -> int {
       if (b >= p.num_seqs) return 0;
       const int ctx = min(max(p.context_lens[b], 0), p.width), len = min(max(p.tree_lens[b], 0), p.nodes);
       return (min(ctx + len, p.width) + BN - 1) / BN * ((len * G + BM - 1) / BM);
     };
-    long long mine = 0;
-    for (int k = 0; k < per; ++k) mine += tiles_of(tid * per + k);
-    long long upto = mine;
+    const int one = tiles_of(tid * per);
+    int mine = one;
+    for (int k = 1; k < per; ++k) mine += tiles_of(tid * per + k);
+    int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const int lo = __builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)(uint32_t)(unsigned long long)upto);
-      const int hi = __builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)((unsigned long long)upto >> 32));
-      if (lane >= d) upto += (long long)((unsigned long long)(uint32_t)hi << 32 | (uint32_t)lo);
+      const int other = __builtin_amdgcn_ds_bpermute((lane - d) << 2, upto);
+      if (lane >= d) upto += other;
     }
     if (lane == 63) wave_tiles[wave] = upto;
     if (tid == 0) start_seq = -1;
     __syncthreads();
-    long long total = 0, before = upto - mine;
+    int total = 0, before = upto - mine;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       if (w < wave) before += wave_tiles[w];
       total += wave_tiles[w];
     }
-    const long long share = max((total + p.groups - 1) / p.groups, (long long)p.least_tiles);
-    const long long from = share * group, to = min(from + share, total);
+    const int share = max((int)(((unsigned)total + p.groups - 1) / (unsigned)p.groups), p.least_tiles);
+    const long long from = (long long)share * group;
+    const int here = from < total ? (int)from : total;       // a group past the last tile has none
     for (int k = 0; k < per; ++k) {
-      const int b = tid * per + k;
-      const long long n = tiles_of(b);
+      const int b = tid * per + k, n = k ? tiles_of(b) : one;
       if (wg == 0 && b < p.num_seqs) p.first_tiles[b] = before;
-      if (from >= before && from < before + n) {
+      if (here >= before && here < before + n) {
         start_seq = b;
-        start_tile = (int)(from - before);
+        start_tile = here - before;
       }
       before += n;
     }
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
     __syncthreads();
     const int b0 = __builtin_amdgcn_readfirstlane(start_seq);
     if (b0 < 0) return;                        // no tiles are left for it
-    left = __builtin_amdgcn_readfirstlane((int)(to - from));
+    left = uniform(min(share, total - here));
     tile = __builtin_amdgcn_readfirstlane(start_tile);
     cu = unit_of(b0);
     cu.rt = uniform(tile / cu.tiles);
@@ -524,13 +524,18 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
 }
 
 // Joins the parts of a unit's rows that several work-groups have: out = sum w_s o_s / sum w_s, w_s = l_s 2^(m_s - max m).
-template <typename T, int D>
+// A work-group has rows of one row tile, whose parts are then the same for all its threads.
+template <typename T, int D, int TILE_ROWS>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
   constexpr int TPR = D / 4;                   // threads of a row
+  constexpr int ROWS = 256 / TPR;
+  static_assert(TILE_ROWS % ROWS == 0, "rows of a work-group");
   const int b = blockIdx.z, kh = blockIdx.y;
   const int G = p.group;
-  const int len = min(max(p.tree_lens[b], 0), p.nodes);
-  const int row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int len = min(max(uniform_load(p.tree_lens + b), 0), p.nodes);
+  const int ctx = min(max(uniform_load(p.context_lens + b), 0), p.width);
+  const int share = uniform_load(p.first_tiles + p.num_seqs), first = uniform_load(p.first_tiles + b);
+  const int row = blockIdx.x * ROWS + threadIdx.x / TPR;
   if (row >= p.nodes * G) return;
   const int d = (threadIdx.x % TPR) * 4;
   const int node = row / G;
@@ -542,19 +547,18 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
       *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + out_at) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
   };
   if (node >= len) return store(f32x4{0.f, 0.f, 0.f, 0.f});      // padding
-  const int ctx = min(max(p.context_lens[b], 0), p.width);
-  const int tiles = (min(ctx + len, p.width) + p.tile_keys - 1) / p.tile_keys;
-  const int rt = row / p.tile_rows;
-  const long long share = p.first_tiles[p.num_seqs], from = p.first_tiles[b] + (long long)rt * tiles;
-  const int g0 = (int)(from / share), g1 = (int)((from + tiles - 1) / share);
+  const unsigned tiles = (unsigned)(min(ctx + len, p.width) + p.tile_keys - 1) / p.tile_keys;
+  const unsigned rt = blockIdx.x * ROWS / TILE_ROWS;
+  const unsigned from = first + rt * tiles;
+  const int g0 = from / (unsigned)share, g1 = (from + tiles - 1) / (unsigned)share;
   if (g0 == g1) return;                        // written already
   const int parts = g1 - g0 + 1;
   // a part that begins where its work-group does is that one's first, others its second.  Within 16 rows the values
   // lie as the kernel's accumulators do, [D / 16][16 rows][16]
+  const bool second = from > (unsigned)share * g0;
   auto place = [&](int s) -> size_t {
-    const int g = g0 + s;
-    const size_t slot = 2 * ((size_t)g * p.num_kv_heads + kh) + (s == 0 && from > share * g ? 1 : 0);
-    return slot * p.tile_rows + row - rt * p.tile_rows;
+    const unsigned slot = 2 * ((unsigned)(g0 + s) * p.num_kv_heads + kh) + (s == 0 && second ? 1 : 0);
+    return (size_t)slot * TILE_ROWS + (row - rt * TILE_ROWS);
   };
   f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
   float den = 0.0f, M = kNegInf;
@@ -608,7 +612,7 @@ template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool N
       p.groups = std::max(1, p.work_groups / p.num_kv_heads);
       p.work_groups = p.groups * p.num_kv_heads;
       p.part_ml = p.part_o + (size_t)2 * p.work_groups * kRows * D;
-      p.first_tiles = reinterpret_cast<long long*>(p.part_ml + (size_t)4 * p.work_groups * kRows);
+      p.first_tiles = reinterpret_cast<int*>(p.part_ml + (size_t)4 * p.work_groups * kRows);
     }
     const dim3 grid(p.work_groups ? p.work_groups : (unsigned)((long long)p.row_tiles * p.num_kv_heads * p.num_seqs));
     if (p.bs_log2 >= 4)
@@ -617,7 +621,7 @@ template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool N
       hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, false>), grid, dim3(kThreads), 0, s, p);
     if (p.work_groups) {
       constexpr int per = 256 / (D / 4);
-      hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((rows + per - 1) / per, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((tree_merge_kernel<T, D, kRows>), dim3((rows + per - 1) / per, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
     }
   }
   static long long resident() {

@@ -63,7 +63,7 @@ struct TreeParams {
   int tile_rows, tile_keys;
   float* part_o;             // [work_groups, 2, tile_rows, D] normalised parts: of a work-group's first unit, of a later one
   float* part_ml;            // [work_groups, 2, tile_rows, 2] (max in log2 units, sum)
-  long long* first_tiles;    // [B + 1] tiles of the sequences before; then the tiles of a group
+  int* first_tiles;          // [B + 1] tiles of the sequences before; then the tiles of a group
 };
 
 struct VerifyParams {
