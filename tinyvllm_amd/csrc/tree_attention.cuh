@@ -524,77 +524,87 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
 }
 
 // Joins the parts of a unit's rows that several work-groups have: out = sum w_s o_s / sum w_s, w_s = l_s 2^(m_s - max m).
-// A work-group has rows of one row tile, whose parts are then the same for all its threads.
+// A work-group has 16 rows of a row tile, whose parts are the same for all its threads, in the order in which the kernel's
+// accumulators left them, [D / 16][16 rows][16].
 template <typename T, int D, int TILE_ROWS>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
-  constexpr int TPR = D / 4;                   // threads of a row
-  constexpr int ROWS = 256 / TPR;
-  static_assert(TILE_ROWS % ROWS == 0, "rows of a work-group");
+  constexpr int R = D / 64;                    // 16-byte vectors a thread, of one row
   const int b = blockIdx.z, kh = blockIdx.y;
   const int G = p.group;
   const int len = min(max(uniform_load(p.tree_lens + b), 0), p.nodes);
   const int ctx = min(max(uniform_load(p.context_lens + b), 0), p.width);
   const int share = uniform_load(p.first_tiles + p.num_seqs), first = uniform_load(p.first_tiles + b);
-  const int row = blockIdx.x * ROWS + threadIdx.x / TPR;
+  const int tid = threadIdx.x;
+  const int row = blockIdx.x * 16 + tid / 4 % 16;
   if (row >= p.nodes * G) return;
-  const int d = (threadIdx.x % TPR) * 4;
   const int node = row / G;
+  const int d = tid / 64 * 16 + tid % 4 * 4;   // and 64 on, for every further vector
   const size_t out_at = (((size_t)b * p.nodes + node) * p.num_kv_heads * G + (size_t)kh * G + row - node * G) * D + d;
-  auto store = [&](f32x4 x) {
+  auto store = [&](int r, f32x4 x) {
     if (sizeof(T) == 4 || p.out_dtype == kF32)
-      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + out_at) = x;
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + out_at + 64 * r) = x;
     else if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + out_at) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+      *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + out_at + 64 * r) =
+          u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
   };
-  if (node >= len) return store(f32x4{0.f, 0.f, 0.f, 0.f});      // padding
-  const unsigned tiles = (unsigned)(min(ctx + len, p.width) + p.tile_keys - 1) / p.tile_keys;
-  const unsigned rt = blockIdx.x * ROWS / TILE_ROWS;
-  const unsigned from = first + rt * tiles;
-  const int g0 = from / (unsigned)share, g1 = (from + tiles - 1) / (unsigned)share;
-  if (g0 == g1) return;                        // written already
-  const int parts = g1 - g0 + 1;
-  // a part that begins where its work-group does is that one's first, others its second.  Within 16 rows the values
-  // lie as the kernel's accumulators do, [D / 16][16 rows][16]
-  const bool second = from > (unsigned)share * g0;
-  auto place = [&](int s) -> size_t {
-    const unsigned slot = 2 * ((unsigned)(g0 + s) * p.num_kv_heads + kh) + (s == 0 && second ? 1 : 0);
-    return (size_t)slot * TILE_ROWS + (row - rt * TILE_ROWS);
-  };
-  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-  float den = 0.0f, M = kNegInf;
-  // U parts on the way at once; past the last one they are read again and weigh nothing
-  auto join = [&](auto count) {
-    constexpr int U = decltype(count)::value;
-    for (int s0 = 0; s0 < parts; s0 += U) {
-      float mv[U], lv[U];
-      f32x4 o[U];
+  f32x4 x[R];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const size_t at = place(min(s0 + u, parts - 1));
-        mv[u] = p.part_ml[2 * at];
-        lv[u] = p.part_ml[2 * at + 1];
-        o[u] = *reinterpret_cast<const f32x4*>(p.part_o + at / 16 * 16 * D + d / 16 * 256 + at % 16 * 16 + d % 16);
+  for (int r = 0; r < R; ++r) x[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (node < len) {                            // else padding: zeros
+    const unsigned tiles = (unsigned)(min(ctx + len, p.width) + p.tile_keys - 1) / p.tile_keys;
+    const unsigned rt = blockIdx.x * 16 / TILE_ROWS;
+    const unsigned from = first + rt * tiles;
+    const int g0 = from / (unsigned)share, g1 = (from + tiles - 1) / (unsigned)share;
+    if (g0 == g1) return;                      // written already
+    const int parts = g1 - g0 + 1;
+    // a part that begins where its work-group does is that one's first, others its second
+    const bool second = from > (unsigned)share * g0;
+    auto place = [&](int s) -> size_t {        // of the 16 rows
+      const unsigned slot = 2 * ((unsigned)(g0 + s) * p.num_kv_heads + kh) + (s == 0 && second ? 1 : 0);
+      return (size_t)slot * TILE_ROWS + (blockIdx.x * 16 - rt * TILE_ROWS);
+    };
+    float den = 0.0f, M = kNegInf;
+    // U parts on the way at once; past the last one they are read again and weigh nothing
+    auto join = [&](auto count) {
+      constexpr int U = decltype(count)::value;
+      for (int s0 = 0; s0 < parts; s0 += U) {
+        float mv[U], lv[U];
+        f32x4 o[U][R];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const size_t at = place(min(s0 + u, parts - 1));
+          const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[at + tid / 4 % 16];
+          mv[u] = ml.x;
+          lv[u] = ml.y;
+#pragma unroll
+          for (int r = 0; r < R; ++r) o[u][r] = reinterpret_cast<const f32x4*>(p.part_o + at * D)[tid + 256 * r];
+        }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmaxf(top, mv[u]);
+        const float f = M == kNegInf ? 1.0f : fast_exp2(M - top);    // (without a maximum: nothing, or NaN)
+        den *= f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[r] *= f;
+        M = top;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (s0 + u >= parts || lv[u] == 0.0f) continue;            // no keys of this row
+          const float w = lv[u] * (mv[u] == kNegInf ? 1.0f : fast_exp2(mv[u] - M));
+          den += w;
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[r] += o[u][r] * w;
+        }
       }
-      float top = M;
+    };
+    if (parts <= 2) join(std::integral_constant<int, 2>());
+    else join(std::integral_constant<int, (D == 256 ? 4 : 8)>());
+    const float inv = den != 0.0f ? 1.0f / den : 0.0f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) top = fmaxf(top, mv[u]);
-      const float f = M == kNegInf ? 1.0f : fast_exp2(M - top);      // (without a maximum: nothing, or NaN)
-      x *= f;
-      den *= f;
-      M = top;
+    for (int r = 0; r < R; ++r) x[r] *= inv;
+  }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (s0 + u >= parts || lv[u] == 0.0f) continue;  // no keys of this row
-        const float w = lv[u] * (mv[u] == kNegInf ? 1.0f : fast_exp2(mv[u] - M));
-        den += w;
-        x += o[u] * w;
-      }
-    }
-  };
-  if (parts <= 2) join(std::integral_constant<int, 2>());
-  else join(std::integral_constant<int, 8>());
-  x *= den != 0.0f ? 1.0f / den : 0.0f;
-  store(x);
+  for (int r = 0; r < R; ++r) store(r, x[r]);
 }
 
 // What a (type, head size, number of rows) runs as.
@@ -620,8 +630,7 @@ template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool N
     else
       hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, false>), grid, dim3(kThreads), 0, s, p);
     if (p.work_groups) {
-      constexpr int per = 256 / (D / 4);
-      hipLaunchKernelGGL((tree_merge_kernel<T, D, kRows>), dim3((rows + per - 1) / per, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((tree_merge_kernel<T, D, kRows>), dim3((rows + 15) / 16, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
     }
   }
   static long long resident() {
