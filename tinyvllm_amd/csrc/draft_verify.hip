@@ -26,6 +26,7 @@ namespace {
 constexpr int kWalkThreads = 512;
 constexpr int kStatThreads = 256;
 constexpr int kStatVecs = 8;             // 16-byte vectors a thread of the stats kernel: 32 KiB of a row
+constexpr int kPartsAtOnce = 8;          // parts of a row that a lane of the walk fetches together
 constexpr int kDrawThreads = 256;
 constexpr int kDrawPer = 8;              // elements a thread of the draw kernels
 constexpr int kDrawChunk = kDrawThreads * kDrawPer;
@@ -217,6 +218,7 @@ __device__ __forceinline__ float temperature_of(const VerifyParams& p, int b) {
 // What the walk leaves for the draw after a sequence's last node.
 struct DrawJob {
   double mass;                           // E: the children's e
+  double u;
   int node;                              // -1: no draw
   float top;                             // m
   int children;
@@ -302,12 +304,25 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
     for (int i = tid; i < len; i += kThreads) {
       const RowStat* parts = stats + (size_t)i * p.stat_parts;
       u64 key = 0;
-      for (int k = 0; k < p.stat_parts; ++k) key = max(key, parts[k].key);
-      const float top = from_order_bits((uint32_t)(key >> 32));
+      float top = kNegInf;
       double S = 0.0;
-      if (sampled && key != 0 && key != ~0ull)
-        for (int k = 0; k < p.stat_parts; ++k)
-          if (parts[k].m > kNegInf) S += (double)parts[k].s * weight(parts[k].m, top, c);
+      for (int k0 = 0; k0 < p.stat_parts; k0 += kPartsAtOnce) {
+        RowStat part[kPartsAtOnce];
+#pragma unroll
+        for (int k = 0; k < kPartsAtOnce; ++k) part[k] = parts[min(k0 + k, p.stat_parts - 1)];
+        const float old = top;
+#pragma unroll
+        for (int k = 0; k < kPartsAtOnce; ++k) {
+          key = max(key, part[k].key);
+          top = fmaxf(top, part[k].m);
+        }
+        if (sampled && top > kNegInf) {
+          S = old > kNegInf ? S * weight(old, top, c) : 0.0;
+#pragma unroll
+          for (int k = 0; k < kPartsAtOnce; ++k)
+            if (k0 + k < p.stat_parts && part[k].m > kNegInf) S += (double)part[k].s * weight(part[k].m, top, c);
+        }
+      }
       keys[i] = key;
       totals[i] = S;
     }
@@ -427,6 +442,7 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
           }
           if (lane == 0) {
             job.mass = mass;
+            job.u = u;
             job.top = M;
             job.children = before;
           }
@@ -514,15 +530,14 @@ template <typename T> __global__ void __launch_bounds__(kDrawThreads) verify_dra
   const int b = blockIdx.x, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const VerifyWorkspace ws = workspace_of(p);
+  // the rest's chunks: every wave sums and searches them for itself
+  const double* sums = ws.sums + (size_t)b * p.draw_chunks;
+  const int per = (p.draw_chunks + 63) / 64;
+  double mine = 0.0;                                      // (without a draw of no meaning, and not used)
+  for (int k = 0; k < per; ++k) mine += lane * per + k < p.draw_chunks ? sums[lane * per + k] : 0.0;
+  const double mass = ws.jobs[b].mass, u = ws.jobs[b].u;
   const DrawRow<T> row(p, ws.jobs[b], b);
   if (row.node < 0) return;
-  const double* sums = ws.sums + (size_t)b * p.draw_chunks;
-  const double mass = ws.jobs[b].mass;
-  const double u = p.uniforms[(size_t)b * p.nodes + row.node];
-  // the rest's chunks: every wave sums and searches them for itself
-  const int per = (p.draw_chunks + 63) / 64;
-  double mine = 0.0;
-  for (int k = 0; k < per; ++k) mine += lane * per + k < p.draw_chunks ? sums[lane * per + k] : 0.0;
   const double upto = wave_prefix(mine, lane);
   const double rest = lane_value(upto, 63);
   const double target = u * (mass + rest) - mass;
