@@ -176,6 +176,24 @@ def test_layout_with_lengths_out_of_range_and_short_tables():
 
 
 @gpu
+def test_contexts_next_to_32_bits():
+    """No table reaches these positions; the lengths are only counted."""
+    from tinyvllm_amd.draft_tree import draft_tree_layout
+    ctx = cuda(np.array([2 ** 31 - 6, 2 ** 31 - 1], np.int32))
+    parents = cuda(np.tile(np.arange(-1, 4, dtype=np.int32), (2, 1)))
+    lens, table = cuda(np.array([5, 1], np.int32)), cuda(np.arange(8, dtype=np.int32).reshape(2, 4))
+    out = draft_tree_layout(parents, lens, ctx, table, 16, 8)
+    assert out.positions.tolist() == [[2 ** 31 - 6 + i for i in range(5)], [2 ** 31 - 1, 0, 0, 0, 0]]
+    assert (out.slots == -1).all()
+    k = torch.randn((8, 16, 2, 8), device="cuda")
+    before = k.clone()
+    path = cuda(np.array([[0, 2, 4, -1, -1], [0, -1, -1, -1, -1]], np.int32))
+    from tinyvllm_amd.kv_cache import keep_draft_rows
+    keep_draft_rows([k], [k], path, cuda(np.array([3, 1], np.int32)), ctx, table)
+    assert torch.equal(k, before)
+
+
+@gpu
 def test_layout_of_no_sequences():
     from tinyvllm_amd.draft_tree import draft_tree_layout
     none = torch.zeros((0,), dtype=torch.int32, device="cuda")

@@ -156,6 +156,27 @@ def test_work_groups(dtype, size):
 
 
 @gpu
+@pytest.mark.parametrize("size", [0, 5, 300, None])
+def test_many_sequences(size):
+    """More sequences than a work-group has threads, long runs of empty ones among them, at the ends too."""
+    rng = rng_of(600)
+    lens, ctx = rng.integers(0, 4, 700), rng.integers(0, 90, 700)
+    lens[:5] = lens[100:480] = lens[-300:] = 0
+    case = Case(rng, "float16", 4, 2, 64, 16, lens, ctx, 3)
+    case.check(case.run(work_groups=size))
+
+
+@gpu
+def test_sequences_that_share_blocks():
+    """A prompt's blocks in several sequences' tables, each with its own after them."""
+    rng = rng_of(601)
+    case = Case(rng, "bfloat16", 8, 2, 128, 16, [9, 9, 5], [100, 71, 96], 9)
+    case.table[1:, :4] = case.table[0, :4]
+    case.check(case.run())
+    case.check(case.run(work_groups=9))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_long_context(dtype):
     rng = rng_of(77)

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kDraftMaxNodes) draft_layout_kernel(const Draf
     const int blk = p.block_tables[(size_t)b * p.bt_stride + pos / p.block_size];
     if ((unsigned)blk < (unsigned)p.num_blocks) slot = blk * p.block_size + (int)(pos % p.block_size);
   }
-  p.positions[at] = live ? ctx + bits - 1 : 0;
+  p.positions[at] = live ? (int)((unsigned)ctx + (bits - 1)) : 0;
   p.slots[at] = slot;
 }
 
