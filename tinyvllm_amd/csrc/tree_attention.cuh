@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
     const int k0 = t * BN;
     f32x4 st[RB][KB];
     // reads first, then products, so that one wait covers many reads
-    constexpr int FG = QF * KB > 16 ? 16 / KB : QF;      // reads of at most 16 fragments at once
+    constexpr int FM = F32 && D == 256 ? 8 : 16, FG = QF * KB > FM ? FM / KB : QF;      // reads of at most FM fragments at once
 #pragma unroll
     for (int f0 = 0; f0 < QF; f0 += FG) {
       u32x4 kf[FG][KB];
@@ -362,7 +362,22 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
         vf[x & 1][db] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     };
-    if constexpr (!F32) values(0);
+    // fp32: element e of vector b of a row is A row col of accumulator 4 b + e, which so holds d = 64 b + 4 col + e
+    constexpr int VS = !F32 ? 1 : D == 256 ? 2 : 4 * KB;      // rows on the way: all, where there are registers for them
+    f32x4 vw[VS][F32 ? D / 64 : 1];
+    auto value_row = [&](int y) {              // key 4 g + y % 4 of block y / 4
+#pragma unroll
+      for (int b = 0; b < D / 64; ++b) {
+        const int r = y / 4 * 16 + 4 * g + y % 4;
+        vw[y % VS][b] = *reinterpret_cast<const f32x4*>(sv + r * ROW + ((b * 16 + col) ^ tree_perm<CPR>(r)) * 16);
+      }
+    };
+    if constexpr (F32) {
+#pragma unroll
+      for (int y = 0; y < VS; ++y) value_row(y);
+    } else {
+      values(0);
+    }
     float base[RB], mt[RB];
     bool need = false;
 #pragma unroll
@@ -419,15 +434,15 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
 #pragma unroll
         for (int r = 0; r < RB; ++r) sums[r][0] += (st[r][kb][0] + st[r][kb][1]) + (st[r][kb][2] + st[r][kb][3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)            // keys 4 g + i of the block
+        for (int i = 0; i < 4; ++i) {
+          const int y = 4 * kb + i;
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const int r = kb * 16 + 4 * g + i;
-            const float v = *reinterpret_cast<const float*>(sv + r * ROW + ((db * 4 + (col >> 2)) ^ tree_perm<CPR>(r)) * 16 + (col & 3) * 4);
+          for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int r = 0; r < RB; ++r)
-              oacc[r][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, st[r][kb][i], oacc[r][db], 0, 0, 0);
-          }
+              oacc[r][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(vw[y % VS][db / 4][db % 4], st[r][kb][i], oacc[r][db], 0, 0, 0);
+          if (y + VS < 4 * KB) value_row(y + VS);
+        }
       }
     } else {
       const u32x4 ones = u32x4{kOnes2<T>, kOnes2<T>, kOnes2<T>, kOnes2<T>};
@@ -450,6 +465,13 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
     }
   };
 
+  // Four consecutive outputs of a lane's row, and their place: the 16-element block and the element in it.
+  auto four = [&](int r, int db) -> f32x4 {
+    if constexpr (F32) return f32x4{oacc[r][db & ~3][db & 3], oacc[r][(db & ~3) + 1][db & 3], oacc[r][(db & ~3) + 2][db & 3], oacc[r][(db & ~3) + 3][db & 3]};
+    else return oacc[r][db];
+  };
+  auto block_of = [&](int db) { return F32 ? (db & ~3) + g : db; };
+  auto element_of = [&](int db) { return F32 ? 4 * (db & 3) : 4 * g; };
   // A unit's rows go out, or, where other work-groups have tiles of it, its part of them.
   auto end_unit = [&](int first, int past, int slot) {
     const bool whole = first == 0 && past == cu.tiles;
@@ -460,14 +482,15 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
       if (!(live || (!p.work_groups && qrow[r] < rows))) continue;
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;     // a row that sees nothing is zero
       if (whole) {
-        const size_t at = (((size_t)cu.b * p.nodes + node[r]) * p.num_kv_heads * G + (size_t)kh * G + qrow[r] - node[r] * G) * D + 4 * g;
+        const size_t at = (((size_t)cu.b * p.nodes + node[r]) * p.num_kv_heads * G + (size_t)kh * G + qrow[r] - node[r] * G) * D;
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const f32x4 x = live ? oacc[r][db] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+          const f32x4 x = live ? four(r, db) * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+          const size_t to = at + block_of(db) * 16 + element_of(db);
           if (F32 || p.out_dtype == kF32)
-            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at + db * 16) = x;
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + to) = x;
           else if constexpr (!F32)
-            *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + at + db * 16) =
+            *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + to) =
                 u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
         }
       } else {
@@ -478,7 +501,7 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          *reinterpret_cast<f32x4*>(p.part_o + (at - col) * D + db * 256 + col * 16 + 4 * g) = oacc[r][db] * inv;
+          *reinterpret_cast<f32x4*>(p.part_o + (at - col) * D + block_of(db) * 256 + col * 16 + element_of(db)) = four(r, db) * inv;
       }
     }
   };
