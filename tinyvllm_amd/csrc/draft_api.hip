@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "../../include/tv_draft.h"
+#include "tv_device_cache.h"
 #include "tv_draft.h"
 #include "tv_error.h"
 
@@ -158,7 +159,7 @@ int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv
     return fail(TV_EUNSUPPORTED, "%s: head_dim %d not supported (64/128/256)", who, head_dim), -1;
   const long long rows = (long long)nodes * (num_heads / num_kv_heads);
   const tv::TreeShapeInfo shape = tree_info(rows, head_dim, dtype);
-  const long long slots = shape.resident();
+  const long long resident = shape.resident();
   const long long units = (rows + shape.tile_rows - 1) / shape.tile_rows * num_kv_heads * num_seqs;
   const long long tiles = ((long long)max_blocks * block_size + shape.tile_keys - 1) / shape.tile_keys;
   // In tiles that a work-group takes one after the other: undealt, its rounds of whole units; dealt, its share and
@@ -168,9 +169,14 @@ int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv
   // 245 / 248, over 512..4096 444 / 432; 32 / 4 heads of 64: 64 x 8 over 200..1000 17 / 22, 1 x 32 over 1000 23 / 15,
   // 1 x 64 over 8000 134 / 23; in fp32 4 x 8 over 17..250 17 / 11.
   const long long cost = dtype == TV_F32 ? 6 : head_dim == 64 ? 12 : 8;
-  const long long undealt = (units + slots - 1) / slots * tiles, dealt = units * tiles / slots + cost;
+  const long long undealt = (units + resident - 1) / resident * tiles, dealt = units * tiles / resident + cost;
   const bool counted = ((long long)max_blocks * block_size / 16 + 1) * ((rows + 63) / 64) * num_seqs <= 0x7fffffff;
-  return counted && (dealt < undealt || tiles >= 6 * cost) ? (int)slots : 0;
+  if (!counted || !(dealt < undealt || tiles >= 6 * cost)) return 0;
+  // Two on a CU load as fast as more do and leave fewer parts; only several tiles of rows in 16 bits, which wait for their own
+  // arithmetic, take as many as are resident.  MI355X, us, two a CU / all, 32 / 4 heads of 64 over 1000..4000 tokens in fp16:
+  // 64 x 8 nodes 38 / 44, 32 x 16 34 / 36, 32 x 32 47 / 48, 32 x 61 over 1000..6000 98 / 93; in fp32 over 500..2000 tokens 16 x 16 38 / 42.
+  const long long two = 2LL * std::max(tv::device_cus(), 1);
+  return (int)(rows > 128 && dtype != TV_F32 ? resident : std::min(resident, two));
 }
 
 int tv_paged_tree(void* out, const void* queries, const void* k_cache, const void* v_cache,

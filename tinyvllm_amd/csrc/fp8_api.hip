@@ -78,17 +78,6 @@ int write_common(const char* who, void* k_cache, void* v_cache, float* k_scale, 
 constexpr int kOrderMinSeqs = 32;
 constexpr int kOrderMaxSeqs = 1024;
 
-// Compute units of the current device, asked for once per device.
-int device_cus() {
-  static std::atomic<int> known[tv::kMaxDevices];
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
-  if (dev < tv::kMaxDevices && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
-  if (dev < tv::kMaxDevices) known[dev].store(cus, std::memory_order_relaxed);
-  return cus;
-}
-
 long long decode_rows(int num_seqs, int num_heads, int num_kv_heads) {
   const int group = num_heads / num_kv_heads;
   return (long long)num_seqs * num_kv_heads * ((group + 15) / 16);
@@ -173,7 +162,7 @@ int tv_paged_decode_fp8_partition_size(int num_seqs, int num_heads, int num_kv_h
     return fail(TV_EINVAL, "%s: bad arguments", who), 0;
   if (!valid_head_dim(head_dim))
     return fail(TV_EUNSUPPORTED, "%s: head_dim %d not supported (64/128/256)", who, head_dim), 0;
-  const int cus = device_cus();
+  const int cus = tv::device_cus();
   if (cus < 1) return fail(TV_EHIP, "%s: no device", who), 0;
   const long long width = (long long)max_blocks * block_size;
   const int whole = (int)((width + 31) / 32 * 32);
@@ -230,7 +219,7 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
   // 1152 144 / 148, 128 to 1152 39.3 / 39.9; 32 / 4 heads of 64, 256 to 4096 67 / 76,
   // and with 256 work-groups (64 to 1152) 15.4 / 10.0.
   const bool ordered = max_parts == 1 && need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4) &&
-                       decode_rows(num_seqs, num_heads, num_kv_heads) > 2LL * device_cus() &&
+                       decode_rows(num_seqs, num_heads, num_kv_heads) > 2LL * tv::device_cus() &&
                        decode_rows(num_seqs, num_heads, num_kv_heads) < 1LL << 24;   // 256 threads each in one dimension
   const int group = num_heads / num_kv_heads;
   const int chunks = (group + 15) / 16;
@@ -275,7 +264,7 @@ int tv_paged_decode_fp8(void* out, const void* queries, const void* k_cache, con
   // 6.9; with heads of 128 the larger merge takes it back: 1 x 500 7.7 / 7.5, 32 x
   // 500 8.3 / 7.9.
   const bool wide = !ordered && max_parts == 1 && head_dim == 64 && width <= tv::kFp8WideTokens &&
-                    decode_rows(num_seqs, num_heads, num_kv_heads) <= device_cus();
+                    decode_rows(num_seqs, num_heads, num_kv_heads) <= tv::device_cus();
   tv::launch_paged_decode_fp8(p, head_dim, dtype, wide, s);
   return check_launch(who);
 }
@@ -285,7 +274,7 @@ size_t tv_flash_prefill_paged_fp8_workspace_bytes(int q_len, int start_pos, int 
   if (q_len <= 0 || start_pos < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       !valid_head_dim(head_dim))
     return 0;
-  const int splits = tv::prefill_fp8_splits(q_len, start_pos, num_heads, num_kv_heads, head_dim, device_cus());
+  const int splits = tv::prefill_fp8_splits(q_len, start_pos, num_heads, num_kv_heads, head_dim, tv::device_cus());
   return splits > 1 ? (size_t)splits * q_len * num_heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
@@ -337,11 +326,11 @@ int tv_flash_prefill_paged_fp8(void* out, const void* q, const void* k_cache, co
   p.out_dtype = out_dtype;
   p.splits = 1;
   if (workspace && need) {
-    p.splits = tv::prefill_fp8_splits(q_len, start_pos, num_heads, num_kv_heads, head_dim, device_cus());
+    p.splits = tv::prefill_fp8_splits(q_len, start_pos, num_heads, num_kv_heads, head_dim, tv::device_cus());
     p.part_o = reinterpret_cast<float*>(workspace);
     p.part_ml = p.part_o + (size_t)p.splits * q_len * num_heads * head_dim;
   }
-  tv::launch_prefill_fp8(p, head_dim, dtype, device_cus(), reinterpret_cast<hipStream_t>(stream));
+  tv::launch_prefill_fp8(p, head_dim, dtype, tv::device_cus(), reinterpret_cast<hipStream_t>(stream));
   return check_launch(who);
 }
 

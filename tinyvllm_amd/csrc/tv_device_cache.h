@@ -31,4 +31,15 @@ long long resident_work_groups(std::atomic<long long> (&slots)[kMaxDevices], K k
   return v;
 }
 
+// Compute units of the current device, asked for once per device.
+inline int device_cus() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
+  if (dev < kMaxDevices && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+  if (dev < kMaxDevices) known[dev].store(cus, std::memory_order_relaxed);
+  return cus;
+}
+
 }  // namespace tv
