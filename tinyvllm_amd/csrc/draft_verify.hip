@@ -14,7 +14,9 @@
 // probability 2^17 d.
 //
 // A walk over a path is serial and reads its rows only; reading the rows of all
-// nodes first is parallel (all_rows).
+// nodes first is parallel (all_rows): bound by HBM, then by the latency of the walk and the draw, a work-group a sequence.
+// MI355X: greedy, 64 sequences of 16 nodes, 32000 fp32 logits: rows 23 us (131 MB, 5.7 TB/s), walk 4; sampled, 2 of 32, 128256 in
+// bf16: rows 7.3, walk 6.3, rest 4.6, draw 8.6.
 #include "tv_draft.h"
 
 #include <algorithm>

@@ -14,6 +14,17 @@
 // In a tile past the context rows differ in what they see, and a weight of zero would
 // not hide a NaN or infinity in V: there such a value is zero in LDS and its key's score
 // NaN, which the mask replaces for the rows that do not see the key.
+//
+// Tiles come by LDS DMA, one that is read and one on the way: loads into registers made a wave wait for all of them
+// wherever it reused one.  Work is dealt by the lengths on the device (work_groups): what a launch of whole units takes
+// is its longest unit's time.  MI355X, kernel and merge, us; GB/s and TFLOP/s of the keys and products that cannot be left out:
+//   64 sequences x 16 nodes over 512..4096 tokens, 32 / 8 heads of 128, fp16       117 +  9   4.7 TB/s   bound by HBM
+//   2 x 32 over 31000..32700, 32 / 8 of 128, bf16                                   55 +  9   4.2 TB/s   HBM
+//   32 x 61 over 1000..6000, 32 / 4 of 64, bf16                                     86 + 10   450 TFLOP/s
+//   16 x 32 over 2000, 32 / 8 of 128, fp32                                         166        103 TFLOP/s   matrix units
+// (a large copy reaches 5.2 TB/s, a large product 1140 TFLOP/s, 153 in fp32).  In the third the matrix units are busy for
+// 27% of the time and the vector units for 55%: a head of 64 has 128 products a weight, and its exponential, scaling,
+// maximum and conversion cost more cycles than those.  Without loads it takes 74 us, without the softmax 70.
 #pragma once
 
 #include "tv_device_cache.h"
@@ -630,7 +641,11 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
   for (int r = 0; r < R; ++r) store(r, x[r]);
 }
 
-// What a (type, head size, number of rows) runs as.
+// What a (type, head size, number of rows) runs as.  A wave of 32 rows reads a key or value from LDS once for both its row
+// blocks, but is half empty at 64 rows, and holds twice the registers; keys that one row tile reads bypass the
+// caches, those that several read do not.  MI355X, us, 16 rows a wave / 16 cached / 32 / 32 cached, fp16, 32 / 8 heads of 128 over
+// 500..2000 tokens: 64 x 16 nodes (64 rows) 70 / 80 / 82 / 90, 32 x 32 (128) 67 / 62 / 55 / 59, 16 x 48 (192) 60 / 57 / 52 / 48,
+// 16 x 64 (256) 74 / 67 / 56 / 53.
 template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool NT_> struct TreeShape {
   static constexpr int RB = RB_, RG = RG_, BN = BN_, NS = NS_, EU = EU_;
   static constexpr bool NT = NT_;
