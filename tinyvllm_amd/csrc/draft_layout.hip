@@ -58,8 +58,8 @@ __global__ void __launch_bounds__(kDraftMaxNodes) draft_layout_kernel(const Draf
 // A work-group moves 256 vectors of every row that has to, of one sequence and layer, K and V.  The rows' places are
 // looked up first, one by a thread, and listed in their order.  A thread then owns a vector of every row; it reads kAhead rows
 // before it writes them: row path[j] > j is read before any row past j is written, since every write up to then went to
-// rows below j.  Bound by HBM and by the pages that
-// the rows are spread over.  MI355X: 64 sequences of 48 nodes, 32 layers, rows of 2 KiB in K and V each (72 MB) 24 us, 2.9 TB/s.
+// rows below j.  Bound by HBM after the look-ups,
+// a chain of three loads.  MI355X: 64 sequences of 48 nodes, 32 layers, rows of 2 KiB in K and V each (72 MB) 24 us, 2.9 TB/s.
 template <typename V>
 __global__ void __launch_bounds__(256) keep_rows_kernel(const KeepParams p) {
   constexpr int kAhead = 8;

@@ -23,8 +23,9 @@
 //   32 x 61 over 1000..6000, 32 / 4 of 64, bf16                                     86 + 10   450 TFLOP/s
 //   16 x 32 over 2000, 32 / 8 of 128, fp32                                         166        103 TFLOP/s   matrix units
 // (a large copy reaches 5.2 TB/s, a large product 1140 TFLOP/s, 153 in fp32).  In the third the matrix units are busy for
-// 27% of the time and the vector units for 55%: a head of 64 has 128 products a weight, and its exponential, scaling,
-// maximum and conversion cost more cycles than those.  Without loads it takes 74 us, without the softmax 70.
+// 27% of the cycles and the vector units for 42%: a head of 64 has 128 products a weight, and its exponential, scaling,
+// maximum and conversion cost more cycles than those; its four row tiles read 382 MB past the L2 caches, since
+// they are at different keys at a time.  Without loads it takes 74 us, without the softmax 70, with loads alone 65.
 #pragma once
 
 #include "tv_device_cache.h"
