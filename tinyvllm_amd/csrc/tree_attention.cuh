@@ -231,14 +231,17 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
   // The next tile to request: tile lt of unit lu, with `to_load` to come; its block ids are looked up a tile ahead.
   TreeUnit lu = cu;
   int lt = tile, to_load = left;
-  struct Ids { int id[NV]; } ids;
+  // UB: load i's in lane i, by a vector load: it arrives with the tile before, where a scalar load would have every read
+  // from LDS wait for it.  Else each lane's own.
+  struct Ids { int id[UB ? 1 : NV]; } ids;
   auto look_up = [&]() {
     if (to_load <= 0) return;
     const int* table = p.block_tables + (size_t)lu.b * p.bt_stride;
+    if constexpr (UB) {
+      ids.id[0] = table[min(lt * BN + wr + RPP * (lane % NV), lu.keys - 1) >> p.bs_log2];
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int key = min(lt * BN + wr + RPP * i + (UB ? 0 : lr), lu.keys - 1);
-      ids.id[i] = UB ? uniform_load(table + (key >> p.bs_log2)) : table[key / bs];
+      for (int i = 0; i < NV; ++i) ids.id[i] = table[min(lt * BN + wr + RPP * i + lr, lu.keys - 1) / bs];
     }
   };
   // Requests it into a stage and moves on; returns bit i for a load whose block is outside the cache.  Where no tile is
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
     for (int i = 0; i < NV; ++i) {
       const uint32_t at = sgpr(smem_at + stage * STAGE + (wr + RPP * i) * ROW);
       if constexpr (UB) {
-        const uint32_t id = sgpr(ids.id[i]);
+        const uint32_t id = __builtin_amdgcn_readlane(ids.id[0], i);
         const bool ok = id < (uint32_t)p.num_blocks;
         const u64 off = (u64)(ok ? id : 0) * block_bytes + (uint32_t)((lt * BN + wr + RPP * i) & (bs - 1)) * (uint32_t)row_bytes;
         const u64 ka = kc + off, va = vc + off;
