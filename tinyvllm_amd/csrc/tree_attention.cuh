@@ -648,8 +648,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
 // What a (type, head size, number of rows) runs as.  A wave of 32 rows reads a key or value from LDS once for both its row
 // blocks, but is half empty at 64 rows, and holds twice the registers; keys that one row tile reads bypass the
 // caches, those that several read do not.  MI355X, us, 16 rows a wave / 16 cached / 32 / 32 cached, fp16, 32 / 8 heads of 128 over
-// 500..2000 tokens: 64 x 16 nodes (64 rows) 70 / 80 / 82 / 90, 32 x 32 (128) 67 / 62 / 55 / 59, 16 x 48 (192) 60 / 57 / 52 / 48,
-// 16 x 64 (256) 74 / 67 / 56 / 53.
+// 500..2000 tokens: 64 x 16 nodes (64 rows) 74 / 81 / 89 / 95, 32 x 32 (128) 67 / 62 / 56 / 60, 16 x 48 (192) 59 / 55 / 53 / 47,
+// 16 x 64 (256) 75 / 65 / 57 / 52.
 template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool NT_> struct TreeShape {
   static constexpr int RB = RB_, RG = RG_, BN = BN_, NS = NS_, EU = EU_;
   static constexpr bool NT = NT_;
