@@ -77,15 +77,15 @@ __device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds_base) 
 // A row tile of a sequence: its lengths, and the tiles of its keys.
 struct TreeUnit { int b, rt, ctx, len, keys, tiles; };
 
-// RG groups of four waves, 16 RB rows a wave.  BN keys a tile, NS tiles in LDS: one that is read and NS - 1 on the way.
+// Four waves, 16 RB rows a wave.  BN keys a tile, two tiles in LDS: one that is read and one on the way.
 // UB: the block size is 16 or a larger power of two: the rows of a load lie in one
 // block, whose id and address are then scalar, and whose range ends at the last key.
-template <typename T, int D, int RB, int RG, int BN, int NS, int EU, bool NT, bool UB>
-__global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(const TreeParams p) {
+template <typename T, int D, int RB, int BN, int EU, bool NT, bool UB>
+__global__ void __launch_bounds__(kTreeThreads, EU) tree_attention_kernel(const TreeParams p) {
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int THREADS = kTreeThreads * RG;
-  constexpr int WAVES = 4 * RG;
-  constexpr int BM = 64 * RB * RG;
+  constexpr int THREADS = kTreeThreads;
+  constexpr int WAVES = THREADS / 64;
+  constexpr int BM = 64 * RB;
   constexpr int KB = BN / 16;
   constexpr int DB = D / 16;
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
   constexpr int NV = BN * CPR / THREADS;       // loads of a wave for a tile, each of K and V
   constexpr int RPI = 64 / CPR;                // rows of a load
   constexpr int RPP = WAVES * RPI;             // rows of all waves' loads
-  static_assert(NV * THREADS == BN * CPR && NV >= 1 && NV * NS <= 64, "tile shape");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE];
+  static_assert(NV * THREADS == BN * CPR && NV >= 1 && NV <= 32, "tile shape");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
   __shared__ int wave_tiles[WAVES];
   __shared__ int start_seq, start_tile;        // the work-group's first tile
 
@@ -482,7 +482,8 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
 
   // Four consecutive outputs of a lane's row, and their place: the 16-element block and the element in it.
   auto four = [&](int r, int db) -> f32x4 {
-    if constexpr (F32) return f32x4{oacc[r][db & ~3][db & 3], oacc[r][(db & ~3) + 1][db & 3], oacc[r][(db & ~3) + 2][db & 3], oacc[r][(db & ~3) + 3][db & 3]};
+    const int b = db & ~3, i = db & 3;
+    if constexpr (F32) return f32x4{oacc[r][b][i], oacc[r][b + 1][i], oacc[r][b + 2][i], oacc[r][b + 3][i]};
     else return oacc[r][db];
   };
   auto block_of = [&](int db) { return F32 ? (db & ~3) + g : db; };
@@ -527,26 +528,21 @@ __global__ void __launch_bounds__(kTreeThreads * RG, EU) tree_attention_kernel(c
     return;
   }
   look_up();
-  u64 bad = 0;                                 // NV bits a tile, the next one's lowest
-#pragma unroll
-  for (int k = 0; k < NS - 1; ++k) {
-    bad |= (u64)issue(k) << (NV * k);
-    look_up();
-  }
+  uint32_t lost = issue(0);
+  look_up();
   int first = tile, slot = 2 * wg;
   int stage = 0;
   while (true) {
-    wait_vmcnt<2 * NV * (NS - 2)>();
-    const uint32_t lost = (uint32_t)bad & ((1u << NV) - 1);
+    wait_vmcnt<0>();
     if (__builtin_amdgcn_ballot_w64((tile + 1) * BN > cu.ctx || lost != 0) != 0) {
       __asm__ volatile("" ::: "memory");
       amend(tile, lost, stage);
     }
     lds_barrier();                             // the tile is there; the one before has been read
-    bad = bad >> NV | (u64)issue(stage == 0 ? NS - 1 : stage - 1) << (NV * (NS - 2));
+    lost = issue(stage ^ 1);
     look_up();
     compute(stage, tile);
-    stage = stage + 1 == NS ? 0 : stage + 1;
+    stage ^= 1;
     ++tile;
     --left;
     if (tile == cu.tiles || left == 0) {
@@ -650,10 +646,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams p) {
 // caches, those that several read do not.  MI355X, us, 16 rows a wave / 16 cached / 32 / 32 cached, fp16, 32 / 8 heads of 128 over
 // 500..2000 tokens: 64 x 16 nodes (64 rows) 74 / 81 / 89 / 95, 32 x 32 (128) 67 / 62 / 56 / 60, 16 x 48 (192) 59 / 55 / 53 / 47,
 // 16 x 64 (256) 75 / 65 / 57 / 52.
-template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool NT_> struct TreeShape {
-  static constexpr int RB = RB_, RG = RG_, BN = BN_, NS = NS_, EU = EU_;
-  static constexpr bool NT = NT_;
-  static constexpr int kRows = 64 * RB * RG, kThreads = kTreeThreads * RG;
+template <typename T, int D, int RB, int BN, int EU, bool NT> struct TreeShape {
+  static constexpr int kRows = 64 * RB, kKeys = BN;
 
   static void launch(TreeParams p, hipStream_t s) {
     const int rows = p.nodes * p.group;
@@ -668,16 +662,15 @@ template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool N
     }
     const dim3 grid(p.work_groups ? p.work_groups : (unsigned)((long long)p.row_tiles * p.num_kv_heads * p.num_seqs));
     if (p.bs_log2 >= 4)
-      hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, true>), grid, dim3(kThreads), 0, s, p);
+      hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, BN, EU, NT, true>), grid, dim3(kTreeThreads), 0, s, p);
     else
-      hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, false>), grid, dim3(kThreads), 0, s, p);
-    if (p.work_groups) {
+      hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, BN, EU, NT, false>), grid, dim3(kTreeThreads), 0, s, p);
+    if (p.work_groups)
       hipLaunchKernelGGL((tree_merge_kernel<T, D, kRows>), dim3((rows + 15) / 16, p.num_kv_heads, p.num_seqs), dim3(256), 0, s, p);
-    }
   }
   static long long resident() {
     static std::atomic<long long> slots[kMaxDevices];
-    return resident_work_groups(slots, tree_attention_kernel<T, D, RB, RG, BN, NS, EU, NT, true>, kThreads);
+    return resident_work_groups(slots, tree_attention_kernel<T, D, RB, BN, EU, NT, true>, kTreeThreads);
   }
 };
 
@@ -685,13 +678,13 @@ template <typename T, int D, int RB_, int RG_, int BN_, int NS_, int EU_, bool N
 template <typename T, int D, typename F> auto tree_shape(long long rows, F f) {
   if constexpr (sizeof(T) == 4) {
     constexpr int BN = D == 256 ? 16 : 32;
-    return rows <= 64 ? f(TreeShape<T, D, 1, 1, BN, 2, 2, true>()) : f(TreeShape<T, D, 1, 1, BN, 2, 2, false>());
+    return rows <= 64 ? f(TreeShape<T, D, 1, BN, 2, true>()) : f(TreeShape<T, D, 1, BN, 2, false>());
   } else if constexpr (D == 256) {
-    return rows <= 64 ? f(TreeShape<T, D, 1, 1, 32, 2, 2, true>()) : f(TreeShape<T, D, 1, 1, 32, 2, 2, false>());
+    return rows <= 64 ? f(TreeShape<T, D, 1, 32, 2, true>()) : f(TreeShape<T, D, 1, 32, 2, false>());
   } else {
     constexpr int BN = D == 64 ? 64 : 32, EU = D == 64 ? 3 : 2;
-    if (rows <= 64) return f(TreeShape<T, D, 1, 1, 64, 2, (D == 64 ? 4 : 2), true>());
-    return rows <= 128 ? f(TreeShape<T, D, 2, 1, BN, 2, EU, true>()) : f(TreeShape<T, D, 2, 1, BN, 2, EU, false>());
+    if (rows <= 64) return f(TreeShape<T, D, 1, 64, (D == 64 ? 4 : 2), true>());
+    return rows <= 128 ? f(TreeShape<T, D, 2, BN, EU, true>()) : f(TreeShape<T, D, 2, BN, EU, false>());
   }
 }
 template <typename T, typename F> auto tree_shape(long long rows, int head_dim, F f) {
@@ -707,7 +700,7 @@ template <typename T> void tree_launch(const TreeParams& p, int head_dim, hipStr
 }
 template <typename T> TreeShapeInfo tree_info(long long rows, int head_dim) {
   return tree_shape<T>(rows, head_dim, [](auto shape) {
-    return TreeShapeInfo{decltype(shape)::kRows, decltype(shape)::BN, [] { return decltype(shape)::resident(); }};
+    return TreeShapeInfo{decltype(shape)::kRows, decltype(shape)::kKeys, [] { return decltype(shape)::resident(); }};
   });
 }
 
