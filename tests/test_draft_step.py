@@ -162,6 +162,29 @@ def test_sampled_steps_accept_what_is_likely():
 
 
 @gpu
+def test_rows_of_a_cache_of_more_than_4_gib():
+    """Writes and moves beyond 2^32 bytes and 2^31 elements are those in a small cache."""
+    from tinyvllm_amd.kv_cache import keep_draft_rows, rope_and_cache
+    from tests.test_rope_cache import table_of
+    rng = rng_of(8)
+    n, hq, hkv, d, bs, nb = 20, 4, 2, 128, 16, 6
+    first = (1 << 31) // (bs * hkv * d)
+    small = [torch.from_numpy(rng.standard_normal((nb, bs, hkv, d))).to("cuda", torch.bfloat16) for _ in range(2)]
+    large = [torch.empty((first + nb, bs, hkv, d), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for x, y in zip(large, small):
+        x[first:] = y
+    q, k, v = (torch.from_numpy(rng.standard_normal((n, h, d))).to("cuda", torch.bfloat16) for h in (hq, hkv, hkv))
+    slots, positions = rng.permutation(nb * bs)[:n].astype(np.int32), np.arange(n, dtype=np.int32)
+    path, counts = np.array([[0, 3, 4, 11] + [-1] * 8], np.int32), np.array([4], np.int32)
+    ctx, table = np.array([21], np.int32), rng.permutation(nb).astype(np.int32)[None]
+    for caches, base in ((small, 0), (large, first)):
+        rope_and_cache(*caches, q, k, v, cuda(slots + np.int32(base * bs)), cuda(positions), cuda(table_of(64, d)))
+        keep_draft_rows(caches[:1], caches[1:], cuda(path), cuda(counts), cuda(ctx), cuda(table + np.int32(base)))
+    for x, y in zip(large, small):
+        assert torch.equal(x[first:], y)
+
+
+@gpu
 def test_a_step_in_one_graph():
     """Layout, write, attention, verdict and kept rows captured together: replays follow their inputs and agree with eager calls."""
     from tinyvllm_amd.attention import PagedTreePlan

@@ -381,9 +381,15 @@ def test_two_streams_at_once():
 def test_cache_of_more_than_4_gib(dtype):
     """Blocks beyond 2^32 bytes and 2^31 elements."""
     rng = rng_of(89)
-    case = Case(rng, dtype, 8, 2, 128, 16, [9, 9], [100, 45], 9, spare=(1 << 31) // (16 * 2 * 128) + 40)
-    assert case.k.numel() > 1 << 31
+    case = Case(rng, dtype, 8, 2, 128, 16, [9, 9], [100, 45], 9)
+    first = (1 << 31) // (16 * 2 * 128)
+    for name in ("k", "v"):
+        large = torch.empty((first + case.pool, 16, 2, 128), dtype=case.k.dtype, device="cuda")
+        large[first:] = getattr(case, name)
+        setattr(case, name, large)
+    case.table, case.pool = case.table + np.int32(first), first + case.pool
     case.check(case.run())
+    case.check(case.run(work_groups=0))
 
 
 @gpu
