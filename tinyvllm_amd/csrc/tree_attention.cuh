@@ -192,6 +192,11 @@ __global__ void __launch_bounds__(kTreeThreads, EU) tree_attention_kernel(const 
     while (uniform(u.b + 1 < p.num_seqs && u.len == 0));
   };
 
+  // The wave's place among the tile's rows.  Few rows leave waves without any, which only load; work-groups 256 apart mostly
+  // share a CU (8 XCDs of 32), and their rows go to different SIMDs.  MI355X, us, all waves in their places at work / so, over
+  // 500..2000 tokens: 16 rows 61 / 55 (64 x 2 nodes, 32 / 4 heads of 64, fp32), 32 rows 68 / 65 (64 x 8, 32 / 8 of 128, fp16), 48 rows
+  // 70 / 66 and 64 rows 69 / 71 (16 x 12 and 16 x 16, 32 / 8 of 128, fp32).
+  const int part = (wave + (rows <= 16 ? 1 : 2) * (blockIdx.x >> 8)) & 3;
   int qrow[RB], node[RB];
   constexpr int QF = F32 ? D / 16 : D / 32;
   u32x4 qf[RB][QF];
@@ -201,7 +206,7 @@ __global__ void __launch_bounds__(kTreeThreads, EU) tree_attention_kernel(const 
   auto begin_unit = [&]() {
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      qrow[r] = cu.rt * BM + (wave * RB + r) * 16 + col;
+      qrow[r] = cu.rt * BM + (part * RB + r) * 16 + col;
       node[r] = qrow[r] / G;
       const T* qg = reinterpret_cast<const T*>(p.q) + (size_t)cu.b * p.q_seq_stride + (size_t)node[r] * p.q_node_stride +
                     (size_t)(kh * G + qrow[r] - node[r] * G) * D;
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kTreeThreads, EU) tree_attention_kernel(const 
                 u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
         }
       } else {
-        const size_t at = (size_t)slot * BM + (wave * RB + r) * 16 + col;
+        const size_t at = (size_t)slot * BM + (part * RB + r) * 16 + col;
         if (g == 0) {
           p.part_ml[2 * at] = m[r];
           p.part_ml[2 * at + 1] = l;           // zero: no keys of this row
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(kTreeThreads, EU) tree_attention_kernel(const 
     lds_barrier();                             // the tile is there; the one before has been read
     lost = issue(stage ^ 1);
     look_up();
-    compute(stage, tile);
+    if (cu.rt * BM + part * RB * 16 < cu.len * G) compute(stage, tile);
     stage ^= 1;
     ++tile;
     --left;
