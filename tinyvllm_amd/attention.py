@@ -396,7 +396,8 @@ class PagedTreePlan:
     spoils the nodes that see it and no others; a score of -inf has weight 0.  head_dim 64, 128 or 256, T at most 256, any block size.
     ``max_context_len`` (context and tree) trims the table.  ``work_groups``: 0 gives every (sequence, KV head, tile of
     rows) a work-group; n > 0 deals all their keys evenly to n work-groups and joins what that cuts, and results then depend
-    on the batch in their last digits.  The tensors are read on every ``run()`` and must keep their storage.
+    on the batch in their last digits.  The tensors are read on every ``run()`` and must keep their storage; the
+    runs of a plan, which share its output and workspace, follow each other in stream order.
     """
 
     def __init__(self, queries, k_cache, v_cache, block_tables, context_lens, tree_lens, tree_mask,
