@@ -147,6 +147,56 @@ def test_many_logits_are_read_by_path(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_many_sequences_are_read_by_path(dtype):
+    """So many short rows that the walk reads its own, greedy ones too; bf16 logits tie often."""
+    rng = rng_of(14)
+    b, t, v = 9000, 9, 100
+    logits, tokens, parents, lens = make(rng, b, t, v, dtype)
+    check(logits, tokens, parents, lens)
+    temps = np.where(np.arange(b) % 2 == 0, 0.0, 0.7).astype(np.float32)
+    check(logits, tokens, parents, lens, temps, rng.random((b, t)).astype(np.float32))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("v", [60, 9000])
+def test_long_greedy_paths_past_likely_siblings(dtype, v):
+    """Paths of up to 128 nodes, whose every node has siblings of the same logit (a higher token, or the same one later), of a
+    higher logit than other children's but no maximum, outside the vocabulary, or with NaN."""
+    rng = rng_of(v + 15)
+    b, t = 5, 256
+    x = rng.standard_normal((b, t, v)) * 0.5
+    tokens, parents = rng.integers(0, v, (b, t)).astype(np.int32), np.zeros((b, t), np.int32)
+    parents[:, 0] = -1
+    for i in range(b):
+        end = 0                                             # of the path
+        for j in range(1, t):
+            parents[i, j] = end
+            kind = rng.integers(0, 5)
+            if j % 2 == 0 or kind == 0:                     # the path goes on (to this node, or to an earlier one of its kind)
+                best = int(rng.integers(0, v - 1))
+                x[i, end, best] = 4.0
+                tokens[i, j] = best
+                end = j
+                continue
+            parents[i, j] = rng.integers(0, j) if kind == 1 else end
+            up, best = parents[i, j], int(x[i, parents[i, j]].argmax())
+            if kind == 2:
+                tokens[i, j] = v + 3
+            elif kind == 3:
+                x[i, up, min(best + 1, v - 1)] = x[i, up, best]
+                tokens[i, j] = min(best + 1, v - 1)
+            elif kind == 4:
+                tokens[i, j] = best
+    x[2, 60:, 5] = np.nan
+    x[3, 100:, 7] = np.inf
+    logits = torch.from_numpy(x).to("cuda", DTYPES[dtype])
+    out = check(logits, tokens, parents, np.array([t, t - 1, t, t, 40], np.int32))
+    assert int(out.counts.max()) > 16                       # more than any group of work-groups takes at a time
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("rows", [0, 60])
 def test_ties_go_to_the_lowest_index(dtype, rows):
     """Equal maxima at every distance, -0 beside +0, siblings of one token."""

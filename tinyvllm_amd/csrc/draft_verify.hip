@@ -13,9 +13,9 @@
 // vocabulary has a bound every 2^-17 of S, and an error of d in u S meets one with
 // probability 2^17 d.
 //
-// A walk over a path is serial and reads its rows only; reading the rows of all
-// nodes first is parallel (all_rows): bound by HBM, then by the latency of the walk and the draw, a work-group a sequence.
-// MI355X: greedy, 64 sequences of 16 nodes, 32000 fp32 logits: rows 23 us (131 MB, 5.7 TB/s), walk 4; sampled, 2 of 32, 128256 in
+// A walk over a path is serial and reads its rows only; reading the rows that it may come to
+// first is parallel (all_rows): bound by HBM, then by the latency of the walk and the draw, a work-group a sequence.
+// MI355X: greedy, 64 sequences of 16 nodes, 32000 fp32 logits: chains' rows 13 us, walk 4; sampled, 2 of 32, 128256 in
 // bf16: rows 7.3, walk 6.3, rest 4.6, draw 8.6.
 #include "tv_draft.h"
 
@@ -29,6 +29,7 @@ constexpr int kWalkThreads = 512;
 constexpr int kStatThreads = 256;
 constexpr int kStatVecs = 8;             // 16-byte vectors a thread of the stats kernel: 32 KiB of a row
 constexpr int kPartsAtOnce = 8;          // parts of a row that a lane of the walk fetches together
+constexpr int kChainRows = 8;            // work-groups a part for a chain's rows
 constexpr int kDrawThreads = 256;
 constexpr int kDrawPer = 8;              // elements a thread of the draw kernels
 constexpr int kDrawChunk = kDrawThreads * kDrawPer;
@@ -241,32 +242,64 @@ __host__ __device__ inline VerifyWorkspace workspace_of(const VerifyParams& p) {
   return w;
 }
 
-// Parts of the rows of all live nodes.
+// Parts of the rows of all live nodes; where all sequences are greedy, of those that a path can come to: of a node's
+// children only that with the largest logit (the lowest token of equal ones, the first of equal tokens) can be the row's first
+// maximum, so there is one path, a chain from node 0 on, known without its rows.  Every work-group finds it for itself;
+// p.chain_rows of them share its rows.
 template <typename T> __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyParams p) {
+  static_assert(kStatThreads == kDraftMaxNodes, "a thread for every node");
   __shared__ RowStat red[kStatThreads / 64];
-  const int row = blockIdx.x, part = blockIdx.y;
-  const int b = row / p.nodes;
-  if (row - b * p.nodes >= p.tree_lens[b]) return;
-  const int tid = threadIdx.x;
+  __shared__ u64 best[kDraftMaxNodes];                       // of a node's children: logit, token, node, by order
+  const int part = blockIdx.y, tid = threadIdx.x;
+  const bool chain = p.chain_rows != 0;
+  const int each = chain ? p.chain_rows : p.nodes;
+  // sequences innermost: the rows of a chain's end, often none, are spread over the XCDs
+  const int j = blockIdx.x / p.num_seqs, b = blockIdx.x - j * p.num_seqs;
+  const int len = min(p.tree_lens[b], p.nodes);
+  const T* row0 = reinterpret_cast<const T*>(p.logits) + (size_t)b * p.nodes * p.row_stride;
+  if (chain) {
+    best[tid] = 0;
+    __syncthreads();
+    if (tid < len) {
+      const int tok = p.tokens[(size_t)b * p.nodes + tid], up = p.parents[(size_t)b * p.nodes + tid];
+      if (up >= 0 && up < tid && (unsigned)tok < (unsigned)p.vocab) {
+        const float x = to_float<T>(row0[(size_t)up * p.row_stride + tok]);
+        atomicMax(&best[up], (u64)order_bits(x) << 32 | (u64)(0xffffffu - tok) << 8 | (u64)(255 - tid));
+      }
+    }
+    __syncthreads();
+  }
+  auto further = [&](int node, int steps) {                  // along the chain (children have higher indexes)
+    for (; steps > 0 && node < len; --steps) {
+      const u64 child = best[node];
+      node = __builtin_amdgcn_readfirstlane(child ? 255 - (int)(child & 255u) : len);
+    }
+    return node;
+  };
   const float temp = temperature_of(p, b);
   const bool sampled = temp > 0.0f;
   const float c = sampled ? kLog2e / temp : 0.0f;
   const int first = part * p.stat_size, n = min(p.stat_size, p.vocab - first);
-  const T* x = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride + first;
-  RowStat r = wave_stat(thread_stat<T>(x, n, tid, kStatThreads, c, sampled), c, sampled);
-  if ((tid & 63) == 0) red[tid >> 6] = r;
-  __syncthreads();
-  if (tid != 0) return;
+  int node = chain ? further(0, j) : j;
+  while (node < len) {
+    RowStat r = wave_stat(thread_stat<T>(row0 + (size_t)node * p.row_stride + first, n, tid, kStatThreads, c, sampled), c, sampled);
+    if ((tid & 63) == 0) red[tid >> 6] = r;
+    __syncthreads();
+    if (tid == 0) {
 #pragma unroll
-  for (int w = 1; w < kStatThreads / 64; ++w) {
-    const RowStat o = red[w];
-    r.key = max(r.key, o.key);
-    const float top = fmaxf(r.m, o.m);
-    if (top > kNegInf) r.s = r.s * weight(r.m, top, c) + o.s * weight(o.m, top, c);
-    r.m = top;
+      for (int w = 1; w < kStatThreads / 64; ++w) {
+        const RowStat o = red[w];
+        r.key = max(r.key, o.key);
+        const float top = fmaxf(r.m, o.m);
+        if (top > kNegInf) r.s = r.s * weight(r.m, top, c) + o.s * weight(o.m, top, c);
+        r.m = top;
+      }
+      if (r.key != 0 && r.key != ~0ull) r.key -= first;      // ~(index + first)
+      workspace_of(p).stats[((size_t)b * p.nodes + node) * p.stat_parts + part] = r;
+    }
+    node = chain ? further(node, each) : len;
+    if (node < len) __syncthreads();                         // red: read
   }
-  if (r.key != 0 && r.key != ~0ull) r.key -= first;          // ~(index + first)
-  workspace_of(p).stats[(size_t)row * p.stat_parts + part] = r;
 }
 
 // A work-group per sequence.  STATS: the rows' parts are there.  NC: nodes of a lane.
@@ -596,19 +629,28 @@ template <typename T> __global__ void __launch_bounds__(kDrawThreads) verify_dra
 
 int stat_size(int dtype) { return kStatThreads * kStatVecs * 16 / (dtype == kF32 ? 4 : 2); }
 
-// Whether the rows of all nodes are read first: at 5.2 GB/ms, against seven steps of a walk, each 0.9 us and 36 ns for a KiB of
-// its row (paths are about so long; their lengths are known on the device only).  MI355X, us, all rows / walk, trees with
-// paths of up to 7 nodes: greedy, 32000 fp32 logits: 16 x 32 nodes 19 / 26, 64 x 16 27.5 / 29, 64 x 32 48 / 29; 128256 bf16:
-// 8 x 64 27 / 48, 64 x 16 50 / 72; sampled, 2 x 32 of 128256 bf16 31 / 74.
-bool all_rows(int num_seqs, int nodes, int vocab, int dtype) {
+// Whether rows are read first: at 5.2 GB/ms, against seven steps of a walk, each 0.9 us and 36 ns for a KiB of its row (paths
+// are about so long; their lengths are known on the device only).  Sampled, all rows; greedy, chains, of about eight nodes,
+// but at the worst of all.  MI355X, us, rows first / walk, trees with paths of up to 7 nodes: greedy, 32000 fp32 logits: 64 x 16
+// nodes 16 / 25, 64 x 64 15 / 29, 128 x 8 25 / 21, 256 x 16 32 / 35; 128256 bf16: 8 x 64 15 / 24, 64 x 16 27 / 38, 64 x 32 26 / 37;
+// sampled: 2 x 32 of 128256 bf16 27 / 74, 64 x 64 of 32000 fp32 107 / 57.
+bool all_rows(int num_seqs, int nodes, int vocab, int dtype, bool sampled) {
   const long long rows = (long long)num_seqs * nodes, row = (long long)vocab * (dtype == kF32 ? 4 : 2);
-  return rows <= 1 << 20 && rows * row / 5.2e6 + 4.0 <= 7.0 * (0.9 + row / 1024.0 * 0.036);
+  const double walk = 7.0 * (0.9 + row / 1024.0 * 0.036);
+  auto reading = [&](long long n) { return n * row / 5.2e6 + 4.0; };
+  if (rows > 1 << 20) return false;
+  return sampled ? reading(rows) <= walk : reading((long long)num_seqs * std::min(nodes, 8)) <= walk && reading(rows) <= 3 * walk;
+}
+
+int stat_parts(int num_seqs, int nodes, int vocab, int dtype, bool sampled) {
+  return all_rows(num_seqs, nodes, vocab, dtype, sampled) ? (vocab + stat_size(dtype) - 1) / stat_size(dtype) : 0;
 }
 
 void plan(VerifyParams& p, int dtype) {
   p.draw_chunks = (p.vocab + kDrawChunk - 1) / kDrawChunk;
   p.stat_size = stat_size(dtype);
-  p.stat_parts = all_rows(p.num_seqs, p.nodes, p.vocab, dtype) ? (p.vocab + p.stat_size - 1) / p.stat_size : 0;
+  p.stat_parts = stat_parts(p.num_seqs, p.nodes, p.vocab, dtype, p.temperatures != nullptr);
+  p.chain_rows = p.stat_parts && !p.temperatures ? std::min(p.nodes, kChainRows) : 0;
 }
 
 template <typename T, int NC> void launch_walk(const VerifyParams& p, hipStream_t s) {
@@ -617,8 +659,10 @@ template <typename T, int NC> void launch_walk(const VerifyParams& p, hipStream_
 }
 
 template <typename T> void launch_of(const VerifyParams& p, hipStream_t s) {
-  if (p.stat_parts)
-    hipLaunchKernelGGL(verify_stats_kernel<T>, dim3(p.num_seqs * p.nodes, p.stat_parts), dim3(kStatThreads), 0, s, p);
+  if (p.stat_parts) {
+    const dim3 grid(p.num_seqs * (p.chain_rows ? p.chain_rows : p.nodes), p.stat_parts);
+    hipLaunchKernelGGL(verify_stats_kernel<T>, grid, dim3(kStatThreads), 0, s, p);
+  }
   if (p.nodes <= 64) launch_walk<T, 1>(p, s);
   else if (p.nodes <= 128) launch_walk<T, 2>(p, s);
   else launch_walk<T, 4>(p, s);
@@ -636,7 +680,8 @@ size_t verify_workspace_bytes(int num_seqs, int nodes, int vocab, int dtype) {
   p.nodes = nodes;
   p.vocab = vocab;
   plan(p, dtype);
-  return reinterpret_cast<uintptr_t>(workspace_of(p).stats + (size_t)num_seqs * nodes * p.stat_parts);
+  const int parts = std::max(p.stat_parts, stat_parts(num_seqs, nodes, vocab, dtype, true));      // greedy or not
+  return reinterpret_cast<uintptr_t>(workspace_of(p).stats + (size_t)num_seqs * nodes * parts);
 }
 
 void launch_verify(VerifyParams p, int dtype, hipStream_t s) {

@@ -81,6 +81,7 @@ struct VerifyParams {
   void* workspace;
   int draw_chunks;           // of a row, for the draw
   int stat_size, stat_parts; // elements of a part, and parts, of a row that is read beforehand (0: none is)
+  int chain_rows;            // greedy: work-groups for the rows of a chain (0: all rows are read)
 };
 
 struct KeepParams {
