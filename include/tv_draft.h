@@ -79,7 +79,7 @@ int tv_rope_and_cache(void* q_out, void* k_cache, void* v_cache, const void* q, 
  * out [num_seqs, nodes, num_heads, head_dim] of dtype or TV_F32 (out_dtype).
  * head_dim 64, 128 or 256; any block size; any number of query heads per KV head.
  * work_groups: 0 gives every (sequence, KV head, tile of rows) a work-group.  n > 0 deals
- * the keys of all of them evenly to n work-groups by the lengths on the device, and joins what
+ * the keys of all of them evenly to n work-groups (as many for every KV head, one at least) by the lengths on the device, and joins what
  * that cuts through `workspace` (16-byte aligned, of tv_paged_tree_workspace_bytes bytes,
  * one per launch that may overlap); results then depend on the batch in their last digits.
  */
@@ -111,8 +111,9 @@ int tv_paged_tree(void* out, const void* queries, const void* k_cache, const voi
  * Of children with one token the first counts; a token outside [0, vocab) is never
  * taken.  A node whose logits have a NaN or no number above -inf (sampled: or +inf) ends
  * the path, and the next token is -1.
- * logits [num_seqs * nodes, vocab] of dtype at row_stride elements.  All sums are of fp32
- * exponentials, joined in fp64.  workspace: 16-byte aligned, one per launch that may overlap.
+ * logits [num_seqs * nodes, vocab] of dtype at row_stride elements.  Exponentials and sums are fp32
+ * where u is not next to a bound, and else, and for the draw, fp64.  workspace: 16-byte aligned, one per
+ * launch that may overlap.
  */
 size_t tv_verify_draft_tree_workspace_bytes(int num_seqs, int nodes, int vocab, int dtype);
 int tv_verify_draft_tree(int32_t* path, int32_t* counts, int32_t* next_tokens, const void* logits,
