@@ -69,11 +69,6 @@ template <int CPR> __device__ __forceinline__ int tree_perm(int r) {
   else return ((r & 7) << 1) | ((r >> 3) & 1);
 }
 
-// 16 bytes per lane from a lane's own address into LDS at lds_base + 16 * lane.
-__device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_base), "v"(p) : "memory", "m0");
-}
-
 // A row tile of a sequence: its lengths, and the tiles of its keys.
 struct TreeUnit { int b, rt, ctx, len, keys, tiles; };
 

@@ -20,9 +20,13 @@ template <int D> __device__ __forceinline__ int tile_chunk_perm(int r) {
 
 // 16 bytes per lane from buffer `rsrc` at byte offset voff straight into LDS at
 // lds_base + 16 * lane.  The compiler does not see these loads: callers retire
-// them with wait_vmcnt before the barrier that publishes the tile.
+// them with wait_vmcnt before the barrier that publishes the tile.  Nor does it
+// see what they have to be apart from: a load into LDS comes one wait state after
+// the write of M0 at least, and five after a vector instruction's write of a scalar
+// register that it reads (a descriptor word out of readfirstlane, or out of a spill).
+// The move and s_nop 3 are five, whatever stands before.
 __device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t lds_base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_base), "v"(voff), "s"(rsrc)
                : "memory", "m0");
@@ -30,10 +34,15 @@ __device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t lds_base, uint32
 
 // The same for lines that are read once (non-temporal).
 __device__ __forceinline__ void load_lds16_nt(u32x4 rsrc, uint32_t lds_base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                :
                : "s"(lds_base), "v"(voff), "s"(rsrc)
                : "memory", "m0");
+}
+
+// The same from a lane's own address.
+__device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_base), "v"(p) : "memory", "m0");
 }
 
 // Wait until at most N vector-memory operations of this wave are outstanding
