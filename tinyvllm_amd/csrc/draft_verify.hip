@@ -7,9 +7,15 @@
 // tokens, the first at which their e sum to more than u S - E, E the children's.
 //
 // Precision: whether u is below a sum needs fp32 only where u is not next to it: within
-// kUnsure of a child's bound the sums are taken again in fp64.  (fp32 sums are off by a
-// relative 2^-17 at most: a thread's 128 and more terms, each with the rounding of an
-// argument that matters, below 2^5.)  The draw is in fp64 throughout: a large
+// `unsure` of a child's bound the sums are taken again in fp64.  With h = 2^-24, half a step of
+// fp32, an fp32 sum of a row is off by less than a relative (107 + 11 rounds) h:
+//   67 h  arguments: (x - m) c has four roundings (with those of c), so e is off by 4 ln(2) |y| h, y
+//         its exponent; the maximum has e = 1, so of V terms the weighted mean of |y| is
+//         below log2(V) <= 24.  Raising a maximum in several steps adds up to the same |y|.
+//   40 h  sums in a vector, over lanes and over waves, with 3 h for each product by an exponential
+//   11 h  a round, of which `rounds` follow each other: kStatVecs vectors of a thread, or
+//         kPartsAtOnce parts of a row: eight additions and a raised maximum
+// unsure is more than twice that, 2^-16 + 2^-19 rounds.  The draw is in fp64 throughout: a large
 // vocabulary has a bound every 2^-17 of S, and an error of d in u S meets one with
 // probability 2^17 d.
 //
@@ -33,7 +39,6 @@ constexpr int kChainRows = 8;            // work-groups a part for a chain's row
 constexpr int kDrawThreads = 256;
 constexpr int kDrawPer = 8;              // elements a thread of the draw kernels
 constexpr int kDrawChunk = kDrawThreads * kDrawPer;
-constexpr double kUnsure = 0x1p-13;
 
 // What is known of a row, or of a part of it: the first maximum, and sum e relative to it.
 struct RowStat {
@@ -451,7 +456,7 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
         return found;
       };
       bool sure;
-      go = choose(S, kUnsure, sure);
+      go = choose(S, p.unsure, sure);
       if (!sure) {
         double part = 0.0;
         for (int i = tid; i < vocab; i += kThreads) part += weight64(to_float<T>(x[i]), M, c64);
@@ -651,6 +656,10 @@ void plan(VerifyParams& p, int dtype) {
   p.stat_size = stat_size(dtype);
   p.stat_parts = stat_parts(p.num_seqs, p.nodes, p.vocab, dtype, p.temperatures != nullptr);
   p.chain_rows = p.stat_parts && !p.temperatures ? std::min(p.nodes, kChainRows) : 0;
+  const int vecs = p.vocab / (dtype == kF32 ? 4 : 8);
+  const int rounds = p.stat_parts ? 1 + (p.stat_parts + kPartsAtOnce - 1) / kPartsAtOnce
+                                  : (vecs + kWalkThreads * kStatVecs - 1) / (kWalkThreads * kStatVecs);
+  p.unsure = 0x1p-16 + rounds * 0x1p-19;
 }
 
 template <typename T, int NC> void launch_walk(const VerifyParams& p, hipStream_t s) {

@@ -82,6 +82,7 @@ struct VerifyParams {
   int draw_chunks;           // of a row, for the draw
   int stat_size, stat_parts; // elements of a part, and parts, of a row that is read beforehand (0: none is)
   int chain_rows;            // greedy: work-groups for the rows of a chain (0: all rows are read)
+  double unsure;             // sampled: how near to a bound, of the row's sum, fp32 sums do not decide
 };
 
 struct KeepParams {
