@@ -19,6 +19,10 @@
 // vocabulary has a bound every 2^-17 of S, and an error of d in u S meets one with
 // probability 2^17 d.
 //
+// A sum in fp64 is bound by one CU's fp64 units.  MI355X, us of a captured call, ordinary / with u of one sequence on a bound: 2 x 32
+// nodes of 128256 logits in bf16 34 / 64, 64 x 16 of them 86 / 120, 64 x 64 of 32000 in fp32 41 / 49, 1 x 4 of 2^20 in fp32
+// 41 / 337.
+//
 // A walk over a path is serial and reads its rows only; reading the rows that it may come to
 // first is parallel (all_rows): bound by HBM, then by the latency of the walk and the draw, a work-group a sequence.
 // MI355X: greedy, 64 sequences of 16 nodes, 32000 fp32 logits: chains' rows 13 us, walk 4; sampled, 2 of 32, 128256 in
@@ -198,6 +202,43 @@ __device__ __forceinline__ ThreadStat thread_stat(const T* x, int n, int tid, in
   return ThreadStat{m, s, idx};
 }
 
+// One thread's share of the sum of e in fp64, of the same vectors and elements.  Vectors are on the way four at a time, and
+// their exponentials do not wait for each other (an element at a time, with 64 threads for rows read first: 417 us where a
+// call now takes 64).
+template <typename T>
+__device__ __forceinline__ double thread_sum64(const T* x, int n, int tid, int threads, float m, double c) {
+  constexpr int EPV = 16 / (int)sizeof(T);
+  constexpr int U = 4;
+  const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+  const int vecs = (n - head) / EPV;
+  const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
+  const int tail = head + vecs * EPV + tid;
+  double sum = tid < head ? weight64(to_float<T>(x[tid]), m, c) : 0.0;
+  if (tail < n) sum += weight64(to_float<T>(x[tail]), m, c);
+  for (int v0 = tid; v0 < vecs; v0 += threads * U) {
+    u32x4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = body[min(v0 + u * threads, vecs - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v0 + u * threads >= vecs) break;
+      double e = 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          e += weight64(u32_as_f32(w[u][i]), m, c);
+        } else {
+          float a, b;
+          unpack2<T>(w[u][i], a, b);
+          e += weight64(a, m, c) + weight64(b, m, c);
+        }
+      }
+      sum += e;
+    }
+  }
+  return sum;
+}
+
 // The wave's shares as one, in every lane.
 __device__ __forceinline__ RowStat wave_stat(const ThreadStat& t, float c, bool sampled) {
   RowStat r{0, group_max<64>(t.m), 0.0f};                    // (of a NaN nothing is used)
@@ -307,10 +348,10 @@ template <typename T> __global__ void __launch_bounds__(kStatThreads) verify_sta
   }
 }
 
-// A work-group per sequence.  STATS: the rows' parts are there.  NC: nodes of a lane.
+// A work-group per sequence.  STATS: the rows' parts are there (64 threads do for these, but not for a sum in fp64).  NC: nodes of a lane.
 template <typename T, bool STATS, int NC>
-__global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(const VerifyParams p) {
-  constexpr int kThreads = STATS ? 64 : kWalkThreads;
+__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const VerifyParams p) {
+  constexpr int kThreads = kWalkThreads;
   constexpr int kWaves = kThreads / 64;
   __shared__ int tokens[kDraftMaxNodes], parents[kDraftMaxNodes];
   __shared__ float logits[kDraftMaxNodes];                   // of a node's token after its parent
@@ -458,9 +499,7 @@ __global__ void __launch_bounds__(STATS ? 64 : kWalkThreads) verify_walk_kernel(
       bool sure;
       go = choose(S, p.unsure, sure);
       if (!sure) {
-        double part = 0.0;
-        for (int i = tid; i < vocab; i += kThreads) part += weight64(to_float<T>(x[i]), M, c64);
-        part = wave_sum(part);
+        const double part = wave_sum(thread_sum64<T>(x, vocab, tid, kThreads, M, c64));
         if (lane == 0) red_d[wave] = part;
         __syncthreads();
         S = 0.0;
@@ -663,7 +702,7 @@ void plan(VerifyParams& p, int dtype) {
 }
 
 template <typename T, int NC> void launch_walk(const VerifyParams& p, hipStream_t s) {
-  if (p.stat_parts) hipLaunchKernelGGL((verify_walk_kernel<T, true, NC>), dim3(p.num_seqs), dim3(64), 0, s, p);
+  if (p.stat_parts) hipLaunchKernelGGL((verify_walk_kernel<T, true, NC>), dim3(p.num_seqs), dim3(kWalkThreads), 0, s, p);
   else hipLaunchKernelGGL((verify_walk_kernel<T, false, NC>), dim3(p.num_seqs), dim3(kWalkThreads), 0, s, p);
 }
 
