@@ -387,7 +387,7 @@ class PagedTreePlan:
     counterpart), checked once and pointer-stable: ``run()`` is one C call without an allocation, which a HIP graph
     can capture.
 
-    queries [B, T, Hq, D], rotated, any strides between sequences and nodes; k_cache / v_cache [NB, bs, Hkv, D] of
+    queries [B, T, Hq, D], rotated, sequences and nodes multiples of 16 bytes apart; k_cache / v_cache [NB, bs, Hkv, D] of
     their dtype, the nodes' own K/V at positions context + i; block_tables [B, columns], context_lens [B] (tokens before
     the tree) and tree_lens [B] int32; tree_mask [B, T, ceil(T / 64)] int64 as ``draft_tree.draft_tree_layout`` makes
     it, or [T, ceil(T / 64)] for one shape of tree.  Node i attends all context tokens and the nodes t < tree_lens

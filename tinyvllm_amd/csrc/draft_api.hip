@@ -164,7 +164,7 @@ int tv_paged_tree_work_groups(int num_seqs, int nodes, int num_heads, int num_kv
   const long long tiles = ((long long)max_blocks * block_size + shape.tile_keys - 1) / shape.tile_keys;
   // In tiles that a work-group takes one after the other: undealt, its rounds of whole units; dealt, its share and
   // what dealing and joining cost (8 us).  Long units are dealt in any case: their lengths are rarely equal, and few of them end a
-  // launch on a few CUs.  MI355X, us, undealt / dealt, 32 / 8 heads of 128 in fp16: 16 x 8 nodes over 100..500 tokens 15 / 17,
+  // launch on a few CUs; a batch that fills the card gains nothing by it.  MI355X, us, undealt / dealt, 32 / 8 heads of 128 in fp16: 16 x 8 nodes over 100..500 tokens 15 / 17,
   // over 500..2000 44 / 26; 64 x 8 over 500..1000 41 / 48; 64 x 16 over 512..4096 126 / 125; 256 x 4 over 500..2000
   // 244 / 245, over 512..4096 444 / 430; 32 / 4 heads of 64: 64 x 8 over 200..1000 18 / 21, 1 x 32 over 1000 23 / 15,
   // 1 x 64 over 8000 125 / 25; in fp32 4 x 8 over 17..250 16 / 11.

@@ -25,8 +25,8 @@
 //
 // A walk over a path is serial and reads its rows only; reading the rows that it may come to
 // first is parallel (all_rows): bound by HBM, then by the latency of the walk and the draw, a work-group a sequence.
-// MI355X: greedy, 64 sequences of 16 nodes, 32000 fp32 logits: chains' rows 13 us, walk 4; sampled, 2 of 32, 128256 in
-// bf16: rows 7.3, walk 6.3, rest 4.6, draw 8.6.
+// MI355X: greedy, 64 sequences of 16 nodes, 32000 fp32 logits: chains' rows 12 us, walk 4; sampled, 2 of 32, 128256 in
+// bf16: rows 8.3, walk 6.9, rest 4.5, draw 8.7.
 #include "tv_draft.h"
 
 #include <algorithm>
@@ -678,6 +678,11 @@ int stat_size(int dtype) { return kStatThreads * kStatVecs * 16 / (dtype == kF32
 // but at the worst of all.  MI355X, us, rows first / walk, trees with paths of up to 7 nodes: greedy, 32000 fp32 logits: 64 x 16
 // nodes 16 / 25, 64 x 64 15 / 29, 128 x 8 25 / 21, 256 x 16 32 / 35; 128256 bf16: 8 x 64 15 / 24, 64 x 16 27 / 38, 64 x 32 26 / 37;
 // sampled: 2 x 32 of 128256 bf16 27 / 74, 64 x 64 of 32000 fp32 107 / 57.
+// Shorter paths make a walk shorter and leave the rows as they are.  A path without branches, us, rows first / walk, for 1, 3, 7
+// and all drafted tokens accepted: greedy, 32000 fp32: 1 x 8 7 / 7, 7 / 11, 8 / 20; 16 x 32 20 / 7, 20 / 12, 21 / 21, 26 / 104;
+// 1 x 64 22 / 7, 23 / 11, 24 / 20, 37 / 197; 1 x 256 83 / 7, 83 / 12, 85 / 23, 207 / 819; 64 x 16 26 / 9, 27 / 15, 27 / 30, 29 / 55;
+// 128256 bf16: 1 x 32 13 / 11, 14 / 19, 15 / 37, 20 / 155; 16 x 256 235 / 11, 234 / 21, 236 / 41, 352 / 1650; sampled, 128256
+// bf16: 1 x 32 21 / 35, 22 / 56, 25 / 96, 39 / 365; 64 x 16 78 / 50, 79 / 71, 81 / 116, 87 / 204.
 bool all_rows(int num_seqs, int nodes, int vocab, int dtype, bool sampled) {
   const long long rows = (long long)num_seqs * nodes, row = (long long)vocab * (dtype == kF32 ? 4 : 2);
   const double walk = 7.0 * (0.9 + row / 1024.0 * 0.036);

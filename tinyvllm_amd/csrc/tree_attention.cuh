@@ -18,14 +18,16 @@
 // Tiles come by LDS DMA, one that is read and one on the way: loads into registers made a wave wait for all of them
 // wherever it reused one.  Work is dealt by the lengths on the device (work_groups): what a launch of whole units takes
 // is its longest unit's time.  MI355X, kernel and merge, us; GB/s and TFLOP/s of the keys and products that cannot be left out:
-//   64 sequences x 16 nodes over 512..4096 tokens, 32 / 8 heads of 128, fp16       117 +  9   4.7 TB/s   bound by HBM
-//   2 x 32 over 31000..32700, 32 / 8 of 128, bf16                                   55 +  9   4.2 TB/s   HBM
-//   32 x 61 over 1000..6000, 32 / 4 of 64, bf16                                     86 + 10   450 TFLOP/s
+//   64 sequences x 16 nodes over 512..4096 tokens, 32 / 8 heads of 128, fp16       117 +  9   4.7 TB/s   loads
+//   2 x 32 over 31000..32700, 32 / 8 of 128, bf16                                   55 +  9   4.2 TB/s   loads
+//   32 x 61 over 1000..6000, 32 / 4 of 64, bf16                                     87 + 10   470 TFLOP/s
 //   16 x 32 over 2000, 32 / 8 of 128, fp32                                         166        103 TFLOP/s   matrix units
-// (a large copy reaches 5.2 TB/s, a large product 1140 TFLOP/s, 153 in fp32).  In the third the matrix units are busy for
+// (a large read reaches 7.0 TB/s, a large product 1140 TFLOP/s, 153 in fp32).  One tile on the way, drained before the next is
+// requested, is what bounds the first two: the loads alone take 113 and 50 us, 5.1 and 5.3 TB/s.  In the third the matrix units are busy for
 // 27% of the cycles and the vector units for 42%: a head of 64 has 128 products a weight, and its exponential, scaling,
 // maximum and conversion cost more cycles than those; its four row tiles read 382 MB past the L2 caches, since
-// they are at different keys at a time.  Without loads it takes 74 us, without the softmax 70, with loads alone 65.
+// they are at different keys at a time.  Without loads it takes 74 us, without the softmax 70, with loads alone 65.  Its
+// instance (heads of 64, 32 rows a wave) spills 14 vector registers, used where a unit begins and ends.
 #pragma once
 
 #include "tv_device_cache.h"
